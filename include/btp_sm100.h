@@ -196,6 +196,42 @@ int btp_sm100_decode_step(const void* a_t, const void* x_t, const void* c_t, con
 int btp_sm100_prefill_state(const void* a, const void* x, void* h_loc, void* r_pref, void* c_prev_loc, long long n_heads,
                             int L, int gate_is_log, int dtype, int gate_dtype, void* stream);
 
+/*
+ * Root-mean-square norm of rows, with the residual's addition:  h = x + residual,  y = h * rsqrt(mean(h^2) + eps) * weight.
+ * No counterpart in the reference.  Any alignment and any row pitch >= dim is taken (aligned rows are faster);
+ * dim <= 16384.  The norm is taken of the unrounded sum.
+ *   x         [rows, dim]   dtype: BTP_DTYPE_BF16 | BTP_DTYPE_F16 | BTP_DTYPE_F32, row pitch ld_x elements
+ *   residual  [rows, dim]   residual_dtype: x's type | BTP_DTYPE_F32, row pitch ld_r; NULL: none (h is then not written)
+ *   weight    [dim]         weight_dtype: x's type | BTP_DTYPE_F32; NULL: ones
+ *   h         [rows, dim]   residual's type, dense
+ *   rstd      [rows]        float, rsqrt(mean(h^2) + eps) for the backward, or NULL
+ *   out_mode  BTP_NORM_SAME    y [rows, dim] in x's type, dense; scale may be NULL
+ *             BTP_NORM_ROW8    y [rows, dim] e4m3 bytes, scale [rows] float: max|y| / 448 of the row
+ *             BTP_NORM_BLOCK8  y [rows, dim] e4m3 bytes, scale [rows, ceil(dim/128)]: the same per 128 columns
+ *             The stored byte is e4m3(y / scale), rounded to nearest even; the scale is 1 where the maximum is 0 or NaN.
+ */
+#define BTP_NORM_SAME 0
+#define BTP_NORM_ROW8 1
+#define BTP_NORM_BLOCK8 2
+int btp_sm100_rms_norm_forward(const void* x, const void* residual, const void* weight, void* y, void* h, float* rstd,
+                               float* scale, long long rows, int dim, long long ld_x, long long ld_r, float eps, int dtype,
+                               int residual_dtype, int weight_dtype, int out_mode, void* stream);
+
+/* Rows of the scratch that btp_sm100_rms_norm_backward takes for the weight's gradient (a status code if negative). */
+int btp_sm100_rms_norm_partial_rows(long long rows, int dim);
+
+/*
+ * Backward of btp_sm100_rms_norm_forward (BTP_NORM_SAME).
+ *   h, rstd    as the forward left them; without a residual h is x.  h has residual_dtype and row pitch ld_h
+ *   dy         [rows, dim] x's type, dense;   dh  [rows, dim] residual's type, dense, or NULL: gradient of h
+ *   dx         [rows, dim] x's type, or NULL;   dresidual  [rows, dim] residual's type, or NULL (the same values)
+ *   dweight    [dim] weight's type, or NULL;  partial  [btp_sm100_rms_norm_partial_rows(rows, dim), dim] float scratch
+ * Sums are taken in a fixed order: the same call gives the same bits.
+ */
+int btp_sm100_rms_norm_backward(const void* h, const void* weight, const void* dy, const void* dh, const float* rstd, void* dx,
+                                void* dresidual, void* dweight, float* partial, long long rows, int dim, long long ld_h,
+                                int dtype, int residual_dtype, int weight_dtype, void* stream);
+
 /* Name of a status code ("BTP_OK", "BTP_ERR_BAD_SHAPE", ...).  Never NULL. */
 const char* btp_sm100_status_string(int status);
 

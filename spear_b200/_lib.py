@@ -27,7 +27,7 @@ SEAM_HANDOFF = 1    # forward: the carry is handed over through distributed shar
 ABI_VERSION = 4
 
 # every symbol include/btp_sm100.h declares: name -> (restype, argtypes)
-_vp, _i, _ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
+_vp, _i, _ll, _f = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
 SYMBOLS = {
     "btp_sm100_forward": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
     "btp_sm100_backward": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
@@ -36,6 +36,9 @@ SYMBOLS = {
     "btp_sm100_gated_backward": (_i, [_vp] * 9 + [_i, _i, _i, _i] + [_ll] * 9 + [_i, _vp]),
     "btp_sm100_decode_step": (_i, [_vp] * 11 + [_ll, _i, _i, _i, _i, _i, _vp]),
     "btp_sm100_prefill_state": (_i, [_vp] * 5 + [_ll, _i, _i, _i, _i, _vp]),
+    "btp_sm100_rms_norm_forward": (_i, [_vp] * 7 + [_ll, _i, _ll, _ll, _f, _i, _i, _i, _i, _vp]),
+    "btp_sm100_rms_norm_partial_rows": (_i, [_ll, _i]),
+    "btp_sm100_rms_norm_backward": (_i, [_vp] * 9 + [_ll, _i, _ll, _i, _i, _i, _vp]),
     "btp_sm100_noalloc_read_record": (_i, [_vp, _ll, _vp]),
     "btp_sm100_set_wait_limit": (ctypes.c_ulonglong, [ctypes.c_ulonglong]),
     "btp_sm100_set_seam_mode": (_i, [_i]),

@@ -1,0 +1,70 @@
+// Storage types of the token-major operators (scan, convolution, norm): conversion to and from float, and loads and
+// stores of runs of consecutive elements that fall back to single elements where a row is not aligned or ends.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace btp_elem {
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+
+template <class T>
+__device__ __forceinline__ T from_f(float v);
+template <>
+__device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+
+// N consecutive elements as whole 16-byte (or smaller) words.
+template <class T, int N>
+struct alignas(sizeof(T) * N >= 16 ? 16 : sizeof(T) * N) Pack {
+  T v[N];
+};
+
+// out[0..N) = p[0..N) as floats; elements from `count` on are 0 and are not read.  `aligned`: p is a multiple of the
+// pack's size (16 bytes at most) and all N elements may be read.
+template <class T, int N>
+__device__ __forceinline__ void load_run(float (&out)[N], const T* p, bool aligned, int count) {
+  if (aligned) {
+    const Pack<T, N> w = *reinterpret_cast<const Pack<T, N>*>(p);
+#pragma unroll
+    for (int i = 0; i < N; ++i) out[i] = to_f(w.v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) out[i] = i < count ? to_f(p[i]) : 0.f;
+  }
+}
+
+template <class T, int N>
+__device__ __forceinline__ void store_run(T* p, const float (&in)[N], bool aligned, int count) {
+  if (aligned) {
+    Pack<T, N> w;
+#pragma unroll
+    for (int i = 0; i < N; ++i) w.v[i] = from_f<T>(in[i]);
+    *reinterpret_cast<Pack<T, N>*>(p) = w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < count) p[i] = from_f<T>(in[i]);
+  }
+}
+
+// A parameter vector that is stored in the activations' type or in float.
+template <class T, int N>
+__device__ __forceinline__ void load_param(float (&out)[N], const void* base, long long at, bool is_f32, bool aligned, int count) {
+  if (is_f32)
+    load_run<float, N>(out, static_cast<const float*>(base) + at, aligned, count);
+  else
+    load_run<T, N>(out, static_cast<const T*>(base) + at, aligned, count);
+}
+
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+}  // namespace btp_elem

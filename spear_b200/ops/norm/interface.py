@@ -1,0 +1,188 @@
+"""``rms_norm`` and ``rms_norm_8bit`` on the sm_100a kernels.
+
+    h = x + residual            y = h * rsqrt(mean(h^2) + eps) * weight
+
+One pass over the row: the sum, its norm and the output (in 8 bits: with its scale) come from registers.  The
+residual stream may be float32 next to 16-bit activations.  CUDA only, no fallback.
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from ..btp import interface as _iface
+from .. import _call
+
+__all__ = ["rms_norm", "rms_norm_8bit", "F8_MAX", "SCALE_BLOCK", "MAX_DIM"]
+
+F8_MAX = 448.0     # largest e4m3 magnitude
+SCALE_BLOCK = 128  # columns that share a scale in the blockwise form
+MAX_DIM = 16384
+_OUT = {None: 1, SCALE_BLOCK: 2}
+
+
+def _check(what, x, weight, residual, eps) -> int:
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_DIM:
+        raise ValueError(f"{what}: x must be [..., D] with 1 <= D <= {MAX_DIM}, got {tuple(x.shape)}")
+    _call.activation(x, f"{what}: x")
+    if weight is not None:
+        if tuple(weight.shape) != (x.shape[-1],):
+            raise ValueError(f"{what}: weight must be [{x.shape[-1]}], got {tuple(weight.shape)}")
+        if weight.dtype != x.dtype and weight.dtype != torch.float32:
+            raise RuntimeError(f"{what}: weight must have x's dtype ({x.dtype}) or be float32 (got {weight.dtype})")
+    if residual is not None:
+        if residual.shape != x.shape:
+            raise ValueError(f"{what}: residual must have x's shape {tuple(x.shape)}, got {tuple(residual.shape)}")
+        if residual.dtype != x.dtype and residual.dtype != torch.float32:
+            raise RuntimeError(f"{what}: residual must have x's dtype ({x.dtype}) or be float32 (got {residual.dtype})")
+    if not eps >= 0.0:
+        raise ValueError(f"{what}: eps must not be negative (got {eps})")
+    return _call.on_gpu(what, x, weight, residual)
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """t as [rows, D] with dense rows at one pitch; copied only where its strides allow no such view."""
+    d = t.shape[-1]
+    r = t.reshape(-1, d)
+    if (d > 1 and r.stride(1) != 1) or (r.shape[0] > 1 and r.stride(0) < d):
+        r = r.contiguous()
+    return r
+
+
+def _pitch(r: torch.Tensor) -> int:
+    return r.stride(0) if r.shape[0] > 1 else r.shape[1]
+
+
+def _launch_forward(x, residual, weight, y, h, rstd, scale, eps, mode) -> None:
+    rows, dim = x.shape
+    if rows == 0:
+        return
+    _call.call("btp_sm100_rms_norm_forward", x.device.index, x.data_ptr(), _call.ptr(residual), _call.ptr(weight), y.data_ptr(),
+               _call.ptr(h), _call.ptr(rstd), _call.ptr(scale), rows, dim, _pitch(x), dim if residual is None else _pitch(residual),
+               eps, _call.TAG[x.dtype], 0 if residual is None else _call.TAG[residual.dtype],
+               0 if weight is None else _call.TAG[weight.dtype], mode)
+
+
+def _op_forward(x: torch.Tensor, residual: Optional[torch.Tensor], weight: Optional[torch.Tensor], y: torch.Tensor,
+                h: Optional[torch.Tensor], rstd: torch.Tensor, eps: float) -> None:
+    _launch_forward(x, residual, weight, y, h, rstd, None, eps, 0)
+
+
+def _op_backward(h: torch.Tensor, weight: Optional[torch.Tensor], dy: torch.Tensor, dh: Optional[torch.Tensor], rstd: torch.Tensor,
+                 dx: Optional[torch.Tensor], dresidual: Optional[torch.Tensor], dweight: Optional[torch.Tensor]) -> None:
+    rows, dim = h.shape
+    if rows == 0:
+        if dweight is not None:
+            dweight.zero_()
+        return
+    index = h.device.index
+    partial = None
+    if dweight is not None:
+        parts = _call.query("btp_sm100_rms_norm_partial_rows", index, rows, dim)
+        partial = torch.empty(parts, dim, device=h.device, dtype=torch.float32)
+    _call.call("btp_sm100_rms_norm_backward", index, h.data_ptr(), _call.ptr(weight), dy.data_ptr(), _call.ptr(dh), rstd.data_ptr(),
+               _call.ptr(dx), _call.ptr(dresidual), _call.ptr(dweight), _call.ptr(partial), rows, dim, _pitch(h),
+               _call.TAG[dy.dtype], _call.TAG[h.dtype], 0 if weight is None else _call.TAG[weight.dtype])
+
+
+def _fake(*args) -> None:
+    return None
+
+
+_iface._register(_iface._LIB, "spear_btp", "rms_norm_forward", _op_forward, _fake, ["y", "h", "rstd"])
+_iface._register(_iface._LIB, "spear_btp", "rms_norm_backward", _op_backward, _fake, ["dx", "dresidual", "dweight"])
+
+
+class _RMSNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        x2 = _rows(x)
+        r2 = None if residual is None else _rows(residual)
+        y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        h = None if residual is None else torch.empty(x.shape, device=x.device, dtype=residual.dtype)
+        rstd = torch.empty(x2.shape[0], device=x.device, dtype=torch.float32)
+        d = x.shape[-1]
+        torch.ops.spear_btp.rms_norm_forward(x2, r2, weight, y.view(-1, d), None if h is None else h.view(-1, d), rstd, eps)
+        ctx.save_for_backward(x2 if h is None else h, weight, rstd)
+        ctx.has_residual = h is not None
+        ctx.dtype = x.dtype
+        ctx.set_materialize_grads(False)
+        return y if h is None else (y, h)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh=None):
+        h, weight, rstd = ctx.saved_tensors
+        need_x, need_w, need_r = ctx.needs_input_grad[:3]
+        if dy is None:  # y was not used: the sum passes its gradient on
+            dx = dh.to(ctx.dtype) if dh is not None and need_x else None
+            return dx, None, dh if need_r else None, None
+        shape, d = dy.shape, dy.shape[-1]
+        dy2 = dy.reshape(-1, d).contiguous()
+        h2 = _rows(h)
+        dh2 = None if dh is None else dh.reshape(-1, d).contiguous()
+        one = h.dtype == ctx.dtype  # one tensor serves as the gradient of both terms of the sum
+        dx = torch.empty(shape, device=dy.device, dtype=ctx.dtype) if need_x or (one and need_r) else None
+        dres = torch.empty(shape, device=dy.device, dtype=h.dtype) if need_r and not one else None
+        dw = torch.empty_like(weight, memory_format=torch.contiguous_format) if need_w and weight is not None else None
+        if dx is not None or dres is not None or dw is not None:
+            torch.ops.spear_btp.rms_norm_backward(h2, weight, dy2, dh2, rstd, None if dx is None else dx.view(-1, d),
+                                                  None if dres is None else dres.view(-1, d), dw)
+        return dx if need_x else None, dw, (dx if one else dres) if need_r else None, None
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, residual: torch.Tensor | None = None, *, eps: float = 1e-6):
+    """Root-mean-square norm over the last dimension, with the residual's addition.
+
+    Args:
+        x: [..., D] bfloat16, float16 or float32, D <= 16384; the last dimension is copied to be dense if it is not.
+        weight: [D] in x's dtype or float32, or None for ones.
+        residual: [..., D] in x's dtype or float32 (a residual stream kept in 32 bits), or None.
+        eps: added to the mean square.
+    Returns:
+        y [..., D] in x's dtype; with a residual (y, h) where h = x + residual in the residual's dtype.  y is the
+        norm of the sum before that rounding.  Both outputs have gradients.
+    """
+    index = _check("rms_norm", x, weight, residual, eps)
+    weight = weight if weight is None or weight.is_contiguous() else weight.contiguous()
+    if torch.compiler.is_compiling() or (torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in (x, weight, residual))):
+        return _RMSNorm.apply(x, weight, residual, float(eps))
+    d = x.shape[-1]
+    x2 = _rows(x)
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    if residual is None:
+        _launch_forward(x2, None, weight, y.view(-1, d), None, None, None, float(eps), 0)
+        return y
+    h = torch.empty(x.shape, device=x.device, dtype=residual.dtype)
+    _launch_forward(x2, _rows(residual), weight, y.view(-1, d), h.view(-1, d), None, None, float(eps), 0)
+    return y, h
+
+
+@torch.no_grad()
+def rms_norm_8bit(x: torch.Tensor, weight: torch.Tensor | None = None, residual: torch.Tensor | None = None, *,
+                  eps: float = 1e-6, block: int | None = None):
+    """rms_norm whose output is e4m3 with float32 scales, the operand of an 8-bit product.  No gradient.
+
+    Args:
+        x, weight, residual, eps: as for ``rms_norm``.
+        block: None for one scale per row, 128 for one scale per 128 columns (the last may hold fewer).
+    Returns:
+        (q, scale) or, with a residual, (q, scale, h): q [..., D] float8_e4m3fn, scale [...] or
+        [..., ceil(D / 128)] with y = q * scale; scale = max|y| / 448, or 1 where that maximum is 0 or NaN.
+    """
+    if block not in _OUT:
+        raise ValueError(f"rms_norm_8bit: block must be None or {SCALE_BLOCK} (got {block})")
+    _check("rms_norm_8bit", x, weight, residual, eps)
+    weight = weight if weight is None or weight.is_contiguous() else weight.contiguous()
+    d = x.shape[-1]
+    x2 = _rows(x)
+    q = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn)
+    scale = torch.empty(x.shape[:-1] if block is None else (*x.shape[:-1], -(-d // SCALE_BLOCK)), device=x.device, dtype=torch.float32)
+    h = None if residual is None else torch.empty(x.shape, device=x.device, dtype=residual.dtype)
+    _launch_forward(x2, None if residual is None else _rows(residual), weight, q.view(-1, d), None if h is None else h.view(-1, d),
+                    None, scale, float(eps), _OUT[block])
+    return (q, scale) if h is None else (q, scale, h)
