@@ -232,6 +232,43 @@ int btp_sm100_rms_norm_backward(const void* h, const void* weight, const void* d
                                 void* dresidual, void* dweight, float* partial, long long rows, int dim, long long ld_h,
                                 int dtype, int residual_dtype, int weight_dtype, void* stream);
 
+/*
+ * Short causal convolution over tokens, one filter per channel, token-major.  No counterpart in the reference.
+ *   pre[b,t,d] = bias[d] + sum_w weight[d,w] xx[b, t-(width-1)+w, d],   y = pre or (silu) pre * sigmoid(pre)
+ *   x        [B, L, dim]  dtype: BTP_DTYPE_BF16 | BTP_DTYPE_F16 | BTP_DTYPE_F32; the element at (b, t, d) lies at
+ *                         b * sx_b + t * sx_t + d; any alignment (16-byte aligned rows are faster)
+ *   weight   [dim, width], bias [dim] (NULL: zeros)   weight_dtype: x's type | BTP_DTYPE_F32;  width 2, 3 or 4
+ *   initial  [B, width-1, dim] x's type, dense: the inputs before token 0, oldest first; NULL: zeros
+ *   lengths  [B] int32 on the device, or NULL: tokens of sequence b from lengths[b] on are not read, y is 0 there
+ *            (values are held to 0 ... L)
+ *   y        [B, L, dim] dense;   state  [B, width-1, dim] dense, or NULL: the inputs before each sequence's end
+ */
+int btp_sm100_causal_conv_forward(const void* x, const void* weight, const void* bias, const void* initial, const int* lengths,
+                                  void* y, void* state, int B, int L, int dim, int width, long long sx_b, long long sx_t, int silu,
+                                  int dtype, int weight_dtype, void* stream);
+
+/* Rows of width + 1 times dim floats of the scratch that the convolution's backward takes (a status code if negative). */
+int btp_sm100_causal_conv_partial_rows(int B, int L, int dim);
+
+/*
+ * Backward of btp_sm100_causal_conv_forward, for gradients dy of y and dstate of state (NULL: none).
+ *   dy, dx [B, L, dim] x's type, dense (dx is 0 from lengths[b] on);  dstate, dinitial [B, width-1, dim] x's type, dense
+ *   dweight [dim, width], dbias [dim] weight's type, either NULL; partial: scratch of
+ *   btp_sm100_causal_conv_partial_rows(B, L, dim) * (width + 1) * dim floats, needed for either of the two.
+ * Sums are taken in a fixed order.
+ */
+int btp_sm100_causal_conv_backward(const void* x, const void* weight, const void* bias, const void* initial, const int* lengths,
+                                   const void* dy, const void* dstate, void* dx, void* dweight, void* dbias, void* dinitial,
+                                   float* partial, int B, int L, int dim, int width, long long sx_b, long long sx_t, int silu,
+                                   int dtype, int weight_dtype, void* stream);
+
+/*
+ * One token of the same convolution: x, y [B, dim] (x with row pitch ld_x), state and state_out [B, width-1, dim]
+ * dense.  state_out may be state itself (an update in place); any other overlap is an error of the caller's.
+ */
+int btp_sm100_causal_conv_step(const void* x, const void* state, const void* weight, const void* bias, void* y, void* state_out,
+                               int B, int dim, int width, long long ld_x, int silu, int dtype, int weight_dtype, void* stream);
+
 /* Name of a status code ("BTP_OK", "BTP_ERR_BAD_SHAPE", ...).  Never NULL. */
 const char* btp_sm100_status_string(int status);
 

@@ -39,6 +39,10 @@ SYMBOLS = {
     "btp_sm100_rms_norm_forward": (_i, [_vp] * 7 + [_ll, _i, _ll, _ll, _f, _i, _i, _i, _i, _vp]),
     "btp_sm100_rms_norm_partial_rows": (_i, [_ll, _i]),
     "btp_sm100_rms_norm_backward": (_i, [_vp] * 9 + [_ll, _i, _ll, _i, _i, _i, _vp]),
+    "btp_sm100_causal_conv_forward": (_i, [_vp] * 7 + [_i] * 4 + [_ll, _ll, _i, _i, _i, _vp]),
+    "btp_sm100_causal_conv_partial_rows": (_i, [_i] * 3),
+    "btp_sm100_causal_conv_backward": (_i, [_vp] * 12 + [_i] * 4 + [_ll, _ll, _i, _i, _i, _vp]),
+    "btp_sm100_causal_conv_step": (_i, [_vp] * 6 + [_i] * 3 + [_ll, _i, _i, _i, _vp]),
     "btp_sm100_noalloc_read_record": (_i, [_vp, _ll, _vp]),
     "btp_sm100_set_wait_limit": (ctypes.c_ulonglong, [ctypes.c_ulonglong]),
     "btp_sm100_set_seam_mode": (_i, [_i]),

@@ -24,7 +24,7 @@ __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_
 
 // N consecutive elements as whole 16-byte (or smaller) words.
 template <class T, int N>
-struct alignas(sizeof(T) * N >= 16 ? 16 : sizeof(T) * N) Pack {
+struct alignas((N & (N - 1)) != 0 ? sizeof(T) : sizeof(T) * N >= 16 ? 16 : sizeof(T) * N) Pack {
   T v[N];
 };
 
@@ -63,6 +63,28 @@ __device__ __forceinline__ void load_param(float (&out)[N], const void* base, lo
     load_run<float, N>(out, static_cast<const float*>(base) + at, aligned, count);
   else
     load_run<T, N>(out, static_cast<const T*>(base) + at, aligned, count);
+}
+
+// 2^v, 1/v on the special-function unit (2 and 1 units in the last place).
+__device__ __forceinline__ float ex2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float rcp(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+// 1 / (1 + e^-v); the exponent's rounding makes it |v| 2^-24 off relative for very negative v, a few 2^-24 elsewhere.
+__device__ __forceinline__ float sigmoid(float v) { return rcp(1.f + ex2(-v * kLog2e)); }
+
+// Tokens of sequence b that are there: `lengths` may be null (all L), its values are held to 0 ... L.
+__device__ __forceinline__ int tokens_of(const int* lengths, long long b, int L) {
+  if (!lengths) return L;
+  const int n = lengths[b];
+  return n < 0 ? 0 : (n < L ? n : L);
 }
 
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }

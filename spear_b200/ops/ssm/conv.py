@@ -1,0 +1,211 @@
+"""``causal_conv`` and ``causal_conv_step``: a short convolution over tokens, one filter per channel.
+
+    pre[b, t, d] = bias[d] + sum_w weight[d, w] * x[b, t - (W - 1) + w, d]        y = pre, or silu(pre)
+
+Token-major, [batch, length, channels], as a projection leaves its output (a column slice of a wider one is read in
+place).  CUDA only, no fallback.
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from ..btp import interface as _iface
+from .. import _call
+
+__all__ = ["causal_conv", "causal_conv_step"]
+
+WIDTHS = (2, 3, 4)
+
+
+def _check_filter(what, dim, dtype, weight, bias, activation) -> int:
+    if weight.dim() != 2 or weight.shape[0] != dim or weight.shape[1] not in WIDTHS:
+        raise ValueError(f"{what}: weight must be [{dim}, W] with W in {WIDTHS}, got {tuple(weight.shape)}")
+    if weight.dtype != dtype and weight.dtype != torch.float32:
+        raise RuntimeError(f"{what}: weight must have x's dtype ({dtype}) or be float32 (got {weight.dtype})")
+    if bias is not None:
+        if tuple(bias.shape) != (dim,):
+            raise ValueError(f"{what}: bias must be [{dim}], got {tuple(bias.shape)}")
+        if bias.dtype != weight.dtype:
+            raise RuntimeError(f"{what}: bias must have the weight's dtype ({weight.dtype}), got {bias.dtype}")
+    if activation not in (None, "silu"):
+        raise ValueError(f"{what}: activation must be None or 'silu' (got {activation!r})")
+    return weight.shape[1]
+
+
+def check_lengths(what, lengths, batch) -> None:
+    if lengths is None:
+        return
+    if tuple(lengths.shape) != (batch,) or lengths.dtype != torch.int32:
+        raise ValueError(f"{what}: lengths must be int32 [{batch}], got {lengths.dtype} {tuple(lengths.shape)}")
+
+
+def dense(t: torch.Tensor | None) -> torch.Tensor | None:
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+def dense_last(t: torch.Tensor | None) -> torch.Tensor | None:
+    return t if t is None or t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def strides(t: torch.Tensor) -> tuple[int, int]:
+    """Batch and token strides of [B, L, D]; a dimension of one element has none of its own."""
+    st = t.stride(1) if t.shape[1] > 1 else t.shape[2]
+    return (t.stride(0) if t.shape[0] > 1 else t.shape[1] * st), st
+
+
+def _launch_forward(x, weight, bias, initial, lengths, y, state, silu) -> None:
+    B, L, D = x.shape
+    sb, st = strides(x)
+    _call.call("btp_sm100_causal_conv_forward", x.device.index, x.data_ptr(), weight.data_ptr(), _call.ptr(bias), _call.ptr(initial),
+               _call.ptr(lengths), y.data_ptr(), _call.ptr(state), B, L, D, weight.shape[1], sb, st, int(silu), _call.TAG[x.dtype],
+               _call.TAG[weight.dtype])
+
+
+def _op_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], initial: Optional[torch.Tensor],
+                lengths: Optional[torch.Tensor], y: torch.Tensor, state: Optional[torch.Tensor], silu: bool) -> None:
+    _launch_forward(x, weight, bias, initial, lengths, y, state, silu)
+
+
+def _op_backward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], initial: Optional[torch.Tensor],
+                 lengths: Optional[torch.Tensor], dy: torch.Tensor, dstate: Optional[torch.Tensor], dx: torch.Tensor,
+                 dweight: Optional[torch.Tensor], dbias: Optional[torch.Tensor], dinitial: Optional[torch.Tensor], silu: bool) -> None:
+    B, L, D = x.shape
+    W = weight.shape[1]
+    index = x.device.index
+    sb, st = strides(x)
+    partial = None
+    if dweight is not None or dbias is not None:
+        rows = _call.query("btp_sm100_causal_conv_partial_rows", index, B, L, D)
+        partial = torch.empty(rows, W + 1, D, device=x.device, dtype=torch.float32)
+    _call.call("btp_sm100_causal_conv_backward", index, x.data_ptr(), weight.data_ptr(), _call.ptr(bias), _call.ptr(initial),
+               _call.ptr(lengths), dy.data_ptr(), _call.ptr(dstate), dx.data_ptr(), _call.ptr(dweight), _call.ptr(dbias),
+               _call.ptr(dinitial), _call.ptr(partial), B, L, D, W, sb, st, int(silu), _call.TAG[x.dtype], _call.TAG[weight.dtype])
+
+
+def _fake(*args) -> None:
+    return None
+
+
+_iface._register(_iface._LIB, "spear_btp", "causal_conv_forward", _op_forward, _fake, ["y", "state"])
+_iface._register(_iface._LIB, "spear_btp", "causal_conv_backward", _op_backward, _fake, ["dx", "dweight", "dbias", "dinitial"])
+
+
+class _CausalConv(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, initial, lengths, silu, want_state):
+        B, L, D = x.shape
+        y = torch.empty(B, L, D, device=x.device, dtype=x.dtype)
+        state = torch.empty(B, weight.shape[1] - 1, D, device=x.device, dtype=x.dtype) if want_state else None
+        torch.ops.spear_btp.causal_conv_forward(x, weight, bias, initial, lengths, y, state, silu)
+        ctx.save_for_backward(x, weight, bias, initial, lengths)
+        ctx.silu = silu
+        ctx.set_materialize_grads(False)
+        return (y, state) if want_state else y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dstate=None):
+        x, weight, bias, initial, lengths = ctx.saved_tensors
+        need_x, need_w, need_b, need_i = ctx.needs_input_grad[:4]
+        if dy is None and dstate is None:
+            return (None,) * 7
+        dy = torch.zeros(x.shape, device=x.device, dtype=x.dtype) if dy is None else dy.contiguous()
+        dstate = None if dstate is None else dstate.contiguous()
+        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        dw = torch.empty(weight.shape, device=x.device, dtype=weight.dtype) if need_w else None
+        db = torch.empty(bias.shape, device=x.device, dtype=bias.dtype) if need_b and bias is not None else None
+        di = torch.empty(initial.shape, device=x.device, dtype=x.dtype) if need_i and initial is not None else None
+        torch.ops.spear_btp.causal_conv_backward(x, weight, bias, initial, lengths, dy, dstate, dx, dw, db, di, ctx.silu)
+        return dx if need_x else None, dw, db, di, None, None, None
+
+
+def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *, activation: str | None = None,
+                initial_state: torch.Tensor | None = None, lengths: torch.Tensor | None = None, return_state: bool = False):
+    """Short causal convolution over tokens, one filter per channel.
+
+    Args:
+        x: [B, L, D] bfloat16, float16 or float32 (a view with dense channels is read in place).
+        weight: [D, W], W = 2, 3 or 4, the last tap on the token itself; x's dtype or float32.
+        bias: [D] in the weight's dtype, or None.
+        activation: None or "silu".
+        initial_state: [B, W-1, D] in x's dtype, the inputs before token 0, oldest first; None for zeros.
+        lengths: int32 [B] on the GPU: tokens from lengths[b] on (a padded batch) are not read and give 0; values are
+            held to 0 ... L.
+        return_state: also return the last W-1 inputs of each sequence, the ``state`` of ``causal_conv_step``.
+    Returns:
+        y [B, L, D], or (y, state [B, W-1, D]).  Gradients for x, weight, bias and initial_state.
+    """
+    what = "causal_conv"
+    if x.dim() != 3 or x.shape[2] < 1:
+        raise ValueError(f"{what}: x must be [B, L, D], got {tuple(x.shape)}")
+    B, L, D = x.shape
+    _call.activation(x, f"{what}: x")
+    W = _check_filter(what, D, x.dtype, weight, bias, activation)
+    if initial_state is not None:
+        if tuple(initial_state.shape) != (B, W - 1, D):
+            raise ValueError(f"{what}: initial_state must be {(B, W - 1, D)}, got {tuple(initial_state.shape)}")
+        if initial_state.dtype != x.dtype:
+            raise RuntimeError(f"{what}: initial_state must have x's dtype ({x.dtype}), got {initial_state.dtype}")
+    check_lengths(what, lengths, B)
+    _call.on_gpu(what, x, weight, bias, initial_state, lengths)
+    if B == 0 or L == 0:  # nothing to compute; the state passes through
+        y = x * 1
+        if not return_state:
+            return y
+        return y, (x.new_zeros(B, W - 1, D) if initial_state is None else initial_state.clone())
+    x, weight, bias = dense_last(x), dense(weight), dense(bias)
+    initial_state, lengths = dense(initial_state), dense(lengths)
+    silu = activation == "silu"
+    if torch.compiler.is_compiling() or (torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in (x, weight, bias, initial_state))):
+        return _CausalConv.apply(x, weight, bias, initial_state, lengths, silu, bool(return_state))
+    y = torch.empty(B, L, D, device=x.device, dtype=x.dtype)
+    state = torch.empty(B, W - 1, D, device=x.device, dtype=x.dtype) if return_state else None
+    _launch_forward(x, weight, bias, initial_state, lengths, y, state, silu)
+    return (y, state) if return_state else y
+
+
+def check_state_out(what, state, state_out) -> torch.Tensor:
+    """Where the new state goes: fresh memory, or the caller's tensor, which may be the old state itself."""
+    if state_out is None:
+        return torch.empty(state.shape, device=state.device, dtype=state.dtype)
+    if state_out is state:
+        return state_out
+    if state_out.shape != state.shape or state_out.dtype != state.dtype or state_out.device != state.device or not state_out.is_contiguous():
+        raise ValueError(f"{what}: state_out must be contiguous and have the state's shape, dtype and device")
+    a, b, n = state.data_ptr(), state_out.data_ptr(), state.numel() * state.element_size()
+    if a != b and a < b + n and b < a + n:
+        raise ValueError(f"{what}: state_out overlaps the state without being the same memory")
+    return state_out
+
+
+@torch.no_grad()
+def causal_conv_step(x_t: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
+                     activation: str | None = None, state_out: torch.Tensor | None = None):
+    """One token of ``causal_conv``: returns (y_t [B, D], new state [B, W-1, D]).
+
+    One kernel launch.  ``state`` stays valid and the new state is a fresh tensor, unless ``state_out`` says where to
+    write it: passing the state itself updates it in place (the form for a captured graph).
+    """
+    what = "causal_conv_step"
+    if x_t.dim() != 2 or x_t.shape[1] < 1:
+        raise ValueError(f"{what}: x_t must be [B, D], got {tuple(x_t.shape)}")
+    B, D = x_t.shape
+    _call.activation(x_t, f"{what}: x_t")
+    W = _check_filter(what, D, x_t.dtype, weight, bias, activation)
+    if tuple(state.shape) != (B, W - 1, D) or state.dtype != x_t.dtype or not state.is_contiguous():
+        raise ValueError(f"{what}: state must be contiguous {(B, W - 1, D)} of x_t's dtype, got {state.dtype} {tuple(state.shape)}")
+    index = _call.on_gpu(what, x_t, state, weight, bias)
+    out = check_state_out(what, state, state_out)
+    y = torch.empty(B, D, device=x_t.device, dtype=x_t.dtype)
+    if B == 0:
+        return y, out
+    x_t, weight, bias = dense_last(x_t), dense(weight), dense(bias)
+    _call.call("btp_sm100_causal_conv_step", index, x_t.data_ptr(), state.data_ptr(), weight.data_ptr(), _call.ptr(bias), y.data_ptr(),
+               out.data_ptr(), B, D, W, x_t.stride(0) if B > 1 else D, int(activation is not None), _call.TAG[x_t.dtype],
+               _call.TAG[weight.dtype])
+    return y, out

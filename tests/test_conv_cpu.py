@@ -1,0 +1,80 @@
+"""Refusals of the short causal convolution, on a machine without a GPU too."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from spear_b200.ops.ssm import causal_conv, causal_conv_step
+
+Z = torch.zeros
+
+
+@pytest.mark.parametrize("args,kw,err,text", [
+    ((Z(4, 8), Z(8, 4)), {}, ValueError, "x must be"),
+    ((Z(1, 4, 0), Z(0, 4)), {}, ValueError, "x must be"),
+    ((Z(1, 4, 8).double(), Z(8, 4)), {}, RuntimeError, "x must be bfloat16"),
+    ((Z(1, 4, 8), Z(8, 5)), {}, ValueError, "weight must be"),
+    ((Z(1, 4, 8), Z(8, 1)), {}, ValueError, "weight must be"),
+    ((Z(1, 4, 8), Z(7, 4)), {}, ValueError, "weight must be"),
+    ((Z(1, 4, 8), Z(8, 1, 4)), {}, ValueError, "weight must be"),
+    ((Z(1, 4, 8), Z(8, 4).half()), {}, RuntimeError, "weight must have"),
+    ((Z(1, 4, 8), Z(8, 4), Z(4)), {}, ValueError, "bias must be"),
+    ((Z(1, 4, 8).half(), Z(8, 4), Z(8).half()), {}, RuntimeError, "bias must have"),
+    ((Z(1, 4, 8), Z(8, 4)), {"activation": "relu"}, ValueError, "activation"),
+    ((Z(1, 4, 8), Z(8, 4)), {"initial_state": Z(1, 4, 8)}, ValueError, "initial_state must be"),
+    ((Z(1, 4, 8), Z(8, 4)), {"initial_state": Z(1, 3, 8).half()}, RuntimeError, "initial_state must have"),
+    ((Z(2, 4, 8), Z(8, 4)), {"lengths": Z(3, dtype=torch.int32)}, ValueError, "lengths"),
+    ((Z(2, 4, 8), Z(8, 4)), {"lengths": Z(2, dtype=torch.int64)}, ValueError, "lengths"),
+    ((Z(2, 4, 8), Z(8, 4)), {}, RuntimeError, "no CPU path"),
+])
+def test_refusals(args, kw, err, text):
+    with pytest.raises(err, match=text):
+        causal_conv(*args, **kw)
+
+
+@pytest.mark.parametrize("args,kw,err,text", [
+    ((Z(1, 1, 8), Z(1, 3, 8), Z(8, 4)), {}, ValueError, "x_t must be"),
+    ((Z(1, 8), Z(1, 2, 8), Z(8, 4)), {}, ValueError, "state must be"),
+    ((Z(1, 8), Z(1, 3, 8).half(), Z(8, 4)), {}, ValueError, "state must be"),
+    ((Z(2, 8), Z(2, 8, 3).transpose(1, 2), Z(8, 4)), {}, ValueError, "state must be contiguous"),
+    ((Z(1, 8), Z(1, 3, 8), Z(8, 4)), {}, RuntimeError, "no CPU path"),
+])
+def test_step_refusals(args, kw, err, text):
+    with pytest.raises(err, match=text):
+        causal_conv_step(*args, **kw)
+
+
+def test_where_the_new_state_may_go():
+    from spear_b200.ops.ssm.conv import check_state_out
+
+    pool = Z(3, 3, 8)
+    state = pool[:2]
+    assert check_state_out("f", state, None).data_ptr() != state.data_ptr()
+    assert check_state_out("f", state, state) is state
+    again = pool[:2]
+    assert check_state_out("f", state, again) is again  # the same memory by another name
+    for bad in (pool[1:], Z(2, 3, 9), Z(2, 3, 8).half(), Z(2, 8, 3).transpose(1, 2)):
+        with pytest.raises(ValueError, match="state_out"):
+            check_state_out("f", state, bad)
+
+
+def test_entry_refuses_bad_arguments_before_any_launch():
+    from spear_b200 import _lib
+
+    lib = _lib.load()
+    p = ctypes.c_void_p(16)
+
+    def fwd(x=p, w=p, y=p, B=1, L=4, D=8, W=4, sb=32, st=8, dt=0, wt=0):
+        return lib.btp_sm100_causal_conv_forward(x, w, None, None, None, y, None, B, L, D, W, sb, st, 0, dt, wt, None)
+
+    assert fwd(B=0) == -2 and fwd(L=0) == -2 and fwd(D=-1) == -2 and fwd(sb=-1) == -2 and fwd(L=(1 << 30) + 1) == -2
+    assert fwd(W=1) == -3 and fwd(W=5) == -3 and fwd(dt=2) == -4 and fwd(dt=0, wt=3) == -4
+    assert fwd(x=None) == -1 and fwd(w=None) == -1 and fwd(y=None) == -1
+    bwd = lib.btp_sm100_causal_conv_backward
+    assert bwd(p, p, None, None, None, p, None, p, p, None, None, None, 1, 4, 8, 4, 32, 8, 0, 0, 0, None) == -1
+    step = lib.btp_sm100_causal_conv_step
+    assert step(p, p, p, None, p, None, 1, 8, 4, 8, 0, 0, 0, None) == -1
+    assert step(p, p, p, None, p, p, 1, 8, 9, 8, 0, 0, 0, None) == -3
