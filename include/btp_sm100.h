@@ -269,6 +269,57 @@ int btp_sm100_causal_conv_backward(const void* x, const void* weight, const void
 int btp_sm100_causal_conv_step(const void* x, const void* state, const void* weight, const void* bias, void* y, void* state_out,
                                int B, int dim, int width, long long ld_x, int silu, int dtype, int weight_dtype, void* stream);
 
+/*
+ * Selective state space scan over tokens, token-major.  No counterpart in the reference.
+ *   Delta = delta + delta_bias, or its softplus;  h_t[d,n] = exp(Delta_t[d] A[d,n]) h_{t-1}[d,n] + Delta_t[d] x_t[d] B_t[n]
+ *   y_t[d] = sum_n C_t[n] h_t[d,n] + D[d] x_t[d],  times z_t[d] sigmoid(z_t[d]) where there is a gate
+ *   x, delta, z  [B, L, dim]  dtype: BTP_DTYPE_BF16 | BTP_DTYPE_F16 | BTP_DTYPE_F32; the element at (b, t, d) lies at
+ *                b * (batch stride) + t * (token stride) + d; any alignment (16-byte aligned rows are faster); z NULL: no gate
+ *   Bm, Cm       [B, L, N]    the same type, strides likewise; N 1 ... 64
+ *   A            [dim, N] float;  D, delta_bias [dim] float, NULL: zeros
+ *   initial      [B, dim, N] float, the state before token 0; NULL: zeros
+ *   lengths      [B] int32 on the device, or NULL: tokens of sequence b from lengths[b] on are not read, y is 0 there
+ *                (values are held to 0 ... L)
+ *   y            [B, L, dim] dense;  state  [B, dim, N] float, the state after each sequence's last token, or NULL
+ *   checkpoints  [B, ceil(L/16), dim, N] float, the state before each 16th token, which the backward reads, or NULL
+ *   carry        scratch of btp_sm100_scan_carry_floats(B, L, dim, N) floats; may be NULL where that is 0
+ * A, initial, state, checkpoints and carry are 16-byte aligned.
+ */
+long long btp_sm100_scan_carry_floats(int B, int L, int dim, int N);
+int btp_sm100_scan_forward(const void* x, const void* delta, const float* A, const void* Bm, const void* Cm, const float* D,
+                           const void* z, const float* delta_bias, const float* initial, const int* lengths, void* y, float* state,
+                           float* checkpoints, float* carry, int B, int L, int dim, int N, long long x_b, long long x_t,
+                           long long d_b, long long d_t, long long B_b, long long B_t, long long C_b, long long C_t, long long z_b,
+                           long long z_t, int delta_softplus, int dtype, void* stream);
+
+/*
+ * Backward of btp_sm100_scan_forward, for gradients dy of y and dstate of state (NULL: none).
+ *   checkpoints  as the forward left them
+ *   dy, dx, ddelta, dz  [B, L, dim] dense; dB, dC  [B, L, N] dense (all 0 from lengths[b] on); dz only with a gate
+ *   dparams      float: dA [dim, N], then dD [dim], then the gradient of delta_bias [dim]; room for dim * (N + 2) rounded
+ *                up to a multiple of 4
+ *   dstate, dinitial  [B, dim, N] float, either NULL
+ *   buffer       scratch of btp_sm100_scan_backward_floats(B, L, dim, N) floats, 16-byte aligned
+ * Sums are taken in a fixed order: the same call gives the same bits.
+ */
+long long btp_sm100_scan_backward_floats(int B, int L, int dim, int N);
+int btp_sm100_scan_backward(const void* x, const void* delta, const float* A, const void* Bm, const void* Cm, const float* D,
+                            const void* z, const float* delta_bias, const int* lengths, const float* checkpoints, const void* dy,
+                            const float* dstate, void* dx, void* ddelta, float* dparams, void* dB, void* dC, void* dz,
+                            float* dinitial, float* buffer, int B, int L, int dim, int N, long long x_b, long long x_t, long long d_b,
+                            long long d_t, long long B_b, long long B_t, long long C_b, long long C_t, long long z_b, long long z_t,
+                            int delta_softplus, int dtype, void* stream);
+
+/*
+ * One token of the same scan: x, delta, z, y [B, dim], Bm, Cm [B, N] with row pitches ld_*; state, state_out
+ * [B, dim, N] float, 16-byte aligned.  state_out may be state itself (an update in place); any other overlap is an error
+ * of the caller's.
+ */
+int btp_sm100_scan_step(const void* x, const void* delta, const float* A, const void* Bm, const void* Cm, const float* D,
+                        const void* z, const float* delta_bias, const float* state, void* y, float* state_out, int B, int dim, int N,
+                        long long ld_x, long long ld_d, long long ld_B, long long ld_C, long long ld_z, int delta_softplus, int dtype,
+                        void* stream);
+
 /* Name of a status code ("BTP_OK", "BTP_ERR_BAD_SHAPE", ...).  Never NULL. */
 const char* btp_sm100_status_string(int status);
 

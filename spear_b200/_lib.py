@@ -43,6 +43,11 @@ SYMBOLS = {
     "btp_sm100_causal_conv_partial_rows": (_i, [_i] * 3),
     "btp_sm100_causal_conv_backward": (_i, [_vp] * 12 + [_i] * 4 + [_ll, _ll, _i, _i, _i, _vp]),
     "btp_sm100_causal_conv_step": (_i, [_vp] * 6 + [_i] * 3 + [_ll, _i, _i, _i, _vp]),
+    "btp_sm100_scan_carry_floats": (_ll, [_i] * 4),
+    "btp_sm100_scan_forward": (_i, [_vp] * 14 + [_i] * 4 + [_ll] * 10 + [_i, _i, _vp]),
+    "btp_sm100_scan_backward_floats": (_ll, [_i] * 4),
+    "btp_sm100_scan_backward": (_i, [_vp] * 20 + [_i] * 4 + [_ll] * 10 + [_i, _i, _vp]),
+    "btp_sm100_scan_step": (_i, [_vp] * 11 + [_i] * 3 + [_ll] * 5 + [_i, _i, _vp]),
     "btp_sm100_noalloc_read_record": (_i, [_vp, _ll, _vp]),
     "btp_sm100_set_wait_limit": (ctypes.c_ulonglong, [ctypes.c_ulonglong]),
     "btp_sm100_set_seam_mode": (_i, [_i]),

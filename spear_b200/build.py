@@ -18,7 +18,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libbtp_sm100.so")
 SOURCES = [os.path.join(CSRC, "btp_sm100.cu"), os.path.join(CSRC, "norm_sm100.cu"),
-           os.path.join(CSRC, "conv_sm100.cu")]
+           os.path.join(CSRC, "conv_sm100.cu"), os.path.join(CSRC, "scan_sm100.cu")]
 HEADERS = [
     os.path.join(CSRC, "btp_kernels.cuh"),
     os.path.join(CSRC, "btp_decode.cuh"),
@@ -30,6 +30,9 @@ HEADERS = [
     os.path.join(CSRC, "elem_host.cuh"),
     os.path.join(CSRC, "norm_kernels.cuh"),
     os.path.join(CSRC, "conv_kernels.cuh"),
+    os.path.join(CSRC, "scan_kernels.cuh"),
+    os.path.join(CSRC, "scan_bwd_kernels.cuh"),
+    os.path.join(CSRC, "sum_kernels.cuh"),
     os.path.join(os.path.dirname(HERE), "include", "btp_sm100.h"),
 ]
 

@@ -80,6 +80,57 @@ constexpr float kLog2e = 1.4426950408889634f;
 // 1 / (1 + e^-v); the exponent's rounding makes it |v| 2^-24 off relative for very negative v, a few 2^-24 elsewhere.
 __device__ __forceinline__ float sigmoid(float v) { return rcp(1.f + ex2(-v * kLog2e)); }
 
+// log(1 + e^v) to a few units in the last place, without overflow:  max(v, 0) + log(1 + w) with w = e^-|v| <= 1, and
+// log(1 + w) = 2 atanh(s), s = w / (2 + w) <= 1/3, by the series s + s^3/3 + s^5/5 + ... up to s^15 (the rest is below 2^-28).
+__device__ __forceinline__ float softplus(float v) {
+  const float w = ex2(-fabsf(v) * kLog2e);
+  const float s = w * rcp(2.f + w), q = s * s;
+  float p = 2.f / 15.f;
+  p = fmaf(p, q, 2.f / 13.f);
+  p = fmaf(p, q, 2.f / 11.f);
+  p = fmaf(p, q, 2.f / 9.f);
+  p = fmaf(p, q, 2.f / 7.f);
+  p = fmaf(p, q, 2.f / 5.f);
+  p = fmaf(p, q, 2.f / 3.f);
+  p = fmaf(p, q, 2.f);
+  return (v < 0.f ? 0.f : v) + p * s;  // not fmaxf: NaN stays
+}
+
+// Two floats side by side in one 64-bit register pair: one instruction does the arithmetic of both.
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pack2(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack2(float& lo, float& hi, f32x2 v) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ float lo2(f32x2 v) {
+  float a, b;
+  unpack2(a, b, v);
+  return a;
+}
+__device__ __forceinline__ float hi2(f32x2 v) {
+  float a, b;
+  unpack2(a, b, v);
+  return b;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 ex2_2(f32x2 v) { return pack2(ex2(lo2(v)), ex2(hi2(v))); }
+
 // Tokens of sequence b that are there: `lengths` may be null (all L), its values are held to 0 ... L.
 __device__ __forceinline__ int tokens_of(const int* lengths, long long b, int L) {
   if (!lengths) return L;

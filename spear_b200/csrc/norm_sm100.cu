@@ -1,6 +1,7 @@
 // C entries of the root-mean-square norm: argument checks, launch shapes, launches.
 #include "elem_host.cuh"
 #include "norm_kernels.cuh"
+#include "sum_kernels.cuh"
 
 namespace {
 

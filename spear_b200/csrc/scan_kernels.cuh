@@ -1,0 +1,453 @@
+// Selective state space scan, token-major (sm_100a): forward over prompts and one token.
+//
+//   Delta_t[d] = softplus(delta_t[d] + bias[d])  (or the plain sum)          u_t = Delta_t x_t
+//   h_t[d,n]   = exp(Delta_t[d] A[d,n]) h_{t-1}[d,n] + u_t[d] B_t[n]
+//   y_t[d]     = sum_n C_t[n] h_t[d,n] + D[d] x_t[d],  times z_t sigmoid(z_t) where there is a gate
+//
+// Layout.  A warp walks down the tokens of 128 / SG channels: lane = (channel group g, state group s), SG state groups;
+// a lane holds 4 channels x 4 states of h as pairs of neighbouring channels, so that products and sums are two-wide
+// (f32x2) with the step sizes as they lie in memory and with B and C given twice.  y is summed over a lane's 4 states in
+// registers and over the SG lanes by exchanging halves: 3 exchanges for 4 channels and 4 lanes.
+// Tiles of 16 tokens arrive by asynchronous copies one tile ahead; a first pass over the tile turns the raw values into
+// step sizes, inputs u and doubled B, C in float; a last pass adds D x, applies the gate and stores.
+//
+// Bound: one exponential per (token, channel, state) on the special-function unit, 16 per clock and SM.
+//
+// Few channels or sequences: the tokens are split over `splits` chunks.  A first kernel runs each chunk from state zero and
+// keeps its last state and its sum of step sizes (the product of its decays is exp(A times that sum), one exponential); the second
+// combines the chunks before its own in order and runs its chunk from there.  That doubles the exponentials, so the rule in
+// scan_sm100.cu splits only where warps are missing.
+#pragma once
+
+#include "btp_elem.cuh"
+
+namespace btp_scan {
+
+using namespace btp_elem;
+
+constexpr int kTile = 16;        // tokens per tile
+constexpr int kCheckpoint = 16;  // tokens between the states that the forward keeps for the backward
+
+struct ScanParams {
+  const void* x;
+  const void* delta;
+  const void* B;
+  const void* C;
+  const void* z;          // nullptr: no gate
+  const float* A;         // [dim, N]
+  const float* D;         // [dim] or nullptr
+  const float* bias;      // [dim] or nullptr
+  const float* initial;   // [B, dim, N] or nullptr
+  const int* lengths;     // [B] or nullptr
+  void* y;                // [B, L, dim]
+  float* state;           // [B, dim, N] or nullptr
+  float* checkpoints;     // [B, ceil(L / 16), dim, N] or nullptr: the state before each 16th token
+  float* carry;           // [splits - 1][B][dim][N] last states, then [splits - 1][B][dim] sums of step sizes
+  long long x_b, x_t, d_b, d_t, z_b, z_t, B_b, B_t, C_b, C_t;
+  int batch, L, dim, N;
+  int splits, chunk;      // chunk: tokens per split, a multiple of 32
+  bool softplus;
+  bool al_x, al_d, al_z, al_B, al_C, al_y;  // 16-byte copies (y: pairs) are possible
+};
+
+template <class T, int SG>
+struct Tile {
+  static constexpr int kStates = 4 * SG;
+  static constexpr int kChannels = 128 / SG;
+  T x[2][kTile][kChannels];
+  T d[2][kTile][kChannels];
+  T z[2][kTile][kChannels];
+  T B[2][kTile][kStates];
+  T C[2][kTile][kStates];
+  float delta[kTile][kChannels];
+  float u[kTile][kChannels];
+  float y[kTile][kChannels];
+  float B2[kTile][kStates * 2];
+  float C2[kTile][kStates * 2];
+};
+
+__device__ __forceinline__ void copy16(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy4(void* to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// ROWS rows of COLS elements (row pitch `pitch`, `cols` of them there) into dst[ROWS][COLS], by the threads of a group of
+// GROUP threads.  Rows from `rows` on and columns from `cols` on are not touched.
+template <class T, int ROWS, int COLS, int GROUP>
+__device__ __forceinline__ void fetch(T (*dst)[COLS], const T* src, long long pitch, int rows, int cols, bool aligned, int tid) {
+  constexpr int E = 16 / static_cast<int>(sizeof(T)), CPR = COLS / E;
+  if (aligned) {
+#pragma unroll
+    for (int i0 = 0; i0 < ROWS * CPR; i0 += GROUP) {
+      const int i = i0 + tid, r = i / CPR, c = (i - r * CPR) * E;
+      if ((ROWS * CPR % GROUP == 0 || i < ROWS * CPR) && r < rows && c < cols) copy16(&dst[r][c], src + r * pitch + c);
+    }
+  } else {
+#pragma unroll 4
+    for (int i0 = 0; i0 < ROWS * COLS; i0 += GROUP) {
+      const int i = i0 + tid, r = i / COLS, c = i - r * COLS;
+      if (i < ROWS * COLS && r < rows && c < cols) {
+        if (sizeof(T) == 4)
+          copy4(&dst[r][c], src + r * pitch + c);
+        else
+          dst[r][c] = src[r * pitch + c];
+      }
+    }
+  }
+}
+
+// Sums four values over the SG lanes of a state group.  SG >= 4: lane s ends with value s & 3; SG == 2: lane s with values
+// 2s and 2s + 1.  v[0], v[1] are the pairs (0, 1) and (2, 3).
+template <int SG>
+__device__ __forceinline__ void reduce_states(float (&out)[2], f32x2 v0, f32x2 v1, int s) {
+  if (SG == 2) {
+    const f32x2 keep = (s & 1) ? v1 : v0, give = (s & 1) ? v0 : v1;
+    const f32x2 sum = add2(keep, __shfl_xor_sync(0xffffffffu, give, 1));
+    unpack2(out[0], out[1], sum);
+    return;
+  }
+  const f32x2 keep = (s & 2) ? v1 : v0, give = (s & 2) ? v0 : v1;
+  const f32x2 sum = add2(keep, __shfl_xor_sync(0xffffffffu, give, 2));
+  float a, b;
+  unpack2(a, b, sum);
+  const float k = (s & 1) ? b : a, o = (s & 1) ? a : b;
+  float r = k + __shfl_xor_sync(0xffffffffu, o, 1);
+  if (SG >= 8) r += __shfl_xor_sync(0xffffffffu, r, 4);
+  if (SG >= 16) r += __shfl_xor_sync(0xffffffffu, r, 8);
+  out[0] = r;
+  out[1] = 0.f;
+}
+
+// Four consecutive states of one channel of a [.., N] row; states from N on are 0.
+__device__ __forceinline__ void load_states(float (&v)[4], const float* row, int n0, int N) {
+  if ((N & 3) == 0) {
+    if (n0 < N) {
+      const float4 q = *reinterpret_cast<const float4*>(row + n0);
+      v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+    } else {
+      v[0] = v[1] = v[2] = v[3] = 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = n0 + k < N ? row[n0 + k] : 0.f;
+  }
+}
+__device__ __forceinline__ void store_states(float* row, const float (&v)[4], int n0, int N) {
+  if ((N & 3) == 0) {
+    if (n0 < N) *reinterpret_cast<float4*>(row + n0) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (n0 + k < N) row[n0 + k] = v[k];
+  }
+}
+
+// The lane's 4 channels x 4 states, pairs of channels: r[p][n] holds channels 2p and 2p + 1.
+struct LaneState {
+  f32x2 r[2][4];
+};
+__device__ __forceinline__ void load_lane(LaneState& h, const float* base, int c0, int dim, int n0, int N, float scale) {
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    float a[4] = {}, b[4] = {};
+    if (c0 + 2 * p < dim) load_states(a, base + static_cast<long long>(c0 + 2 * p) * N, n0, N);
+    if (c0 + 2 * p + 1 < dim) load_states(b, base + static_cast<long long>(c0 + 2 * p + 1) * N, n0, N);
+#pragma unroll
+    for (int n = 0; n < 4; ++n) h.r[p][n] = pack2(a[n] * scale, b[n] * scale);
+  }
+}
+__device__ __forceinline__ void store_lane(float* base, const LaneState& h, int c0, int dim, int n0, int N) {
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    float a[4], b[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) unpack2(a[n], b[n], h.r[p][n]);
+    if (c0 + 2 * p < dim) store_states(base + static_cast<long long>(c0 + 2 * p) * N, a, n0, N);
+    if (c0 + 2 * p + 1 < dim) store_states(base + static_cast<long long>(c0 + 2 * p + 1) * N, b, n0, N);
+  }
+}
+// h = exp(A total) h + last: the effect of a whole chunk with step sizes that sum up to `total`.
+__device__ __forceinline__ void apply_chunk(LaneState& h, const LaneState& A2, const LaneState& last, f32x2 t0, f32x2 t1) {
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    h.r[0][n] = fma2(ex2_2(mul2(A2.r[0][n], t0)), h.r[0][n], last.r[0][n]);
+    h.r[1][n] = fma2(ex2_2(mul2(A2.r[1][n], t1)), h.r[1][n], last.r[1][n]);
+  }
+}
+__device__ __forceinline__ void load_totals(f32x2& t0, f32x2& t1, const float* row, int c0, int dim) {
+  float t[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) t[k] = c0 + k < dim ? row[c0 + k] : 0.f;
+  t0 = pack2(t[0], t[1]);
+  t1 = pack2(t[2], t[3]);
+}
+// Lanes that stand for states from N on keep 0 there, whatever the inputs hold.
+__device__ __forceinline__ void clear_padding(LaneState& h, int n0, int N) {
+#pragma unroll
+  for (int n = 0; n < 4; ++n)
+    if (n0 + n >= N) h.r[0][n] = h.r[1][n] = 0ull;
+}
+
+// One warp per (channels, chunk, sequence).  CARRY: only the chunk's last state and sum of step sizes, from state zero.
+template <class T, int SG, bool CARRY>
+__global__ void __launch_bounds__(32) scan_forward_kernel(const ScanParams p) {
+  using S = Tile<T, SG>;
+  constexpr int WC = S::kChannels, NP = S::kStates, CP = WC / 2, RPI = 32 / CP;  // channel pairs per row, rows per pass
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  S& sm = *reinterpret_cast<S*>(smem_raw);
+  grid_dependency_wait();
+  const int lane = threadIdx.x, g = lane / SG, s = lane % SG;
+  const int cblocks = (p.dim + WC - 1) / WC;
+  const int splits = CARRY ? p.splits - 1 : p.splits;
+  const int cb = blockIdx.x % cblocks;
+  const int rest = blockIdx.x / cblocks;
+  const int q = rest % splits;
+  const long long b = rest / splits;
+  const int cw = cb * WC, c0 = cw + 4 * g, n0 = 4 * s;
+  const int n_tok = tokens_of(p.lengths, b, p.L);
+  const int first = q * p.chunk, end = min(p.L, first + p.chunk), live = min(end, n_tok);
+  const int cols = min(WC, p.dim - cw);
+  const bool full = p.N == NP;
+
+  LaneState A2, h;
+  load_lane(A2, p.A, c0, p.dim, n0, p.N, kLog2e);
+  if (CARRY || !p.initial) {
+#pragma unroll
+    for (int n = 0; n < 4; ++n) h.r[0][n] = h.r[1][n] = 0ull;
+  } else {
+    load_lane(h, p.initial + b * p.dim * p.N, c0, p.dim, n0, p.N, 1.f);
+  }
+  const long long per_chunk = static_cast<long long>(p.batch) * p.dim;
+  float* totals = p.carry + (p.splits - 1) * per_chunk * p.N;
+  if (!CARRY) {
+    for (int k = 0; k < q; ++k) {
+      LaneState last;
+      f32x2 t0, t1;
+      load_lane(last, p.carry + (k * per_chunk + b * p.dim) * p.N, c0, p.dim, n0, p.N, 1.f);
+      load_totals(t0, t1, totals + k * per_chunk + b * p.dim, c0, p.dim);
+      apply_chunk(h, A2, last, t0, t1);
+    }
+  }
+  // this lane's channel pair in the passes over a tile
+  const int cp = lane % CP, row0 = lane / CP, pc = cw + 2 * cp;
+  float bias[2], skip[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    bias[k] = p.bias && pc + k < p.dim ? p.bias[pc + k] : 0.f;
+    skip[k] = p.D && pc + k < p.dim ? p.D[pc + k] : 0.f;
+  }
+  const T* x = static_cast<const T*>(p.x) + b * p.x_b + cw;
+  const T* dl = static_cast<const T*>(p.delta) + b * p.d_b + cw;
+  const T* z = p.z ? static_cast<const T*>(p.z) + b * p.z_b + cw : nullptr;
+  const T* Bm = static_cast<const T*>(p.B) + b * p.B_b;
+  const T* Cm = static_cast<const T*>(p.C) + b * p.C_b;
+  T* y = static_cast<T*>(p.y) + (b * p.L) * p.dim + cw;
+  const auto load_tile = [&](int st, int t0) {
+    const int rows = min(kTile, live - t0);
+    fetch<T, kTile, WC, 32>(sm.x[st], x + t0 * p.x_t, p.x_t, rows, cols, p.al_x, lane);
+    fetch<T, kTile, WC, 32>(sm.d[st], dl + t0 * p.d_t, p.d_t, rows, cols, p.al_d, lane);
+    fetch<T, kTile, NP, 32>(sm.B[st], Bm + t0 * p.B_t, p.B_t, rows, p.N, p.al_B, lane);
+    if (!CARRY) {
+      fetch<T, kTile, NP, 32>(sm.C[st], Cm + t0 * p.C_t, p.C_t, rows, p.N, p.al_C, lane);
+      if (z) fetch<T, kTile, WC, 32>(sm.z[st], z + t0 * p.z_t, p.z_t, rows, cols, p.al_z, lane);
+    }
+  };
+  f32x2 sum0 = 0ull, sum1 = 0ull;
+  if (first < live) load_tile(0, first);
+  copy_commit();
+  int st = 0;
+  for (int t0 = first; t0 < live; t0 += kTile, st ^= 1) {
+    if (t0 + kTile < live) load_tile(st ^ 1, t0 + kTile);
+    copy_commit();
+    copy_wait<1>();
+    __syncwarp();
+    const int nt = min(kTile, live - t0);
+    if (!CARRY && p.checkpoints && t0 % kCheckpoint == 0) {
+      const long long at = b * ((p.L + kCheckpoint - 1) / kCheckpoint) + t0 / kCheckpoint;
+      store_lane(p.checkpoints + at * p.dim * p.N, h, c0, p.dim, n0, p.N);
+    }
+#pragma unroll
+    for (int i = 0; i < kTile; i += RPI) {
+      const int r = i + row0;
+      float de[2], uu[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const bool ok = r < nt && pc + k < p.dim;
+        float v = ok ? to_f(sm.d[st][r][2 * cp + k]) + bias[k] : 0.f;
+        if (p.softplus) v = softplus(v);
+        de[k] = ok ? v : 0.f;
+        uu[k] = ok ? v * to_f(sm.x[st][r][2 * cp + k]) : 0.f;
+      }
+      *reinterpret_cast<float2*>(&sm.delta[r][2 * cp]) = make_float2(de[0], de[1]);
+      *reinterpret_cast<float2*>(&sm.u[r][2 * cp]) = make_float2(uu[0], uu[1]);
+    }
+#pragma unroll
+    for (int i = 0; i < kTile * NP / 2; i += 32) {
+      const int r = (i + lane) / (NP / 2), n = (i + lane) % (NP / 2) * 2;
+      const bool ok0 = r < nt && n < p.N, ok1 = r < nt && n + 1 < p.N;
+      const float b0 = ok0 ? to_f(sm.B[st][r][n]) : 0.f, b1 = ok1 ? to_f(sm.B[st][r][n + 1]) : 0.f;
+      *reinterpret_cast<float4*>(&sm.B2[r][2 * n]) = make_float4(b0, b0, b1, b1);
+      if (!CARRY) {
+        const float e0 = ok0 ? to_f(sm.C[st][r][n]) : 0.f, e1 = ok1 ? to_f(sm.C[st][r][n + 1]) : 0.f;
+        *reinterpret_cast<float4*>(&sm.C2[r][2 * n]) = make_float4(e0, e0, e1, e1);
+      }
+    }
+    __syncwarp();
+#pragma unroll 4
+    for (int t = 0; t < nt; ++t) {
+      const ulonglong2 d2 = *reinterpret_cast<const ulonglong2*>(&sm.delta[t][4 * g]);
+      const ulonglong2 u2 = *reinterpret_cast<const ulonglong2*>(&sm.u[t][4 * g]);
+      const ulonglong2 ba = *reinterpret_cast<const ulonglong2*>(&sm.B2[t][8 * s]);
+      const ulonglong2 bb = *reinterpret_cast<const ulonglong2*>(&sm.B2[t][8 * s + 4]);
+      const f32x2 bn[4] = {ba.x, ba.y, bb.x, bb.y};
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        h.r[0][n] = fma2(ex2_2(mul2(d2.x, A2.r[0][n])), h.r[0][n], mul2(u2.x, bn[n]));
+        h.r[1][n] = fma2(ex2_2(mul2(d2.y, A2.r[1][n])), h.r[1][n], mul2(u2.y, bn[n]));
+      }
+      if (!full) clear_padding(h, n0, p.N);
+      if (CARRY) {
+        sum0 = add2(sum0, d2.x);
+        sum1 = add2(sum1, d2.y);
+      } else {
+        const ulonglong2 ca = *reinterpret_cast<const ulonglong2*>(&sm.C2[t][8 * s]);
+        const ulonglong2 cc = *reinterpret_cast<const ulonglong2*>(&sm.C2[t][8 * s + 4]);
+        const f32x2 cn[4] = {ca.x, ca.y, cc.x, cc.y};
+        f32x2 y0 = mul2(cn[0], h.r[0][0]), y1 = mul2(cn[0], h.r[1][0]);
+#pragma unroll
+        for (int n = 1; n < 4; ++n) {
+          y0 = fma2(cn[n], h.r[0][n], y0);
+          y1 = fma2(cn[n], h.r[1][n], y1);
+        }
+        float out[2];
+        reduce_states<SG>(out, y0, y1, s);
+        if (SG == 2)
+          *reinterpret_cast<float2*>(&sm.y[t][4 * g + 2 * s]) = make_float2(out[0], out[1]);
+        else if (SG == 4 || s < 4)
+          sm.y[t][4 * g + (s & 3)] = out[0];
+      }
+    }
+    __syncwarp();
+    if (!CARRY) {
+#pragma unroll
+      for (int i = 0; i < kTile; i += RPI) {
+        const int r = i + row0;
+        if (r >= nt || pc >= p.dim) continue;
+        float out[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          out[k] = fmaf(skip[k], to_f(sm.x[st][r][2 * cp + k]), sm.y[r][2 * cp + k]);
+          if (z) {
+            const float zz = to_f(sm.z[st][r][2 * cp + k]);
+            out[k] *= zz * sigmoid(zz);
+          }
+        }
+        store_run<T, 2>(y + static_cast<long long>(t0 + r) * p.dim + 2 * cp, out, p.al_y, p.dim - pc);
+      }
+    }
+    __syncwarp();
+  }
+  copy_wait<0>();
+  if (CARRY) {
+    store_lane(p.carry + (q * per_chunk + b * p.dim) * p.N, h, c0, p.dim, n0, p.N);
+    if (s == 0) {
+      float t[4];
+      unpack2(t[0], t[1], sum0);
+      unpack2(t[2], t[3], sum1);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (c0 + k < p.dim) totals[q * per_chunk + b * p.dim + c0 + k] = t[k];
+    }
+    return;
+  }
+  const float zero[2] = {};
+  if (pc < p.dim)
+    for (int t = max(first, live) + row0; t < end; t += RPI)
+      store_run<T, 2>(y + static_cast<long long>(t) * p.dim + 2 * cp, zero, p.al_y, p.dim - pc);
+  if (p.state && q == p.splits - 1) store_lane(p.state + b * p.dim * p.N, h, c0, p.dim, n0, p.N);
+}
+
+// ---------------------------------------------------------------------------------------------------- one token
+struct ScanStepParams {
+  const void* x;      // [B, dim], row pitches ld_*
+  const void* delta;
+  const void* B;      // [B, N]
+  const void* C;
+  const void* z;      // or nullptr
+  const float* A;
+  const float* D;
+  const float* bias;
+  const float* state;  // [B, dim, N]
+  float* state_out;    // may be `state`
+  void* y;             // [B, dim]
+  long long ld_x, ld_d, ld_z, ld_B, ld_C;
+  int batch, dim, N;
+  bool softplus;
+};
+
+constexpr int kStepBatch = 4;  // sequences per thread: they share A, D and the bias
+
+// SG lanes share a channel, 4 states each.  The states' traffic bounds it: 8 bytes per state.
+template <class T, int SG>
+__global__ void __launch_bounds__(128) scan_step_kernel(const ScanStepParams p) {
+  grid_dependency_wait();
+  const long long idx = static_cast<long long>(blockIdx.x) * 128 + threadIdx.x;
+  const long long per_group = (static_cast<long long>(p.dim) * SG + 31) / 32 * 32;  // whole warps: the exchange below needs all lanes
+  const long long bg = idx / per_group;
+  const int in = static_cast<int>(idx - bg * per_group);
+  const int d = in / SG, s = in % SG, n0 = 4 * s;
+  if (bg * kStepBatch >= p.batch) return;
+  const bool ok = d < p.dim;
+  const int dd = ok ? d : p.dim - 1;
+  float A[4], h[kStepBatch][4], Bn[kStepBatch][4], Cn[kStepBatch][4], x[kStepBatch], v[kStepBatch], z[kStepBatch];
+  const int nb = min(kStepBatch, p.batch - static_cast<int>(bg) * kStepBatch);
+  const long long b0 = bg * kStepBatch;
+#pragma unroll
+  for (int i = 0; i < kStepBatch; ++i) {
+    if (i >= nb) break;
+    const long long b = b0 + i;
+    load_states(h[i], p.state + (b * p.dim + dd) * p.N, n0, p.N);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      Bn[i][k] = n0 + k < p.N ? to_f(static_cast<const T*>(p.B)[b * p.ld_B + n0 + k]) : 0.f;
+      Cn[i][k] = n0 + k < p.N ? to_f(static_cast<const T*>(p.C)[b * p.ld_C + n0 + k]) : 0.f;
+    }
+    x[i] = to_f(static_cast<const T*>(p.x)[b * p.ld_x + dd]);
+    v[i] = to_f(static_cast<const T*>(p.delta)[b * p.ld_d + dd]);
+    z[i] = p.z ? to_f(static_cast<const T*>(p.z)[b * p.ld_z + dd]) : 0.f;
+  }
+  load_states(A, p.A + static_cast<long long>(dd) * p.N, n0, p.N);
+  const float bias = p.bias ? p.bias[dd] : 0.f, skip = p.D ? p.D[dd] : 0.f;
+#pragma unroll
+  for (int i = 0; i < kStepBatch; ++i) {
+    if (i >= nb) break;
+    const long long b = b0 + i;
+    float de = v[i] + bias;
+    if (p.softplus) de = softplus(de);
+    const float u = de * x[i];
+    float y = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      h[i][k] = fmaf(ex2(de * (A[k] * kLog2e)), h[i][k], u * Bn[i][k]);
+      if (n0 + k < p.N) y = fmaf(Cn[i][k], h[i][k], y);
+    }
+#pragma unroll
+    for (int o = SG / 2; o; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+    if (!ok) continue;
+    store_states(p.state_out + (b * p.dim + dd) * p.N, h[i], n0, p.N);
+    if (s == 0) {
+      y = fmaf(skip, x[i], y);
+      if (p.z) y *= z[i] * sigmoid(z[i]);
+      static_cast<T*>(p.y)[b * p.dim + d] = from_f<T>(y);
+    }
+  }
+}
+
+}  // namespace btp_scan

@@ -1,0 +1,224 @@
+"""``selective_scan`` and ``selective_scan_step``: a state space recurrence whose step size, input and output depend on the token.
+
+    Delta_t = softplus(delta_t + delta_bias)                       step size per channel
+    h_t[d, n] = exp(Delta_t[d] A[d, n]) h_{t-1}[d, n] + Delta_t[d] x_t[d] B_t[n]
+    y_t[d] = sum_n C_t[n] h_t[d, n] + D[d] x_t[d],   times silu(z_t) where there is a gate
+
+Token-major, [batch, length, channels]; the state is float32.  Where the BTP recurrence looks back over one block, this
+one's state reaches over the whole prompt.  CUDA only, no fallback.
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from ..btp import interface as _iface
+from .. import _call
+from .conv import check_lengths, check_state_out, dense, dense_last, strides
+
+__all__ = ["selective_scan", "selective_scan_step", "MAX_STATES"]
+
+MAX_STATES = 64
+_CHECKPOINT = 16  # tokens between the states that the forward keeps for the backward
+
+
+def _aligned(t: torch.Tensor | None) -> torch.Tensor | None:
+    """16-byte aligned: a dense view that starts elsewhere gets copied."""
+    return t if t is None or t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _check_params(what, dim, A, D, delta_bias) -> int:
+    if A.dim() != 2 or A.shape[0] != dim or not 1 <= A.shape[1] <= MAX_STATES:
+        raise ValueError(f"{what}: A must be [{dim}, N] with 1 <= N <= {MAX_STATES}, got {tuple(A.shape)}")
+    for t, name in ((A, "A"), (D, "D"), (delta_bias, "delta_bias")):
+        if t is None:
+            continue
+        if name != "A" and tuple(t.shape) != (dim,):
+            raise ValueError(f"{what}: {name} must be [{dim}], got {tuple(t.shape)}")
+        if t.dtype != torch.float32:
+            raise RuntimeError(f"{what}: {name} must be float32 (got {t.dtype})")
+    return A.shape[1]
+
+
+def _check_tokens(what, x, others) -> None:
+    for t, name, shape in others:
+        if t is None:
+            continue
+        if tuple(t.shape) != shape:
+            raise ValueError(f"{what}: {name} must be {shape}, got {tuple(t.shape)}")
+        if t.dtype != x.dtype:
+            raise RuntimeError(f"{what}: {name} must have x's dtype ({x.dtype}), got {t.dtype}")
+
+
+def _shape_args(x, delta, A, B, C, z):
+    zb, zt = (0, 0) if z is None else strides(z)
+    return (x.shape[0], x.shape[1], x.shape[2], A.shape[1], *strides(x), *strides(delta), *strides(B), *strides(C), zb, zt)
+
+
+def _launch_forward(x, delta, A, B, C, D, z, delta_bias, initial, lengths, y, state, checkpoints, softplus) -> None:
+    index = x.device.index
+    A, initial = _aligned(A), _aligned(initial)
+    shape = _shape_args(x, delta, A, B, C, z)
+    n = _call.query("btp_sm100_scan_carry_floats", index, *shape[:4])
+    carry = torch.empty(n, device=x.device, dtype=torch.float32) if n else None
+    p = _call.ptr
+    _call.call("btp_sm100_scan_forward", index, x.data_ptr(), delta.data_ptr(), A.data_ptr(), B.data_ptr(), C.data_ptr(), p(D), p(z),
+               p(delta_bias), p(initial), p(lengths), y.data_ptr(), p(state), p(checkpoints), p(carry), *shape, int(softplus),
+               _call.TAG[x.dtype])
+
+
+def _op_forward(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, D: Optional[torch.Tensor],
+                z: Optional[torch.Tensor], delta_bias: Optional[torch.Tensor], initial: Optional[torch.Tensor],
+                lengths: Optional[torch.Tensor], y: torch.Tensor, state: Optional[torch.Tensor], checkpoints: torch.Tensor,
+                softplus: bool) -> None:
+    _launch_forward(x, delta, A, B, C, D, z, delta_bias, initial, lengths, y, state, checkpoints, softplus)
+
+
+def _op_backward(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, D: Optional[torch.Tensor],
+                 z: Optional[torch.Tensor], delta_bias: Optional[torch.Tensor], lengths: Optional[torch.Tensor],
+                 checkpoints: torch.Tensor, dy: torch.Tensor, dstate: Optional[torch.Tensor], dx: torch.Tensor, ddelta: torch.Tensor,
+                 dparams: torch.Tensor, dB: torch.Tensor, dC: torch.Tensor, dz: Optional[torch.Tensor],
+                 dinitial: Optional[torch.Tensor], softplus: bool) -> None:
+    index = x.device.index
+    A, dstate = _aligned(A), _aligned(dstate)
+    shape = _shape_args(x, delta, A, B, C, z)
+    buffer = torch.empty(_call.query("btp_sm100_scan_backward_floats", index, *shape[:4]), device=x.device, dtype=torch.float32)
+    p = _call.ptr
+    _call.call("btp_sm100_scan_backward", index, x.data_ptr(), delta.data_ptr(), A.data_ptr(), B.data_ptr(), C.data_ptr(), p(D), p(z),
+               p(delta_bias), p(lengths), checkpoints.data_ptr(), dy.data_ptr(), p(dstate), dx.data_ptr(), ddelta.data_ptr(),
+               dparams.data_ptr(), dB.data_ptr(), dC.data_ptr(), p(dz), p(dinitial), buffer.data_ptr(), *shape, int(softplus),
+               _call.TAG[x.dtype])
+
+
+def _fake(*args) -> None:
+    return None
+
+
+_iface._register(_iface._LIB, "spear_btp", "scan_forward", _op_forward, _fake, ["y", "state", "checkpoints"])
+_iface._register(_iface._LIB, "spear_btp", "scan_backward", _op_backward, _fake, ["dx", "ddelta", "dparams", "dB", "dC", "dz", "dinitial"])
+
+
+class _SelectiveScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, delta, A, B, C, D, z, delta_bias, initial, lengths, softplus, want_state):
+        Bsz, L, dim = x.shape
+        N = A.shape[1]
+        y = torch.empty(Bsz, L, dim, device=x.device, dtype=x.dtype)
+        state = torch.empty(Bsz, dim, N, device=x.device, dtype=torch.float32) if want_state else None
+        checkpoints = torch.empty(Bsz, -(-L // _CHECKPOINT), dim, N, device=x.device, dtype=torch.float32)
+        torch.ops.spear_btp.scan_forward(x, delta, A, B, C, D, z, delta_bias, initial, lengths, y, state, checkpoints, softplus)
+        ctx.save_for_backward(x, delta, A, B, C, D, z, delta_bias, lengths, checkpoints)
+        ctx.softplus = softplus
+        ctx.set_materialize_grads(False)
+        return (y, state) if want_state else y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dstate=None):
+        x, delta, A, B, C, D, z, delta_bias, lengths, checkpoints = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        if dy is None and dstate is None:
+            return (None,) * 12
+        dev, dtype = x.device, x.dtype
+        Bsz, L, dim = x.shape
+        N = A.shape[1]
+        dy = torch.zeros(x.shape, device=dev, dtype=dtype) if dy is None else dy.contiguous()
+        dstate = dense(dstate)
+        dx, ddelta = (torch.empty(x.shape, device=dev, dtype=dtype) for _ in range(2))
+        dz = None if z is None else torch.empty(x.shape, device=dev, dtype=dtype)
+        dB, dC = (torch.empty(B.shape, device=dev, dtype=dtype) for _ in range(2))
+        dparams = torch.empty(-(-dim * (N + 2) // 4) * 4, device=dev, dtype=torch.float32)
+        dinitial = torch.empty(Bsz, dim, N, device=dev, dtype=torch.float32) if need[8] else None
+        torch.ops.spear_btp.scan_backward(x, delta, A, B, C, D, z, delta_bias, lengths, checkpoints, dy, dstate, dx, ddelta, dparams,
+                                          dB, dC, dz, dinitial, ctx.softplus)
+        dA, dD, dbias = dparams[:dim * N].view(dim, N), dparams[dim * N:dim * (N + 1)], dparams[dim * (N + 1):dim * (N + 2)]
+        grads = (dx, ddelta, dA, dB, dC, None if D is None else dD, dz, None if delta_bias is None else dbias, dinitial)
+        return (*(g if n else None for g, n in zip(grads, need)), None, None, None)
+
+
+def selective_scan(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor,
+                   D: torch.Tensor | None = None, z: torch.Tensor | None = None, *, delta_bias: torch.Tensor | None = None,
+                   delta_softplus: bool = False, initial_state: torch.Tensor | None = None, lengths: torch.Tensor | None = None,
+                   return_state: bool = False):
+    """Selective state space scan over tokens.
+
+    Args:
+        x: [B, L, D] inputs, bfloat16, float16 or float32 (views with dense channels are read in place, here and below).
+        delta: [B, L, D] step sizes before bias and softplus, in x's dtype.
+        A: [D, N] float32 rates (negative for a decaying state), 1 <= N <= 64.
+        B, C: [B, L, N] input and output weights of the states, in x's dtype; all channels share them.
+        D: [D] float32 weight of the input itself, or None.
+        z: [B, L, D] gate in x's dtype, or None: y is multiplied by silu(z).
+        delta_bias: [D] float32 added to delta, or None.
+        delta_softplus: whether the step size is softplus(delta + delta_bias).
+        initial_state: [B, D, N] float32 state before token 0, None for zeros.
+        lengths: int32 [B] on the GPU: tokens from lengths[b] on (a padded batch) are not read and give 0; values are
+            held to 0 ... L.
+        return_state: also return the state after each sequence's last token, the ``state`` of ``selective_scan_step``.
+    Returns:
+        y [B, L, D], or (y, state [B, D, N] float32).  Gradients for every floating-point argument; the backward pass
+        keeps one state per 16 tokens from the forward.
+    """
+    what = "selective_scan"
+    if x.dim() != 3 or x.shape[2] < 1:
+        raise ValueError(f"{what}: x must be [B, L, D], got {tuple(x.shape)}")
+    Bsz, L, dim = x.shape
+    _call.activation(x, f"{what}: x")
+    N = _check_params(what, dim, A, D, delta_bias)
+    _check_tokens(what, x, ((delta, "delta", (Bsz, L, dim)), (z, "z", (Bsz, L, dim)), (B, "B", (Bsz, L, N)), (C, "C", (Bsz, L, N))))
+    if initial_state is not None and (tuple(initial_state.shape) != (Bsz, dim, N) or initial_state.dtype != torch.float32):
+        raise ValueError(f"{what}: initial_state must be float32 {(Bsz, dim, N)}, got {initial_state.dtype} {tuple(initial_state.shape)}")
+    check_lengths(what, lengths, Bsz)
+    _call.on_gpu(what, x, delta, A, B, C, D, z, delta_bias, initial_state, lengths)
+    if Bsz == 0 or L == 0:  # nothing to compute; the state passes through
+        y = x * 1
+        if not return_state:
+            return y
+        return y, (torch.zeros(Bsz, dim, N, device=x.device, dtype=torch.float32) if initial_state is None else initial_state.clone())
+    x, delta, B, C, z = dense_last(x), dense_last(delta), dense_last(B), dense_last(C), dense_last(z)
+    A, D, delta_bias, initial_state, lengths = dense(A), dense(D), dense(delta_bias), dense(initial_state), dense(lengths)
+    if torch.compiler.is_compiling() or (torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in (x, delta, A, B, C, D, z, delta_bias, initial_state))):
+        return _SelectiveScan.apply(x, delta, A, B, C, D, z, delta_bias, initial_state, lengths, bool(delta_softplus), bool(return_state))
+    y = torch.empty(Bsz, L, dim, device=x.device, dtype=x.dtype)
+    state = torch.empty(Bsz, dim, N, device=x.device, dtype=torch.float32) if return_state else None
+    _launch_forward(x, delta, A, B, C, D, z, delta_bias, initial_state, lengths, y, state, None, bool(delta_softplus))
+    return (y, state) if return_state else y
+
+
+@torch.no_grad()
+def selective_scan_step(x_t: torch.Tensor, delta_t: torch.Tensor, A: torch.Tensor, B_t: torch.Tensor, C_t: torch.Tensor,
+                        state: torch.Tensor, D: torch.Tensor | None = None, z_t: torch.Tensor | None = None, *,
+                        delta_bias: torch.Tensor | None = None, delta_softplus: bool = False, state_out: torch.Tensor | None = None):
+    """One token of ``selective_scan``: returns (y_t [B, D], new state [B, D, N] float32).
+
+    x_t, delta_t, z_t [B, D] and B_t, C_t [B, N] as there, without the token dimension.  One kernel launch.  ``state``
+    stays valid and the new state is a fresh tensor, unless ``state_out`` says where to write it: passing the state
+    itself updates it in place (the form for a captured graph).
+    """
+    what = "selective_scan_step"
+    if x_t.dim() != 2 or x_t.shape[1] < 1:
+        raise ValueError(f"{what}: x_t must be [B, D], got {tuple(x_t.shape)}")
+    Bsz, dim = x_t.shape
+    _call.activation(x_t, f"{what}: x_t")
+    N = _check_params(what, dim, A, D, delta_bias)
+    _check_tokens(what, x_t, ((delta_t, "delta_t", (Bsz, dim)), (z_t, "z_t", (Bsz, dim)), (B_t, "B_t", (Bsz, N)), (C_t, "C_t", (Bsz, N))))
+    if tuple(state.shape) != (Bsz, dim, N) or state.dtype != torch.float32 or not state.is_contiguous():
+        raise ValueError(f"{what}: state must be contiguous float32 {(Bsz, dim, N)}, got {state.dtype} {tuple(state.shape)}")
+    index = _call.on_gpu(what, x_t, delta_t, A, B_t, C_t, state, D, z_t, delta_bias)
+    out = check_state_out(what, state, state_out)
+    y = torch.empty(Bsz, dim, device=x_t.device, dtype=x_t.dtype)
+    if Bsz == 0:
+        return y, out
+    if (state.data_ptr() | out.data_ptr()) % 16:
+        raise ValueError(f"{what}: state and state_out must be 16-byte aligned")
+    x_t, delta_t, B_t, C_t, z_t = dense_last(x_t), dense_last(delta_t), dense_last(B_t), dense_last(C_t), dense_last(z_t)
+    A, D, delta_bias = _aligned(dense(A)), dense(D), dense(delta_bias)
+    p = _call.ptr
+    _call.call("btp_sm100_scan_step", index, x_t.data_ptr(), delta_t.data_ptr(), A.data_ptr(), B_t.data_ptr(), C_t.data_ptr(), p(D),
+               p(z_t), p(delta_bias), state.data_ptr(), y.data_ptr(), out.data_ptr(), Bsz, dim, N, x_t.stride(0), delta_t.stride(0),
+               B_t.stride(0), C_t.stride(0), 0 if z_t is None else z_t.stride(0), int(bool(delta_softplus)), _call.TAG[x_t.dtype])
+    return y, out
