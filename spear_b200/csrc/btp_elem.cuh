@@ -80,22 +80,6 @@ constexpr float kLog2e = 1.4426950408889634f;
 // 1 / (1 + e^-v); the exponent's rounding makes it |v| 2^-24 off relative for very negative v, a few 2^-24 elsewhere.
 __device__ __forceinline__ float sigmoid(float v) { return rcp(1.f + ex2(-v * kLog2e)); }
 
-// log(1 + e^v) to a few units in the last place, without overflow:  max(v, 0) + log(1 + w) with w = e^-|v| <= 1, and
-// log(1 + w) = 2 atanh(s), s = w / (2 + w) <= 1/3, by the series s + s^3/3 + s^5/5 + ... up to s^15 (the rest is below 2^-28).
-__device__ __forceinline__ float softplus(float v) {
-  const float w = ex2(-fabsf(v) * kLog2e);
-  const float s = w * rcp(2.f + w), q = s * s;
-  float p = 2.f / 15.f;
-  p = fmaf(p, q, 2.f / 13.f);
-  p = fmaf(p, q, 2.f / 11.f);
-  p = fmaf(p, q, 2.f / 9.f);
-  p = fmaf(p, q, 2.f / 7.f);
-  p = fmaf(p, q, 2.f / 5.f);
-  p = fmaf(p, q, 2.f / 3.f);
-  p = fmaf(p, q, 2.f);
-  return (v < 0.f ? 0.f : v) + p * s;  // not fmaxf: NaN stays
-}
-
 // Two floats side by side in one 64-bit register pair: one instruction does the arithmetic of both.
 using f32x2 = unsigned long long;
 __device__ __forceinline__ f32x2 pack2(float lo, float hi) {
@@ -130,6 +114,52 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
   return r;
 }
 __device__ __forceinline__ f32x2 ex2_2(f32x2 v) { return pack2(ex2(lo2(v)), ex2(hi2(v))); }
+
+__device__ __forceinline__ f32x2 both(float v) { return pack2(v, v); }
+
+// log(1 + e^v) = max(v, 0) + log(1 + w) with w = e^-|v| in (0, 1]: no overflow, and relative accuracy where it is small, since
+// log(1 + w) = w P(w).  P: degree 8 through the Chebyshev nodes of log(1 + w) / w on [0, 1], off by 3e-8 relative.
+#define BTP_LOG1P_COEFFICIENTS \
+  {1.f, -0.499995023f, 0.333192706f, -0.248443693f, 0.191114306f, -0.136747703f, 0.0783616677f, -0.0295885075f, 0.00525345793f}
+__device__ __forceinline__ float softplus(float v) {
+  constexpr float kLog1p[9] = BTP_LOG1P_COEFFICIENTS;
+  const float w = ex2(-fabsf(v) * kLog2e);
+  float p = kLog1p[8];
+#pragma unroll
+  for (int i = 7; i >= 0; --i) p = fmaf(p, w, kLog1p[i]);
+  return fmaf(p, w, fmaxf(v, 0.f));  // a NaN stays: w is NaN
+}
+__device__ __forceinline__ f32x2 softplus2(f32x2 v) {
+  constexpr float kLog1p[9] = BTP_LOG1P_COEFFICIENTS;
+  float a, b;
+  unpack2(a, b, v);
+  const f32x2 w = ex2_2(pack2(-fabsf(a) * kLog2e, -fabsf(b) * kLog2e));
+  f32x2 p = both(kLog1p[8]);
+#pragma unroll
+  for (int i = 7; i >= 0; --i) p = fma2(p, w, both(kLog1p[i]));
+  return fma2(p, w, pack2(fmaxf(a, 0.f), fmaxf(b, 0.f)));
+}
+__device__ __forceinline__ f32x2 sigmoid2(f32x2 v) {
+  const f32x2 e = add2(ex2_2(mul2(v, both(-kLog2e))), both(1.f));
+  return pack2(rcp(lo2(e)), rcp(hi2(e)));
+}
+
+// Two neighbouring elements of an array whose element 0 is aligned to the pair, as floats, and back.
+__device__ __forceinline__ f32x2 load_pair(const float* p) { return *reinterpret_cast<const f32x2*>(p); }
+__device__ __forceinline__ f32x2 load_pair(const __nv_bfloat16* p) {
+  const unsigned w = *reinterpret_cast<const unsigned*>(p);
+  return pack2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ f32x2 load_pair(const __half* p) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(p));
+  return pack2(f.x, f.y);
+}
+template <class T>
+__device__ __forceinline__ void store_pair(T* p, f32x2 v, bool aligned, int count) {
+  float f[2];
+  unpack2(f[0], f[1], v);
+  store_run<T, 2>(p, f, aligned, count);
+}
 
 // Tokens of sequence b that are there: `lengths` may be null (all L), its values are held to 0 ... L.
 __device__ __forceinline__ int tokens_of(const int* lengths, long long b, int L) {

@@ -61,7 +61,7 @@ struct Tile {
   T C[2][kTile][kStates];
   float delta[kTile][kChannels];
   float u[kTile][kChannels];
-  float y[kTile][kChannels];
+  float y[kTile][kChannels + 8];  // the odd pitch keeps the four rows that a group stores at once in different banks
   float B2[kTile][kStates * 2];
   float C2[kTile][kStates * 2];
 };
@@ -125,6 +125,49 @@ __device__ __forceinline__ void reduce_states(float (&out)[2], f32x2 v0, f32x2 v
   out[1] = 0.f;
 }
 
+// v[j][c]: pair c of this lane's channels at token j of a group of 4, to be summed over the SG lanes of the state group and
+// stored at row[j][4 g ..].  Lanes exchange halves: first tokens, then (from 8 lanes on) pairs, then channels.
+template <int SG, int PITCH>
+__device__ __forceinline__ void reduce_tokens(float (*row)[PITCH], const f32x2 (&v)[4][2], int g, int s) {
+  f32x2 a[2][2];
+  const bool up = s & (SG / 2);
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const f32x2 keep = up ? v[2 + j][c] : v[j][c], give = up ? v[j][c] : v[2 + j][c];
+      a[j][c] = add2(keep, __shfl_xor_sync(0xffffffffu, give, SG / 2));
+    }
+  int t = up ? 2 : 0;
+  if (SG == 2) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) *reinterpret_cast<ulonglong2*>(&row[t + j][4 * g]) = make_ulonglong2(a[j][0], a[j][1]);
+    return;
+  }
+  f32x2 b[2];
+  const bool odd = s & (SG / 4);
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const f32x2 keep = odd ? a[1][c] : a[0][c], give = odd ? a[0][c] : a[1][c];
+    b[c] = add2(keep, __shfl_xor_sync(0xffffffffu, give, SG / 4));
+  }
+  t += odd ? 1 : 0;
+  if (SG == 4) {
+    *reinterpret_cast<ulonglong2*>(&row[t][4 * g]) = make_ulonglong2(b[0], b[1]);
+    return;
+  }
+  const bool hi = s & (SG / 8);
+  const f32x2 d = add2(hi ? b[1] : b[0], __shfl_xor_sync(0xffffffffu, hi ? b[0] : b[1], SG / 8));
+  if (SG == 8) {
+    *reinterpret_cast<f32x2*>(&row[t][4 * g + (hi ? 2 : 0)]) = d;
+    return;
+  }
+  float x, y;
+  unpack2(x, y, d);
+  const bool last = s & 1;
+  row[t][4 * g + (hi ? 2 : 0) + (last ? 1 : 0)] = (last ? y : x) + __shfl_xor_sync(0xffffffffu, last ? x : y, 1);
+}
+
 // Four consecutive states of one channel of a [.., N] row; states from N on are 0.
 __device__ __forceinline__ void load_states(float (&v)[4], const float* row, int n0, int N) {
   if ((N & 3) == 0) {
@@ -173,6 +216,16 @@ __device__ __forceinline__ void store_lane(float* base, const LaneState& h, int 
     if (c0 + 2 * p + 1 < dim) store_states(base + static_cast<long long>(c0 + 2 * p + 1) * N, b, n0, N);
   }
 }
+// Rates to the base 2, held above -inf so that a step of size 0 keeps the state.
+__device__ __forceinline__ void load_rates(LaneState& A2, const float* A, int c0, int dim, int n0, int N) {
+  load_lane(A2, A, c0, dim, n0, N, kLog2e);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float a, b;
+    unpack2(a, b, A2.r[i >> 2][i & 3]);
+    A2.r[i >> 2][i & 3] = pack2(a < -3e38f ? -3e38f : a, b < -3e38f ? -3e38f : b);
+  }
+}
 // h = exp(A total) h + last: the effect of a whole chunk with step sizes that sum up to `total`.
 __device__ __forceinline__ void apply_chunk(LaneState& h, const LaneState& A2, const LaneState& last, f32x2 t0, f32x2 t1) {
 #pragma unroll
@@ -193,6 +246,10 @@ __device__ __forceinline__ void clear_padding(LaneState& h, int n0, int N) {
 #pragma unroll
   for (int n = 0; n < 4; ++n)
     if (n0 + n >= N) h.r[0][n] = h.r[1][n] = 0ull;
+}
+
+__device__ __forceinline__ f32x2 channel_pair(const float* v, int c, int dim) {
+  return pack2(v && c < dim ? v[c] : 0.f, v && c + 1 < dim ? v[c + 1] : 0.f);
 }
 
 // One warp per (channels, chunk, sequence).  CARRY: only the chunk's last state and sum of step sizes, from state zero.
@@ -217,7 +274,7 @@ __global__ void __launch_bounds__(32) scan_forward_kernel(const ScanParams p) {
   const bool full = p.N == NP;
 
   LaneState A2, h;
-  load_lane(A2, p.A, c0, p.dim, n0, p.N, kLog2e);
+  load_rates(A2, p.A, c0, p.dim, n0, p.N);
   if (CARRY || !p.initial) {
 #pragma unroll
     for (int n = 0; n < 4; ++n) h.r[0][n] = h.r[1][n] = 0ull;
@@ -237,11 +294,10 @@ __global__ void __launch_bounds__(32) scan_forward_kernel(const ScanParams p) {
   }
   // this lane's channel pair in the passes over a tile
   const int cp = lane % CP, row0 = lane / CP, pc = cw + 2 * cp;
-  float bias[2], skip[2];
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    bias[k] = p.bias && pc + k < p.dim ? p.bias[pc + k] : 0.f;
-    skip[k] = p.D && pc + k < p.dim ? p.D[pc + k] : 0.f;
+  const f32x2 bias = channel_pair(p.bias, pc, p.dim), skip = channel_pair(p.D, pc, p.dim);
+  for (int i = lane; i < 2 * kTile * (WC - cols); i += 32) {  // channels that are not there: never copied, read as zeros
+    const int at = i / (WC - cols) * WC + cols + i % (WC - cols);
+    (&sm.x[0][0][0])[at] = (&sm.d[0][0][0])[at] = (&sm.z[0][0][0])[at] = from_f<T>(0.f);
   }
   const T* x = static_cast<const T*>(p.x) + b * p.x_b + cw;
   const T* dl = static_cast<const T*>(p.delta) + b * p.d_b + cw;
@@ -273,66 +329,64 @@ __global__ void __launch_bounds__(32) scan_forward_kernel(const ScanParams p) {
       const long long at = b * ((p.L + kCheckpoint - 1) / kCheckpoint) + t0 / kCheckpoint;
       store_lane(p.checkpoints + at * p.dim * p.N, h, c0, p.dim, n0, p.N);
     }
+    // raw values to step sizes, inputs and doubled B, C; rows behind the last token become zeros, which leave the state as it is
 #pragma unroll
     for (int i = 0; i < kTile; i += RPI) {
       const int r = i + row0;
-      float de[2], uu[2];
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const bool ok = r < nt && pc + k < p.dim;
-        float v = ok ? to_f(sm.d[st][r][2 * cp + k]) + bias[k] : 0.f;
-        if (p.softplus) v = softplus(v);
-        de[k] = ok ? v : 0.f;
-        uu[k] = ok ? v * to_f(sm.x[st][r][2 * cp + k]) : 0.f;
-      }
-      *reinterpret_cast<float2*>(&sm.delta[r][2 * cp]) = make_float2(de[0], de[1]);
-      *reinterpret_cast<float2*>(&sm.u[r][2 * cp]) = make_float2(uu[0], uu[1]);
+      f32x2 v = add2(load_pair(&sm.d[st][r][2 * cp]), bias);
+      if (p.softplus) v = softplus2(v);
+      f32x2 w = mul2(v, load_pair(&sm.x[st][r][2 * cp]));
+      if (nt < kTile && r >= nt) v = w = 0ull;
+      *reinterpret_cast<f32x2*>(&sm.delta[r][2 * cp]) = v;
+      *reinterpret_cast<f32x2*>(&sm.u[r][2 * cp]) = w;
     }
 #pragma unroll
     for (int i = 0; i < kTile * NP / 2; i += 32) {
       const int r = (i + lane) / (NP / 2), n = (i + lane) % (NP / 2) * 2;
+      float b0, b1;
+      unpack2(b0, b1, load_pair(&sm.B[st][r][n]));
       const bool ok0 = r < nt && n < p.N, ok1 = r < nt && n + 1 < p.N;
-      const float b0 = ok0 ? to_f(sm.B[st][r][n]) : 0.f, b1 = ok1 ? to_f(sm.B[st][r][n + 1]) : 0.f;
+      b0 = ok0 ? b0 : 0.f, b1 = ok1 ? b1 : 0.f;
       *reinterpret_cast<float4*>(&sm.B2[r][2 * n]) = make_float4(b0, b0, b1, b1);
       if (!CARRY) {
-        const float e0 = ok0 ? to_f(sm.C[st][r][n]) : 0.f, e1 = ok1 ? to_f(sm.C[st][r][n + 1]) : 0.f;
-        *reinterpret_cast<float4*>(&sm.C2[r][2 * n]) = make_float4(e0, e0, e1, e1);
+        unpack2(b0, b1, load_pair(&sm.C[st][r][n]));
+        b0 = ok0 ? b0 : 0.f, b1 = ok1 ? b1 : 0.f;
+        *reinterpret_cast<float4*>(&sm.C2[r][2 * n]) = make_float4(b0, b0, b1, b1);
       }
     }
     __syncwarp();
-#pragma unroll 4
-    for (int t = 0; t < nt; ++t) {
-      const ulonglong2 d2 = *reinterpret_cast<const ulonglong2*>(&sm.delta[t][4 * g]);
-      const ulonglong2 u2 = *reinterpret_cast<const ulonglong2*>(&sm.u[t][4 * g]);
-      const ulonglong2 ba = *reinterpret_cast<const ulonglong2*>(&sm.B2[t][8 * s]);
-      const ulonglong2 bb = *reinterpret_cast<const ulonglong2*>(&sm.B2[t][8 * s + 4]);
-      const f32x2 bn[4] = {ba.x, ba.y, bb.x, bb.y};
+    // four tokens at a time: no store lies between them, so their loads and exponentials overlap
+    for (int t = 0; t < nt; t += 4) {
+      f32x2 yv[4][2];
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        h.r[0][n] = fma2(ex2_2(mul2(d2.x, A2.r[0][n])), h.r[0][n], mul2(u2.x, bn[n]));
-        h.r[1][n] = fma2(ex2_2(mul2(d2.y, A2.r[1][n])), h.r[1][n], mul2(u2.y, bn[n]));
-      }
-      if (!full) clear_padding(h, n0, p.N);
-      if (CARRY) {
-        sum0 = add2(sum0, d2.x);
-        sum1 = add2(sum1, d2.y);
-      } else {
-        const ulonglong2 ca = *reinterpret_cast<const ulonglong2*>(&sm.C2[t][8 * s]);
-        const ulonglong2 cc = *reinterpret_cast<const ulonglong2*>(&sm.C2[t][8 * s + 4]);
-        const f32x2 cn[4] = {ca.x, ca.y, cc.x, cc.y};
-        f32x2 y0 = mul2(cn[0], h.r[0][0]), y1 = mul2(cn[0], h.r[1][0]);
+      for (int j = 0; j < 4; ++j) {
+        const ulonglong2 d2 = *reinterpret_cast<const ulonglong2*>(&sm.delta[t + j][4 * g]);
+        const ulonglong2 u2 = *reinterpret_cast<const ulonglong2*>(&sm.u[t + j][4 * g]);
+        const ulonglong2 ba = *reinterpret_cast<const ulonglong2*>(&sm.B2[t + j][8 * s]);
+        const ulonglong2 bb = *reinterpret_cast<const ulonglong2*>(&sm.B2[t + j][8 * s + 4]);
+        const f32x2 bn[4] = {ba.x, ba.y, bb.x, bb.y};
 #pragma unroll
-        for (int n = 1; n < 4; ++n) {
-          y0 = fma2(cn[n], h.r[0][n], y0);
-          y1 = fma2(cn[n], h.r[1][n], y1);
+        for (int n = 0; n < 4; ++n) {
+          h.r[0][n] = fma2(ex2_2(mul2(d2.x, A2.r[0][n])), h.r[0][n], mul2(u2.x, bn[n]));
+          h.r[1][n] = fma2(ex2_2(mul2(d2.y, A2.r[1][n])), h.r[1][n], mul2(u2.y, bn[n]));
         }
-        float out[2];
-        reduce_states<SG>(out, y0, y1, s);
-        if (SG == 2)
-          *reinterpret_cast<float2*>(&sm.y[t][4 * g + 2 * s]) = make_float2(out[0], out[1]);
-        else if (SG == 4 || s < 4)
-          sm.y[t][4 * g + (s & 3)] = out[0];
+        if (!full) clear_padding(h, n0, p.N);
+        if (CARRY) {
+          sum0 = add2(sum0, d2.x);
+          sum1 = add2(sum1, d2.y);
+        } else {
+          const ulonglong2 ca = *reinterpret_cast<const ulonglong2*>(&sm.C2[t + j][8 * s]);
+          const ulonglong2 cc = *reinterpret_cast<const ulonglong2*>(&sm.C2[t + j][8 * s + 4]);
+          const f32x2 cn[4] = {ca.x, ca.y, cc.x, cc.y};
+          yv[j][0] = mul2(cn[0], h.r[0][0]), yv[j][1] = mul2(cn[0], h.r[1][0]);
+#pragma unroll
+          for (int n = 1; n < 4; ++n) {
+            yv[j][0] = fma2(cn[n], h.r[0][n], yv[j][0]);
+            yv[j][1] = fma2(cn[n], h.r[1][n], yv[j][1]);
+          }
+        }
       }
+      if (!CARRY) reduce_tokens<SG>(&sm.y[t], yv, g, s);
     }
     __syncwarp();
     if (!CARRY) {
@@ -340,16 +394,12 @@ __global__ void __launch_bounds__(32) scan_forward_kernel(const ScanParams p) {
       for (int i = 0; i < kTile; i += RPI) {
         const int r = i + row0;
         if (r >= nt || pc >= p.dim) continue;
-        float out[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          out[k] = fmaf(skip[k], to_f(sm.x[st][r][2 * cp + k]), sm.y[r][2 * cp + k]);
-          if (z) {
-            const float zz = to_f(sm.z[st][r][2 * cp + k]);
-            out[k] *= zz * sigmoid(zz);
-          }
+        f32x2 out = fma2(skip, load_pair(&sm.x[st][r][2 * cp]), *reinterpret_cast<const f32x2*>(&sm.y[r][2 * cp]));
+        if (z) {
+          const f32x2 zz = load_pair(&sm.z[st][r][2 * cp]);
+          out = mul2(out, mul2(zz, sigmoid2(zz)));
         }
-        store_run<T, 2>(y + static_cast<long long>(t0 + r) * p.dim + 2 * cp, out, p.al_y, p.dim - pc);
+        store_pair<T>(y + static_cast<long long>(t0 + r) * p.dim + 2 * cp, out, p.al_y, p.dim - pc);
       }
     }
     __syncwarp();
