@@ -19,6 +19,8 @@
 // scan_sm100.cu splits only where warps are missing.
 #pragma once
 
+#include <type_traits>
+
 #include "btp_elem.cuh"
 
 namespace btp_scan {
@@ -61,13 +63,15 @@ struct Tile {
   T C[2][kTile][kStates];
   float delta[kTile][kChannels];
   float u[kTile][kChannels];
-  float y[kTile][kChannels + 8];  // the odd pitch keeps the four rows that a group stores at once in different banks
   float B2[kTile][kStates * 2];
   float C2[kTile][kStates * 2];
 };
 
 __device__ __forceinline__ void copy16(void* to, const void* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy8(void* to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from) : "memory");
 }
 __device__ __forceinline__ void copy4(void* to, const void* from) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from) : "memory");
@@ -82,12 +86,18 @@ __device__ __forceinline__ void copy_wait() {
 // GROUP threads.  Rows from `rows` on and columns from `cols` on are not touched.
 template <class T, int ROWS, int COLS, int GROUP>
 __device__ __forceinline__ void fetch(T (*dst)[COLS], const T* src, long long pitch, int rows, int cols, bool aligned, int tid) {
-  constexpr int E = 16 / static_cast<int>(sizeof(T)), CPR = COLS / E;
+  constexpr int kBytes = COLS * static_cast<int>(sizeof(T)) < 16 ? 8 : 16, E = kBytes / static_cast<int>(sizeof(T)), CPR = COLS / E;
+  static_assert(COLS % E == 0 && CPR >= 1, "a row is whole copies");
   if (aligned) {
 #pragma unroll
     for (int i0 = 0; i0 < ROWS * CPR; i0 += GROUP) {
       const int i = i0 + tid, r = i / CPR, c = (i - r * CPR) * E;
-      if ((ROWS * CPR % GROUP == 0 || i < ROWS * CPR) && r < rows && c < cols) copy16(&dst[r][c], src + r * pitch + c);
+      if ((ROWS * CPR % GROUP == 0 || i < ROWS * CPR) && r < rows && c < cols) {
+        if (kBytes == 16)
+          copy16(&dst[r][c], src + r * pitch + c);
+        else
+          copy8(&dst[r][c], src + r * pitch + c);
+      }
     }
   } else {
 #pragma unroll 4
@@ -123,49 +133,6 @@ __device__ __forceinline__ void reduce_states(float (&out)[2], f32x2 v0, f32x2 v
   if (SG >= 16) r += __shfl_xor_sync(0xffffffffu, r, 8);
   out[0] = r;
   out[1] = 0.f;
-}
-
-// v[j][c]: pair c of this lane's channels at token j of a group of 4, to be summed over the SG lanes of the state group and
-// stored at row[j][4 g ..].  Lanes exchange halves: first tokens, then (from 8 lanes on) pairs, then channels.
-template <int SG, int PITCH>
-__device__ __forceinline__ void reduce_tokens(float (*row)[PITCH], const f32x2 (&v)[4][2], int g, int s) {
-  f32x2 a[2][2];
-  const bool up = s & (SG / 2);
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const f32x2 keep = up ? v[2 + j][c] : v[j][c], give = up ? v[j][c] : v[2 + j][c];
-      a[j][c] = add2(keep, __shfl_xor_sync(0xffffffffu, give, SG / 2));
-    }
-  int t = up ? 2 : 0;
-  if (SG == 2) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j) *reinterpret_cast<ulonglong2*>(&row[t + j][4 * g]) = make_ulonglong2(a[j][0], a[j][1]);
-    return;
-  }
-  f32x2 b[2];
-  const bool odd = s & (SG / 4);
-#pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    const f32x2 keep = odd ? a[1][c] : a[0][c], give = odd ? a[0][c] : a[1][c];
-    b[c] = add2(keep, __shfl_xor_sync(0xffffffffu, give, SG / 4));
-  }
-  t += odd ? 1 : 0;
-  if (SG == 4) {
-    *reinterpret_cast<ulonglong2*>(&row[t][4 * g]) = make_ulonglong2(b[0], b[1]);
-    return;
-  }
-  const bool hi = s & (SG / 8);
-  const f32x2 d = add2(hi ? b[1] : b[0], __shfl_xor_sync(0xffffffffu, hi ? b[0] : b[1], SG / 8));
-  if (SG == 8) {
-    *reinterpret_cast<f32x2*>(&row[t][4 * g + (hi ? 2 : 0)]) = d;
-    return;
-  }
-  float x, y;
-  unpack2(x, y, d);
-  const bool last = s & 1;
-  row[t][4 * g + (hi ? 2 : 0) + (last ? 1 : 0)] = (last ? y : x) + __shfl_xor_sync(0xffffffffu, last ? x : y, 1);
 }
 
 // Four consecutive states of one channel of a [.., N] row; states from N on are 0.
@@ -252,11 +219,79 @@ __device__ __forceinline__ f32x2 channel_pair(const float* v, int c, int dim) {
   return pack2(v && c < dim ? v[c] : 0.f, v && c + 1 < dim ? v[c + 1] : 0.f);
 }
 
+// ---------------------------------------------------------------------------------------------------- forward
+// A lane holds 2 neighbouring channels x KN states as pairs of states; SG lanes share the channel pair.  The lane with the odd
+// index in its group takes the odd channel as its first: "own" and "other" below, so that nothing is selected by parity.
+// Of a group of 4 tokens each lane prepares kOwn tokens of its own channel (step size, input, in the end gate and output), straight
+// from the copied rows; the group's lanes pass step sizes and inputs to one another, and sums of y back, by exchanges in the warp.
+template <class T, int KN, int SG>
+struct FwdTile {
+  static constexpr int kStates = KN * SG;
+  static constexpr int kChannels = 64 / SG;
+  T x[2][kTile][kChannels];
+  T d[2][kTile][kChannels];
+  T z[2][kTile][kChannels];
+  T B[2][kTile][kStates];
+  T C[2][kTile][kStates];
+  float Bf[kTile][kStates];
+  float Cf[kTile][kStates];
+};
+
+// KN consecutive states of the channels c0, c1 as pairs; a channel or state that is not there is 0.
+template <int KN>
+struct PairState {
+  f32x2 r[2][KN / 2];
+};
+template <int KN>
+__device__ __forceinline__ void load_pair_state(PairState<KN>& h, const float* base, int c0, int c1, int dim, int n0, int N) {
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const int ch = c ? c1 : c0;
+#pragma unroll
+    for (int q = 0; q < KN / 4; ++q) {
+      float v[4] = {};
+      if (ch < dim) load_states(v, base + static_cast<long long>(ch) * N, n0 + 4 * q, N);
+      h.r[c][2 * q] = pack2(v[0], v[1]);
+      h.r[c][2 * q + 1] = pack2(v[2], v[3]);
+    }
+  }
+}
+template <int KN>
+__device__ __forceinline__ void store_pair_state(float* base, const PairState<KN>& h, int c0, int c1, int dim, int n0, int N) {
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const int ch = c ? c1 : c0;
+#pragma unroll
+    for (int q = 0; q < KN / 4; ++q) {
+      float v[4];
+      unpack2(v[0], v[1], h.r[c][2 * q]);
+      unpack2(v[2], v[3], h.r[c][2 * q + 1]);
+      if (ch < dim) store_states(base + static_cast<long long>(ch) * N, v, n0 + 4 * q, N);
+    }
+  }
+}
+template <int KN>
+__device__ __forceinline__ void clear_pair_padding(PairState<KN>& h, int n0, int N) {
+#pragma unroll
+  for (int k = 0; k < KN / 2; ++k) {
+    const int n = n0 + 2 * k;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      if (n >= N)
+        h.r[c][k] = 0ull;
+      else if (n + 1 >= N)
+        h.r[c][k] = pack2(lo2(h.r[c][k]), 0.f);
+    }
+  }
+}
+
 // One warp per (channels, chunk, sequence).  CARRY: only the chunk's last state and sum of step sizes, from state zero.
-template <class T, int SG, bool CARRY>
+template <class T, int KN, int SG, bool CARRY>
 __global__ void __launch_bounds__(32) scan_forward_kernel(const ScanParams p) {
-  using S = Tile<T, SG>;
-  constexpr int WC = S::kChannels, NP = S::kStates, CP = WC / 2, RPI = 32 / CP;  // channel pairs per row, rows per pass
+  using S = FwdTile<T, KN, SG>;
+  constexpr int WC = S::kChannels, NP = S::kStates;
+  constexpr int kOwn = SG >= 8 ? 1 : (SG == 1 ? 4 : 8 / SG);  // tokens of a group of 4 that a lane prepares
+  constexpr int kMine = SG == 1 ? 2 : 1;                      // channels that it prepares them for
   extern __shared__ __align__(16) unsigned char smem_raw[];
   S& sm = *reinterpret_cast<S*>(smem_raw);
   grid_dependency_wait();
@@ -267,34 +302,49 @@ __global__ void __launch_bounds__(32) scan_forward_kernel(const ScanParams p) {
   const int rest = blockIdx.x / cblocks;
   const int q = rest % splits;
   const long long b = rest / splits;
-  const int cw = cb * WC, c0 = cw + 4 * g, n0 = 4 * s;
+  const int cw = cb * WC, odd = s & 1;
+  const int l0 = 2 * g + odd, l1 = 2 * g + 1 - odd;  // own and other channel within the warp's
+  const int c0 = cw + l0, c1 = cw + l1, n0 = KN * s;
   const int n_tok = tokens_of(p.lengths, b, p.L);
   const int first = q * p.chunk, end = min(p.L, first + p.chunk), live = min(end, n_tok);
   const int cols = min(WC, p.dim - cw);
   const bool full = p.N == NP;
 
-  LaneState A2, h;
-  load_rates(A2, p.A, c0, p.dim, n0, p.N);
-  if (CARRY || !p.initial) {
+  PairState<KN> A2, h;
+  load_pair_state(A2, p.A, c0, c1, p.dim, n0, p.N);
 #pragma unroll
-    for (int n = 0; n < 4; ++n) h.r[0][n] = h.r[1][n] = 0ull;
-  } else {
-    load_lane(h, p.initial + b * p.dim * p.N, c0, p.dim, n0, p.N, 1.f);
-  }
+  for (int c = 0; c < 2; ++c)
+#pragma unroll
+    for (int k = 0; k < KN / 2; ++k) {  // rates to the base 2, held above -inf so that a step of size 0 keeps the state
+      float a, e;
+      unpack2(a, e, mul2(A2.r[c][k], both(kLog2e)));
+      A2.r[c][k] = pack2(a < -3e38f ? -3e38f : a, e < -3e38f ? -3e38f : e);
+      h.r[c][k] = 0ull;
+    }
+  if (!CARRY && p.initial) load_pair_state(h, p.initial + b * p.dim * p.N, c0, c1, p.dim, n0, p.N);
   const long long per_chunk = static_cast<long long>(p.batch) * p.dim;
   float* totals = p.carry + (p.splits - 1) * per_chunk * p.N;
   if (!CARRY) {
-    for (int k = 0; k < q; ++k) {
-      LaneState last;
-      f32x2 t0, t1;
-      load_lane(last, p.carry + (k * per_chunk + b * p.dim) * p.N, c0, p.dim, n0, p.N, 1.f);
-      load_totals(t0, t1, totals + k * per_chunk + b * p.dim, c0, p.dim);
-      apply_chunk(h, A2, last, t0, t1);
+    for (int k = 0; k < q; ++k) {  // the chunks before, in order: h = exp(A total) h + last
+      PairState<KN> last;
+      load_pair_state(last, p.carry + (k * per_chunk + b * p.dim) * p.N, c0, c1, p.dim, n0, p.N);
+      const float* row = totals + k * per_chunk + b * p.dim;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int ch = c ? c1 : c0;
+        const f32x2 total = both(ch < p.dim ? row[ch] : 0.f);
+#pragma unroll
+        for (int i = 0; i < KN / 2; ++i) h.r[c][i] = fma2(ex2_2(mul2(A2.r[c][i], total)), h.r[c][i], last.r[c][i]);
+      }
     }
   }
-  // this lane's channel pair in the passes over a tile
-  const int cp = lane % CP, row0 = lane / CP, pc = cw + 2 * cp;
-  const f32x2 bias = channel_pair(p.bias, pc, p.dim), skip = channel_pair(p.D, pc, p.dim);
+  float bias[kMine], skip[kMine];
+#pragma unroll
+  for (int m = 0; m < kMine; ++m) {
+    const int ch = m ? c1 : c0;
+    bias[m] = p.bias && ch < p.dim ? p.bias[ch] : 0.f;
+    skip[m] = p.D && ch < p.dim ? p.D[ch] : 0.f;
+  }
   for (int i = lane; i < 2 * kTile * (WC - cols); i += 32) {  // channels that are not there: never copied, read as zeros
     const int at = i / (WC - cols) * WC + cols + i % (WC - cols);
     (&sm.x[0][0][0])[at] = (&sm.d[0][0][0])[at] = (&sm.z[0][0][0])[at] = from_f<T>(0.f);
@@ -315,7 +365,14 @@ __global__ void __launch_bounds__(32) scan_forward_kernel(const ScanParams p) {
       if (z) fetch<T, kTile, WC, 32>(sm.z[st], z + t0 * p.z_t, p.z_t, rows, cols, p.al_z, lane);
     }
   };
-  f32x2 sum0 = 0ull, sum1 = 0ull;
+  float total[kMine] = {};
+  const int mine = SG == 1 ? 0 : (s >> 1) * kOwn & 3;       // first token of each group that this lane prepares
+  const int own_src = g * SG + odd, oth_src = g * SG + 1 - odd;  // lanes that prepare token 0 of the own and the other channel
+  // The walk over the chunk, once for the usual case (all states there, softplus, gate or not known) and once with everything tested:
+  // a branch per token would keep the tokens of a group from overlapping.
+  const auto walk = [&](auto usual, auto gated) {
+  constexpr bool kFull = decltype(usual)::value;
+  const bool softplus_on = kFull || p.softplus, gate_on = kFull ? decltype(gated)::value : z != nullptr;
   if (first < live) load_tile(0, first);
   copy_commit();
   int st = 0;
@@ -327,101 +384,164 @@ __global__ void __launch_bounds__(32) scan_forward_kernel(const ScanParams p) {
     const int nt = min(kTile, live - t0);
     if (!CARRY && p.checkpoints && t0 % kCheckpoint == 0) {
       const long long at = b * ((p.L + kCheckpoint - 1) / kCheckpoint) + t0 / kCheckpoint;
-      store_lane(p.checkpoints + at * p.dim * p.N, h, c0, p.dim, n0, p.N);
+      store_pair_state(p.checkpoints + at * p.dim * p.N, h, c0, c1, p.dim, n0, p.N);
     }
-    // raw values to step sizes, inputs and doubled B, C; rows behind the last token become zeros, which leave the state as it is
+    // B and C to float; rows behind the last token and states that are not there become zeros
 #pragma unroll
-    for (int i = 0; i < kTile; i += RPI) {
-      const int r = i + row0;
-      f32x2 v = add2(load_pair(&sm.d[st][r][2 * cp]), bias);
-      if (p.softplus) v = softplus2(v);
-      f32x2 w = mul2(v, load_pair(&sm.x[st][r][2 * cp]));
-      if (nt < kTile && r >= nt) v = w = 0ull;
-      *reinterpret_cast<f32x2*>(&sm.delta[r][2 * cp]) = v;
-      *reinterpret_cast<f32x2*>(&sm.u[r][2 * cp]) = w;
-    }
-#pragma unroll
-    for (int i = 0; i < kTile * NP / 2; i += 32) {
-      const int r = (i + lane) / (NP / 2), n = (i + lane) % (NP / 2) * 2;
-      float b0, b1;
-      unpack2(b0, b1, load_pair(&sm.B[st][r][n]));
+    for (int i0 = 0; i0 < kTile * NP / 2; i0 += 32) {
+      const int i = i0 + lane, r = i / (NP / 2), n = i % (NP / 2) * 2;
       const bool ok0 = r < nt && n < p.N, ok1 = r < nt && n + 1 < p.N;
-      b0 = ok0 ? b0 : 0.f, b1 = ok1 ? b1 : 0.f;
-      *reinterpret_cast<float4*>(&sm.B2[r][2 * n]) = make_float4(b0, b0, b1, b1);
+      float v0, v1;
+      unpack2(v0, v1, load_pair(&sm.B[st][r][n]));
+      *reinterpret_cast<float2*>(&sm.Bf[r][n]) = make_float2(ok0 ? v0 : 0.f, ok1 ? v1 : 0.f);
       if (!CARRY) {
-        unpack2(b0, b1, load_pair(&sm.C[st][r][n]));
-        b0 = ok0 ? b0 : 0.f, b1 = ok1 ? b1 : 0.f;
-        *reinterpret_cast<float4*>(&sm.C2[r][2 * n]) = make_float4(b0, b0, b1, b1);
+        unpack2(v0, v1, load_pair(&sm.C[st][r][n]));
+        *reinterpret_cast<float2*>(&sm.Cf[r][n]) = make_float2(ok0 ? v0 : 0.f, ok1 ? v1 : 0.f);
       }
     }
     __syncwarp();
-    // four tokens at a time: no store lies between them, so their loads and exponentials overlap
     for (int t = 0; t < nt; t += 4) {
-      f32x2 yv[4][2];
+      float de[kMine][kOwn], xx[kMine][kOwn], uu[kMine][kOwn];
+#pragma unroll
+      for (int m = 0; m < kMine; ++m) {
+        const int col = m ? l1 : l0;
+#pragma unroll
+        for (int k = 0; k < kOwn; ++k) {
+          de[m][k] = to_f(sm.d[st][t + mine + k][col]) + bias[m];
+          xx[m][k] = to_f(sm.x[st][t + mine + k][col]);
+        }
+        if (softplus_on) {
+          if (kOwn == 1) {
+            de[m][0] = softplus(de[m][0]);
+          } else {
+#pragma unroll
+            for (int k = 0; k < kOwn; k += 2) unpack2(de[m][k], de[m][k + 1], softplus2(pack2(de[m][k], de[m][k + 1])));
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < kOwn; ++k) {
+          uu[m][k] = de[m][k] * xx[m][k];
+          if (nt < kTile && t + mine + k >= nt) de[m][k] = uu[m][k] = 0.f;  // they leave the state as it is
+          total[m] += de[m][k];
+        }
+      }
+      float yo[4], yt[4];  // sums of the own and the other channel
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const ulonglong2 d2 = *reinterpret_cast<const ulonglong2*>(&sm.delta[t + j][4 * g]);
-        const ulonglong2 u2 = *reinterpret_cast<const ulonglong2*>(&sm.u[t + j][4 * g]);
-        const ulonglong2 ba = *reinterpret_cast<const ulonglong2*>(&sm.B2[t + j][8 * s]);
-        const ulonglong2 bb = *reinterpret_cast<const ulonglong2*>(&sm.B2[t + j][8 * s + 4]);
-        const f32x2 bn[4] = {ba.x, ba.y, bb.x, bb.y};
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          h.r[0][n] = fma2(ex2_2(mul2(d2.x, A2.r[0][n])), h.r[0][n], mul2(u2.x, bn[n]));
-          h.r[1][n] = fma2(ex2_2(mul2(d2.y, A2.r[1][n])), h.r[1][n], mul2(u2.y, bn[n]));
-        }
-        if (!full) clear_padding(h, n0, p.N);
-        if (CARRY) {
-          sum0 = add2(sum0, d2.x);
-          sum1 = add2(sum1, d2.y);
+        float dc[2], uc[2];
+        if (SG == 1) {
+          dc[0] = de[0][j], dc[1] = de[kMine - 1][j], uc[0] = uu[0][j], uc[1] = uu[kMine - 1][j];
+        } else if (SG == 2) {
+          dc[0] = de[0][j % kOwn], uc[0] = uu[0][j % kOwn];
+          dc[1] = __shfl_xor_sync(0xffffffffu, dc[0], 1);
+          uc[1] = __shfl_xor_sync(0xffffffffu, uc[0], 1);
         } else {
-          const ulonglong2 ca = *reinterpret_cast<const ulonglong2*>(&sm.C2[t + j][8 * s]);
-          const ulonglong2 cc = *reinterpret_cast<const ulonglong2*>(&sm.C2[t + j][8 * s + 4]);
-          const f32x2 cn[4] = {ca.x, ca.y, cc.x, cc.y};
-          yv[j][0] = mul2(cn[0], h.r[0][0]), yv[j][1] = mul2(cn[0], h.r[1][0]);
+          const int up = 2 * (j / kOwn);
+          dc[0] = __shfl_sync(0xffffffffu, de[0][j % kOwn], own_src + up);
+          dc[1] = __shfl_sync(0xffffffffu, de[0][j % kOwn], oth_src + up);
+          uc[0] = __shfl_sync(0xffffffffu, uu[0][j % kOwn], own_src + up);
+          uc[1] = __shfl_sync(0xffffffffu, uu[0][j % kOwn], oth_src + up);
+        }
+        f32x2 bn[KN / 2], cn[KN / 2];
 #pragma unroll
-          for (int n = 1; n < 4; ++n) {
-            yv[j][0] = fma2(cn[n], h.r[0][n], yv[j][0]);
-            yv[j][1] = fma2(cn[n], h.r[1][n], yv[j][1]);
+        for (int k = 0; k < KN / 4; ++k) {
+          const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&sm.Bf[t + j][n0 + 4 * k]);
+          bn[2 * k] = v.x, bn[2 * k + 1] = v.y;
+          if (!CARRY) {
+            const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(&sm.Cf[t + j][n0 + 4 * k]);
+            cn[2 * k] = w.x, cn[2 * k + 1] = w.y;
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const f32x2 d2 = both(dc[c]), u2 = both(uc[c]);
+#pragma unroll
+          for (int k = 0; k < KN / 2; ++k) h.r[c][k] = fma2(ex2_2(mul2(d2, A2.r[c][k])), h.r[c][k], mul2(u2, bn[k]));
+        }
+        if (!kFull) clear_pair_padding(h, n0, p.N);
+        if (!CARRY) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            f32x2 v = mul2(cn[0], h.r[c][0]);
+#pragma unroll
+            for (int k = 1; k < KN / 2; ++k) v = fma2(cn[k], h.r[c][k], v);
+            (c ? yt : yo)[j] = lo2(v) + hi2(v);
           }
         }
       }
-      if (!CARRY) reduce_tokens<SG>(&sm.y[t], yv, g, s);
-    }
-    __syncwarp();
-    if (!CARRY) {
+      if (CARRY) continue;
+      // sums over the group's lanes: each ends with the tokens and the channel that it has prepared
+      float out[kMine][kOwn];
+      if (SG == 1) {
 #pragma unroll
-      for (int i = 0; i < kTile; i += RPI) {
-        const int r = i + row0;
-        if (r >= nt || pc >= p.dim) continue;
-        f32x2 out = fma2(skip, load_pair(&sm.x[st][r][2 * cp]), *reinterpret_cast<const f32x2*>(&sm.y[r][2 * cp]));
-        if (z) {
-          const f32x2 zz = load_pair(&sm.z[st][r][2 * cp]);
-          out = mul2(out, mul2(zz, sigmoid2(zz)));
+        for (int j = 0; j < 4; ++j) {
+          out[kMine - 1][j % kOwn] = yt[j];
+          out[0][j % kOwn] = yo[j];
         }
-        store_pair<T>(y + static_cast<long long>(t0 + r) * p.dim + 2 * cp, out, p.al_y, p.dim - pc);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) yo[j] += __shfl_xor_sync(0xffffffffu, yt[j], 1);
+        if (SG == 2) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) out[0][j % kOwn] = yo[j];
+        } else {
+          const bool up = s & (SG == 4 ? 2 : 4);
+          float a[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) a[j] = (up ? yo[2 + j] : yo[j]) + __shfl_xor_sync(0xffffffffu, up ? yo[j] : yo[2 + j], SG == 4 ? 2 : 4);
+          if (SG == 4) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) out[0][j % kOwn] = a[j];
+          } else {
+            const bool hi = s & 2;
+            float r = (hi ? a[1] : a[0]) + __shfl_xor_sync(0xffffffffu, hi ? a[0] : a[1], 2);
+            if (SG == 16) r += __shfl_xor_sync(0xffffffffu, r, 8);
+            out[0][0] = r;
+          }
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < kMine; ++m) {
+        const int col = m ? l1 : l0;
+#pragma unroll
+        for (int k = 0; k < kOwn; ++k) {
+          const int r = t + mine + k;
+          float v = fmaf(skip[m], xx[m][k], out[m][k]);
+          if (gate_on) {
+            const float zz = to_f(sm.z[st][r][col]);
+            v *= zz * sigmoid(zz);
+          }
+          if (r < nt && cw + col < p.dim && (SG < 16 || s < 8)) y[static_cast<long long>(t0 + r) * p.dim + col] = from_f<T>(v);
+        }
       }
     }
     __syncwarp();
   }
+  };
+  if (full && p.softplus) {
+    if (!CARRY && z)
+      walk(std::true_type{}, std::true_type{});
+    else
+      walk(std::true_type{}, std::false_type{});
+  } else {
+    walk(std::false_type{}, std::false_type{});
+  }
   copy_wait<0>();
   if (CARRY) {
-    store_lane(p.carry + (q * per_chunk + b * p.dim) * p.N, h, c0, p.dim, n0, p.N);
-    if (s == 0) {
-      float t[4];
-      unpack2(t[0], t[1], sum0);
-      unpack2(t[2], t[3], sum1);
+    store_pair_state(p.carry + (q * per_chunk + b * p.dim) * p.N, h, c0, c1, p.dim, n0, p.N);
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (c0 + k < p.dim) totals[q * per_chunk + b * p.dim + c0 + k] = t[k];
+    for (int m = 0; m < kMine; ++m) {
+      float v = total[m];  // this lane's tokens; the others of the channel lie in the other lanes of the same parity
+      if (SG >= 4) v += __shfl_xor_sync(0xffffffffu, v, 2);
+      if (SG >= 8) v += __shfl_xor_sync(0xffffffffu, v, 4);
+      const int ch = m ? c1 : c0;
+      if (s < 2 && ch < p.dim) totals[q * per_chunk + b * p.dim + ch] = v;
     }
     return;
   }
-  const float zero[2] = {};
-  if (pc < p.dim)
-    for (int t = max(first, live) + row0; t < end; t += RPI)
-      store_run<T, 2>(y + static_cast<long long>(t) * p.dim + 2 * cp, zero, p.al_y, p.dim - pc);
-  if (p.state && q == p.splits - 1) store_lane(p.state + b * p.dim * p.N, h, c0, p.dim, n0, p.N);
+  for (int t = max(first, live); t < end; ++t)
+    for (int c = lane; c < cols; c += 32) y[static_cast<long long>(t) * p.dim + c] = from_f<T>(0.f);
+  if (p.state && q == p.splits - 1) store_pair_state(p.state + b * p.dim * p.N, h, c0, c1, p.dim, n0, p.N);
 }
 
 // ---------------------------------------------------------------------------------------------------- one token

@@ -13,26 +13,29 @@ using namespace btp_scan;
 int state_groups(int N) { return N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
 
 struct Split {
+  int kn;      // states per lane of the forward
   int splits;
   int chunk;
 };
-// Chunks that the tokens are split into.  A warp takes the channels of one chunk; the device runs `slots` warps side by side at full
-// speed (two per scheduler).  Splitting costs a second pass over the tokens, so it has to more than halve the rounds.
 Split split_tokens(long long batch, int L, int dim, int N, int sms) {
-  const int wc = 128 / state_groups(N);
-  const long long units = batch * ((dim + wc - 1) / wc), slots = static_cast<long long>(sms) * 8;
-  Split best{1, (L + 31) / 32 * 32};
-  double best_cost = static_cast<double>((units + slots - 1) / slots) * best.chunk;
-  for (int s = 2; s <= 256; s = s * 3 / 2 + (s == 2)) {
-    const int chunk = ((L + s - 1) / s + 31) / 32 * 32;
-    if (chunk < 64) break;
-    const int n = (L + chunk - 1) / chunk;
-    if (n < 2) continue;
-    const double rounds = static_cast<double>((units * n + slots - 1) / slots);
-    const double cost = rounds * 2.0 * (chunk + 24) + n * 4.0;  // starting a kernel, combining the chunks before
-    if (cost < best_cost) {
-      best_cost = cost;
-      best = Split{n, chunk};
+  Split best{};
+  double best_cost = 0;
+  const char* ek = getenv("TUNE_KN"); const char* es = getenv("TUNE_S");
+  for (int kn = 8; kn >= 4; kn -= 4) {
+    if (ek && atoi(ek) != kn) continue;
+    const int wc = 64 * kn / (4 * state_groups(N));
+    const long long units = batch * ((dim + wc - 1) / wc), slots = static_cast<long long>(sms) * 4;
+    for (int s = 1; s <= 256; s = s < 4 ? s + 1 : s * 5 / 4) {
+      const int chunk = es ? ((L + atoi(es) - 1) / atoi(es) + 31) / 32 * 32 : ((L + s - 1) / s + 31) / 32 * 32;
+      if (s > 1 && chunk < 64) break;
+      const int n = (L + chunk - 1) / chunk;
+      const double per = (kn == 8 ? 130.0 : 75.0), lat = kn == 8 ? 300.0 : 200.0;
+      const double w = static_cast<double>((units * n + slots - 1) / slots);
+      const double cost = (w * per > lat ? w * per : lat) * (chunk + 24) * (n > 1 ? 1.8 : 1.0);
+      if (best.kn == 0 || cost < best_cost) {
+        best_cost = cost;
+        best = Split{kn, n, chunk};
+      }
     }
   }
   return best;
@@ -44,7 +47,7 @@ Split split_backward(long long batch, int L, int dim, int N, int sms) {
   const int sg = state_groups(N), wc = 128 / sg, cw = (sg == 2 ? 2 : 4) * wc;
   const long long ctas = batch * ((dim + cw - 1) / cw), warps = batch * ((dim + wc - 1) / wc);
   const long long slots = static_cast<long long>(sms) * 2, wslots = static_cast<long long>(sms) * 8;
-  Split best{1, (L + 31) / 32 * 32};
+  Split best{4, 1, (L + 31) / 32 * 32};
   double best_cost = static_cast<double>((ctas + slots - 1) / slots) * 2.6 * best.chunk;
   for (int s = 2; s <= 256; s = s * 3 / 2 + (s == 2)) {
     const int chunk = ((L + s - 1) / s + 31) / 32 * 32;
@@ -56,7 +59,7 @@ Split split_backward(long long batch, int L, int dim, int N, int sms) {
     const double cost = main + carry + n * 4.0;
     if (cost < best_cost) {
       best_cost = cost;
-      best = Split{n, chunk};
+      best = Split{4, n, chunk};
     }
   }
   return best;
@@ -150,26 +153,25 @@ int btp_sm100_scan_forward(const void* x, const void* delta, const float* A, con
   p.al_B = copies16(Bm, B_b, B_t, e, N);
   p.al_C = copies16(Cm, C_b, C_t, e, N);
   p.al_y = dim % 2 == 0 && aligned16(y);
-  const int wc = 128 / state_groups(N);
+  const int wc = 64 * s.kn / (4 * state_groups(N));
   const long long per_split = static_cast<long long>(B) * ((dim + wc - 1) / wc);
   if (per_split * s.splits > 0x7fffffffll) return fail(BTP_ERR_BAD_SHAPE, "%s: too many elements for one launch", fn);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const auto run = [&](auto tag, auto groups, auto carry_pass) {
+    using T = decltype(tag);
+    constexpr int SG = decltype(groups)::value;  // lanes per channel pair at 4 states each
+    constexpr bool kCarry = decltype(carry_pass)::value;
+    static_assert(sizeof(FwdTile<T, 8, SG / 2>) <= 48 * 1024 && sizeof(FwdTile<T, 4, SG>) <= 48 * 1024, "fits without a larger limit");
+    const int grid = static_cast<int>(per_split * (kCarry ? s.splits - 1 : s.splits));
+    if (s.kn == 8)
+      return launch_kernel(scan_forward_kernel<T, 8, SG / 2, kCarry>, grid, 32, static_cast<int>(sizeof(FwdTile<T, 8, SG / 2>)), st, p);
+    return launch_kernel(scan_forward_kernel<T, 4, SG, kCarry>, grid, 32, static_cast<int>(sizeof(FwdTile<T, 4, SG>)), st, p);
+  };
   if (s.splits > 1) {
-    rc = launched(fn, dispatch(dtype, N, [&](auto tag, auto groups) {
-      using T = decltype(tag);
-      constexpr int SG = decltype(groups)::value;
-      return launch_kernel(scan_forward_kernel<T, SG, true>, static_cast<int>(per_split * (s.splits - 1)), 32,
-                           static_cast<int>(sizeof(Tile<T, SG>)), st, p);
-    }));
+    rc = launched(fn, dispatch(dtype, N, [&](auto tag, auto groups) { return run(tag, groups, std::true_type{}); }));
     if (rc) return rc;
   }
-  return launched(fn, dispatch(dtype, N, [&](auto tag, auto groups) {
-    using T = decltype(tag);
-    constexpr int SG = decltype(groups)::value;
-    static_assert(sizeof(Tile<T, SG>) <= 48 * 1024, "a warp's tile must fit without a larger limit");
-    return launch_kernel(scan_forward_kernel<T, SG, false>, static_cast<int>(per_split * s.splits), 32,
-                         static_cast<int>(sizeof(Tile<T, SG>)), st, p);
-  }));
+  return launched(fn, dispatch(dtype, N, [&](auto tag, auto groups) { return run(tag, groups, std::false_type{}); }));
 }
 
 long long btp_sm100_scan_backward_floats(int B, int L, int dim, int N) {
