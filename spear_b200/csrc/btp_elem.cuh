@@ -154,6 +154,11 @@ __device__ __forceinline__ f32x2 load_pair(const __half* p) {
   const float2 f = __half22float2(*reinterpret_cast<const __half2*>(p));
   return pack2(f.x, f.y);
 }
+__device__ __forceinline__ f32x2 word_pair(unsigned w, __nv_bfloat16) { return pack2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+__device__ __forceinline__ f32x2 word_pair(unsigned w, __half) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return pack2(f.x, f.y);
+}
 template <class T>
 __device__ __forceinline__ void store_pair(T* p, f32x2 v, bool aligned, int count) {
   float f[2];

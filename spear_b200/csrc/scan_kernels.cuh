@@ -4,12 +4,13 @@
 //   h_t[d,n]   = exp(Delta_t[d] A[d,n]) h_{t-1}[d,n] + u_t[d] B_t[n]
 //   y_t[d]     = sum_n C_t[n] h_t[d,n] + D[d] x_t[d],  times z_t sigmoid(z_t) where there is a gate
 //
-// Layout.  A warp walks down the tokens of 128 / SG channels: lane = (channel group g, state group s), SG state groups;
-// a lane holds 4 channels x 4 states of h as pairs of neighbouring channels, so that products and sums are two-wide
-// (f32x2) with the step sizes as they lie in memory and with B and C given twice.  y is summed over a lane's 4 states in
-// registers and over the SG lanes by exchanging halves: 3 exchanges for 4 channels and 4 lanes.
-// Tiles of 16 tokens arrive by asynchronous copies one tile ahead; a first pass over the tile turns the raw values into
-// step sizes, inputs u and doubled B, C in float; a last pass adds D x, applies the gate and stores.
+// Layout.  A warp walks down the tokens of 64 / SG channels; a lane holds 2 neighbouring channels x 4 states of h, SG = N / 4 lanes
+// share the channels.  Pairs of states go through two-wide (f32x2) arithmetic.  Raw rows arrive by asynchronous copies one tile
+// of 16 tokens ahead; every lane turns its share of a group of 4 tokens into step sizes and inputs and hands them to the other
+// lanes of its channels by warp exchanges, which also bring the partial sums of y back to it for D x, gate and store.  Nothing but
+// the raw rows goes through shared memory.
+// Measured against lanes of 4 channels x 4 states with step sizes and y staged in shared memory (8 x 2048 tokens x 2048
+// channels x 16 states): 298 us against 520; 2 channels x 8 states 372 (half the warps), 2 x 2 states 343 (more exchanges).
 //
 // Bound: one exponential per (token, channel, state) on the special-function unit, 16 per clock and SM.
 //
@@ -220,78 +221,75 @@ __device__ __forceinline__ f32x2 channel_pair(const float* v, int c, int dim) {
 }
 
 // ---------------------------------------------------------------------------------------------------- forward
-// A lane holds 2 neighbouring channels x KN states as pairs of states; SG lanes share the channel pair.  The lane with the odd
+// A lane holds 2 neighbouring channels x 4 states as pairs of states; SG lanes share the channel pair.  The lane with the odd
 // index in its group takes the odd channel as its first: "own" and "other" below, so that nothing is selected by parity.
 // Of a group of 4 tokens each lane prepares kOwn tokens of its own channel (step size, input, in the end gate and output), straight
 // from the copied rows; the group's lanes pass step sizes and inputs to one another, and sums of y back, by exchanges in the warp.
-template <class T, int KN, int SG>
+template <class T, int SG>
 struct FwdTile {
-  static constexpr int kStates = KN * SG;
+  static constexpr int kStates = 4 * SG;
   static constexpr int kChannels = 64 / SG;
   T x[2][kTile][kChannels];
   T d[2][kTile][kChannels];
   T z[2][kTile][kChannels];
   T B[2][kTile][kStates];
   T C[2][kTile][kStates];
-  float Bf[kTile][kStates];
-  float Cf[kTile][kStates];
 };
 
-// KN consecutive states of the channels c0, c1 as pairs; a channel or state that is not there is 0.
-template <int KN>
+// Four consecutive elements, aligned to all of them, as pairs of floats.
+__device__ __forceinline__ void load_quad(f32x2 (&out)[2], const float* p) {
+  const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(p);
+  out[0] = w.x, out[1] = w.y;
+}
+template <class T>
+__device__ __forceinline__ void load_quad(f32x2 (&out)[2], const T* p) {
+  const uint2 w = *reinterpret_cast<const uint2*>(p);
+  out[0] = word_pair(w.x, T{}), out[1] = word_pair(w.y, T{});
+}
+
+// Four consecutive states of the channels c0, c1 as pairs of states; a channel or state that is not there is 0.
 struct PairState {
-  f32x2 r[2][KN / 2];
+  f32x2 r[2][2];
 };
-template <int KN>
-__device__ __forceinline__ void load_pair_state(PairState<KN>& h, const float* base, int c0, int c1, int dim, int n0, int N) {
+__device__ __forceinline__ void load_pair_state(PairState& h, const float* base, int c0, int c1, int dim, int n0, int N) {
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     const int ch = c ? c1 : c0;
-#pragma unroll
-    for (int q = 0; q < KN / 4; ++q) {
-      float v[4] = {};
-      if (ch < dim) load_states(v, base + static_cast<long long>(ch) * N, n0 + 4 * q, N);
-      h.r[c][2 * q] = pack2(v[0], v[1]);
-      h.r[c][2 * q + 1] = pack2(v[2], v[3]);
-    }
+    float v[4] = {};
+    if (ch < dim) load_states(v, base + static_cast<long long>(ch) * N, n0, N);
+    h.r[c][0] = pack2(v[0], v[1]);
+    h.r[c][1] = pack2(v[2], v[3]);
   }
 }
-template <int KN>
-__device__ __forceinline__ void store_pair_state(float* base, const PairState<KN>& h, int c0, int c1, int dim, int n0, int N) {
+__device__ __forceinline__ void store_pair_state(float* base, const PairState& h, int c0, int c1, int dim, int n0, int N) {
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     const int ch = c ? c1 : c0;
-#pragma unroll
-    for (int q = 0; q < KN / 4; ++q) {
-      float v[4];
-      unpack2(v[0], v[1], h.r[c][2 * q]);
-      unpack2(v[2], v[3], h.r[c][2 * q + 1]);
-      if (ch < dim) store_states(base + static_cast<long long>(ch) * N, v, n0 + 4 * q, N);
-    }
+    float v[4];
+    unpack2(v[0], v[1], h.r[c][0]);
+    unpack2(v[2], v[3], h.r[c][1]);
+    if (ch < dim) store_states(base + static_cast<long long>(ch) * N, v, n0, N);
   }
 }
-template <int KN>
-__device__ __forceinline__ void clear_pair_padding(PairState<KN>& h, int n0, int N) {
+// Lanes that stand for states from N on keep 0 there, whatever the inputs hold.
+__device__ __forceinline__ void clear_pair_padding(PairState& h, int n0, int N) {
 #pragma unroll
-  for (int k = 0; k < KN / 2; ++k) {
-    const int n = n0 + 2 * k;
+  for (int k = 0; k < 2; ++k)
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      if (n >= N)
+      if (n0 + 2 * k >= N)
         h.r[c][k] = 0ull;
-      else if (n + 1 >= N)
+      else if (n0 + 2 * k + 1 >= N)
         h.r[c][k] = pack2(lo2(h.r[c][k]), 0.f);
     }
-  }
 }
 
 // One warp per (channels, chunk, sequence).  CARRY: only the chunk's last state and sum of step sizes, from state zero.
-template <class T, int KN, int SG, bool CARRY>
+template <class T, int SG, bool CARRY>
 __global__ void __launch_bounds__(32) scan_forward_kernel(const ScanParams p) {
-  using S = FwdTile<T, KN, SG>;
+  using S = FwdTile<T, SG>;
   constexpr int WC = S::kChannels, NP = S::kStates;
-  constexpr int kOwn = SG >= 8 ? 1 : (SG == 1 ? 4 : 8 / SG);  // tokens of a group of 4 that a lane prepares
-  constexpr int kMine = SG == 1 ? 2 : 1;                      // channels that it prepares them for
+  constexpr int kOwn = SG >= 8 ? 1 : 8 / SG;  // tokens of a group of 4 that a lane prepares
   extern __shared__ __align__(16) unsigned char smem_raw[];
   S& sm = *reinterpret_cast<S*>(smem_raw);
   grid_dependency_wait();
@@ -304,18 +302,18 @@ __global__ void __launch_bounds__(32) scan_forward_kernel(const ScanParams p) {
   const long long b = rest / splits;
   const int cw = cb * WC, odd = s & 1;
   const int l0 = 2 * g + odd, l1 = 2 * g + 1 - odd;  // own and other channel within the warp's
-  const int c0 = cw + l0, c1 = cw + l1, n0 = KN * s;
+  const int c0 = cw + l0, c1 = cw + l1, n0 = 4 * s;
   const int n_tok = tokens_of(p.lengths, b, p.L);
   const int first = q * p.chunk, end = min(p.L, first + p.chunk), live = min(end, n_tok);
   const int cols = min(WC, p.dim - cw);
   const bool full = p.N == NP;
 
-  PairState<KN> A2, h;
+  PairState A2, h;
   load_pair_state(A2, p.A, c0, c1, p.dim, n0, p.N);
 #pragma unroll
   for (int c = 0; c < 2; ++c)
 #pragma unroll
-    for (int k = 0; k < KN / 2; ++k) {  // rates to the base 2, held above -inf so that a step of size 0 keeps the state
+    for (int k = 0; k < 2; ++k) {  // rates to the base 2, held above -inf so that a step of size 0 keeps the state
       float a, e;
       unpack2(a, e, mul2(A2.r[c][k], both(kLog2e)));
       A2.r[c][k] = pack2(a < -3e38f ? -3e38f : a, e < -3e38f ? -3e38f : e);
@@ -326,7 +324,7 @@ __global__ void __launch_bounds__(32) scan_forward_kernel(const ScanParams p) {
   float* totals = p.carry + (p.splits - 1) * per_chunk * p.N;
   if (!CARRY) {
     for (int k = 0; k < q; ++k) {  // the chunks before, in order: h = exp(A total) h + last
-      PairState<KN> last;
+      PairState last;
       load_pair_state(last, p.carry + (k * per_chunk + b * p.dim) * p.N, c0, c1, p.dim, n0, p.N);
       const float* row = totals + k * per_chunk + b * p.dim;
 #pragma unroll
@@ -334,20 +332,18 @@ __global__ void __launch_bounds__(32) scan_forward_kernel(const ScanParams p) {
         const int ch = c ? c1 : c0;
         const f32x2 total = both(ch < p.dim ? row[ch] : 0.f);
 #pragma unroll
-        for (int i = 0; i < KN / 2; ++i) h.r[c][i] = fma2(ex2_2(mul2(A2.r[c][i], total)), h.r[c][i], last.r[c][i]);
+        for (int i = 0; i < 2; ++i) h.r[c][i] = fma2(ex2_2(mul2(A2.r[c][i], total)), h.r[c][i], last.r[c][i]);
       }
     }
   }
-  float bias[kMine], skip[kMine];
-#pragma unroll
-  for (int m = 0; m < kMine; ++m) {
-    const int ch = m ? c1 : c0;
-    bias[m] = p.bias && ch < p.dim ? p.bias[ch] : 0.f;
-    skip[m] = p.D && ch < p.dim ? p.D[ch] : 0.f;
-  }
+  const float bias = p.bias && c0 < p.dim ? p.bias[c0] : 0.f, skip = p.D && c0 < p.dim ? p.D[c0] : 0.f;
   for (int i = lane; i < 2 * kTile * (WC - cols); i += 32) {  // channels that are not there: never copied, read as zeros
     const int at = i / (WC - cols) * WC + cols + i % (WC - cols);
     (&sm.x[0][0][0])[at] = (&sm.d[0][0][0])[at] = (&sm.z[0][0][0])[at] = from_f<T>(0.f);
+  }
+  for (int i = lane; i < 2 * kTile * (NP - p.N); i += 32) {  // nor states
+    const int at = i / (NP - p.N) * NP + p.N + i % (NP - p.N);
+    (&sm.B[0][0][0])[at] = (&sm.C[0][0][0])[at] = from_f<T>(0.f);
   }
   const T* x = static_cast<const T*>(p.x) + b * p.x_b + cw;
   const T* dl = static_cast<const T*>(p.delta) + b * p.d_b + cw;
@@ -365,158 +361,131 @@ __global__ void __launch_bounds__(32) scan_forward_kernel(const ScanParams p) {
       if (z) fetch<T, kTile, WC, 32>(sm.z[st], z + t0 * p.z_t, p.z_t, rows, cols, p.al_z, lane);
     }
   };
-  float total[kMine] = {};
-  const int mine = SG == 1 ? 0 : (s >> 1) * kOwn & 3;       // first token of each group that this lane prepares
+  float total = 0.f;
+  const int mine = (s >> 1) * kOwn & 3;                          // first token of each group that this lane prepares
   const int own_src = g * SG + odd, oth_src = g * SG + 1 - odd;  // lanes that prepare token 0 of the own and the other channel
-  // The walk over the chunk, once for the usual case (all states there, softplus, gate or not known) and once with everything tested:
-  // a branch per token would keep the tokens of a group from overlapping.
+  // The walk over the chunk, once for the usual cases (all states there, softplus, a gate or none) and once with everything tested: a
+  // branch per token would keep the tokens of a group from overlapping.
   const auto walk = [&](auto usual, auto gated) {
-  constexpr bool kFull = decltype(usual)::value;
-  const bool softplus_on = kFull || p.softplus, gate_on = kFull ? decltype(gated)::value : z != nullptr;
-  if (first < live) load_tile(0, first);
-  copy_commit();
-  int st = 0;
-  for (int t0 = first; t0 < live; t0 += kTile, st ^= 1) {
-    if (t0 + kTile < live) load_tile(st ^ 1, t0 + kTile);
+    constexpr bool kFull = decltype(usual)::value;
+    const bool softplus_on = kFull || p.softplus, gate_on = kFull ? decltype(gated)::value : z != nullptr;
+    if (first < live) load_tile(0, first);
     copy_commit();
-    copy_wait<1>();
-    __syncwarp();
-    const int nt = min(kTile, live - t0);
-    if (!CARRY && p.checkpoints && t0 % kCheckpoint == 0) {
-      const long long at = b * ((p.L + kCheckpoint - 1) / kCheckpoint) + t0 / kCheckpoint;
-      store_pair_state(p.checkpoints + at * p.dim * p.N, h, c0, c1, p.dim, n0, p.N);
-    }
-    // B and C to float; rows behind the last token and states that are not there become zeros
-#pragma unroll
-    for (int i0 = 0; i0 < kTile * NP / 2; i0 += 32) {
-      const int i = i0 + lane, r = i / (NP / 2), n = i % (NP / 2) * 2;
-      const bool ok0 = r < nt && n < p.N, ok1 = r < nt && n + 1 < p.N;
-      float v0, v1;
-      unpack2(v0, v1, load_pair(&sm.B[st][r][n]));
-      *reinterpret_cast<float2*>(&sm.Bf[r][n]) = make_float2(ok0 ? v0 : 0.f, ok1 ? v1 : 0.f);
-      if (!CARRY) {
-        unpack2(v0, v1, load_pair(&sm.C[st][r][n]));
-        *reinterpret_cast<float2*>(&sm.Cf[r][n]) = make_float2(ok0 ? v0 : 0.f, ok1 ? v1 : 0.f);
+    int st = 0;
+    for (int t0 = first; t0 < live; t0 += kTile, st ^= 1) {
+      if (t0 + kTile < live) load_tile(st ^ 1, t0 + kTile);
+      copy_commit();
+      copy_wait<1>();
+      __syncwarp();
+      const int nt = min(kTile, live - t0);
+      if (!CARRY && p.checkpoints && t0 % kCheckpoint == 0) {
+        const long long at = b * ((p.L + kCheckpoint - 1) / kCheckpoint) + t0 / kCheckpoint;
+        store_pair_state(p.checkpoints + at * p.dim * p.N, h, c0, c1, p.dim, n0, p.N);
       }
-    }
-    __syncwarp();
-    for (int t = 0; t < nt; t += 4) {
-      float de[kMine][kOwn], xx[kMine][kOwn], uu[kMine][kOwn];
-#pragma unroll
-      for (int m = 0; m < kMine; ++m) {
-        const int col = m ? l1 : l0;
+      if (nt < kTile) {  // rows behind the last token: zeros leave the state as it is
+        for (int i = lane; i < (kTile - nt) * NP; i += 32) (&sm.B[st][nt][0])[i] = (&sm.C[st][nt][0])[i] = from_f<T>(0.f);
+        __syncwarp();
+      }
+      float de[kOwn], xx[kOwn], uu[kOwn];  // step sizes, x and inputs of this lane's tokens of a group
+      const auto prepare = [&](int t) {
 #pragma unroll
         for (int k = 0; k < kOwn; ++k) {
-          de[m][k] = to_f(sm.d[st][t + mine + k][col]) + bias[m];
-          xx[m][k] = to_f(sm.x[st][t + mine + k][col]);
+          de[k] = to_f(sm.d[st][t + mine + k][l0]) + bias;
+          xx[k] = to_f(sm.x[st][t + mine + k][l0]);
         }
         if (softplus_on) {
-          if (kOwn == 1) {
-            de[m][0] = softplus(de[m][0]);
+          if constexpr (kOwn == 1) {
+            de[0] = softplus(de[0]);
           } else {
 #pragma unroll
-            for (int k = 0; k < kOwn; k += 2) unpack2(de[m][k], de[m][k + 1], softplus2(pack2(de[m][k], de[m][k + 1])));
+            for (int k = 0; k < kOwn; k += 2) unpack2(de[k], de[k + 1], softplus2(pack2(de[k], de[k + 1])));
           }
         }
 #pragma unroll
         for (int k = 0; k < kOwn; ++k) {
-          uu[m][k] = de[m][k] * xx[m][k];
-          if (nt < kTile && t + mine + k >= nt) de[m][k] = uu[m][k] = 0.f;  // they leave the state as it is
-          total[m] += de[m][k];
+          uu[k] = de[k] * xx[k];
+          if (t + mine + k >= nt) de[k] = uu[k] = 0.f;
+          total += de[k];
         }
-      }
-      float yo[4], yt[4];  // sums of the own and the other channel
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float dc[2], uc[2];
-        if (SG == 1) {
-          dc[0] = de[0][j], dc[1] = de[kMine - 1][j], uc[0] = uu[0][j], uc[1] = uu[kMine - 1][j];
-        } else if (SG == 2) {
-          dc[0] = de[0][j % kOwn], uc[0] = uu[0][j % kOwn];
-          dc[1] = __shfl_xor_sync(0xffffffffu, dc[0], 1);
-          uc[1] = __shfl_xor_sync(0xffffffffu, uc[0], 1);
-        } else {
-          const int up = 2 * (j / kOwn);
-          dc[0] = __shfl_sync(0xffffffffu, de[0][j % kOwn], own_src + up);
-          dc[1] = __shfl_sync(0xffffffffu, de[0][j % kOwn], oth_src + up);
-          uc[0] = __shfl_sync(0xffffffffu, uu[0][j % kOwn], own_src + up);
-          uc[1] = __shfl_sync(0xffffffffu, uu[0][j % kOwn], oth_src + up);
-        }
-        f32x2 bn[KN / 2], cn[KN / 2];
-#pragma unroll
-        for (int k = 0; k < KN / 4; ++k) {
-          const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&sm.Bf[t + j][n0 + 4 * k]);
-          bn[2 * k] = v.x, bn[2 * k + 1] = v.y;
-          if (!CARRY) {
-            const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(&sm.Cf[t + j][n0 + 4 * k]);
-            cn[2 * k] = w.x, cn[2 * k + 1] = w.y;
-          }
-        }
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const f32x2 d2 = both(dc[c]), u2 = both(uc[c]);
-#pragma unroll
-          for (int k = 0; k < KN / 2; ++k) h.r[c][k] = fma2(ex2_2(mul2(d2, A2.r[c][k])), h.r[c][k], mul2(u2, bn[k]));
-        }
-        if (!kFull) clear_pair_padding(h, n0, p.N);
-        if (!CARRY) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            f32x2 v = mul2(cn[0], h.r[c][0]);
-#pragma unroll
-            for (int k = 1; k < KN / 2; ++k) v = fma2(cn[k], h.r[c][k], v);
-            (c ? yt : yo)[j] = lo2(v) + hi2(v);
-          }
-        }
-      }
-      if (CARRY) continue;
-      // sums over the group's lanes: each ends with the tokens and the channel that it has prepared
-      float out[kMine][kOwn];
-      if (SG == 1) {
+      };
+      const auto group = [&](int t) {
+        prepare(t);
+        float yo[4], yt[4];  // sums of the own and the other channel
+        float dc[4][2], uc[4][2];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          out[kMine - 1][j % kOwn] = yt[j];
-          out[0][j % kOwn] = yo[j];
+          if (SG == 2) {
+            dc[j][0] = de[j % kOwn], uc[j][0] = uu[j % kOwn];
+            dc[j][1] = __shfl_xor_sync(0xffffffffu, dc[j][0], 1);
+            uc[j][1] = __shfl_xor_sync(0xffffffffu, uc[j][0], 1);
+          } else {
+            const int up = 2 * (j / kOwn);
+            dc[j][0] = __shfl_sync(0xffffffffu, de[j % kOwn], own_src + up);
+            dc[j][1] = __shfl_sync(0xffffffffu, de[j % kOwn], oth_src + up);
+            uc[j][0] = __shfl_sync(0xffffffffu, uu[j % kOwn], own_src + up);
+            uc[j][1] = __shfl_sync(0xffffffffu, uu[j % kOwn], oth_src + up);
+          }
         }
-      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          f32x2 bn[2], cn[2];
+          load_quad(bn, &sm.B[st][t + j][n0]);
+          if (!CARRY) load_quad(cn, &sm.C[st][t + j][n0]);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const f32x2 d2 = both(dc[j][c]), u2 = both(uc[j][c]);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) h.r[c][k] = fma2(ex2_2(mul2(d2, A2.r[c][k])), h.r[c][k], mul2(u2, bn[k]));
+          }
+          if (!kFull) clear_pair_padding(h, n0, p.N);
+          if (!CARRY) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const f32x2 v = fma2(cn[1], h.r[c][1], mul2(cn[0], h.r[c][0]));
+              (c ? yt : yo)[j] = lo2(v) + hi2(v);
+            }
+          }
+        }
+        if (CARRY) return;
+        // sums over the group's lanes: each ends with the tokens and the channel that it has prepared
+        float out[kOwn];
 #pragma unroll
         for (int j = 0; j < 4; ++j) yo[j] += __shfl_xor_sync(0xffffffffu, yt[j], 1);
-        if (SG == 2) {
+        if constexpr (SG == 2) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) out[0][j % kOwn] = yo[j];
+          for (int j = 0; j < 4; ++j) out[j] = yo[j];
         } else {
           const bool up = s & (SG == 4 ? 2 : 4);
           float a[2];
 #pragma unroll
           for (int j = 0; j < 2; ++j) a[j] = (up ? yo[2 + j] : yo[j]) + __shfl_xor_sync(0xffffffffu, up ? yo[j] : yo[2 + j], SG == 4 ? 2 : 4);
-          if (SG == 4) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) out[0][j % kOwn] = a[j];
+          if constexpr (SG == 4) {
+            out[0] = a[0], out[1] = a[1];
           } else {
             const bool hi = s & 2;
-            float r = (hi ? a[1] : a[0]) + __shfl_xor_sync(0xffffffffu, hi ? a[0] : a[1], 2);
-            if (SG == 16) r += __shfl_xor_sync(0xffffffffu, r, 8);
-            out[0][0] = r;
+            out[0] = (hi ? a[1] : a[0]) + __shfl_xor_sync(0xffffffffu, hi ? a[0] : a[1], 2);
+            if (SG == 16) out[0] += __shfl_xor_sync(0xffffffffu, out[0], 8);
           }
         }
-      }
-#pragma unroll
-      for (int m = 0; m < kMine; ++m) {
-        const int col = m ? l1 : l0;
 #pragma unroll
         for (int k = 0; k < kOwn; ++k) {
           const int r = t + mine + k;
-          float v = fmaf(skip[m], xx[m][k], out[m][k]);
+          float v = fmaf(skip, xx[k], out[k]);
           if (gate_on) {
-            const float zz = to_f(sm.z[st][r][col]);
+            const float zz = to_f(sm.z[st][r][l0]);
             v *= zz * sigmoid(zz);
           }
-          if (r < nt && cw + col < p.dim && (SG < 16 || s < 8)) y[static_cast<long long>(t0 + r) * p.dim + col] = from_f<T>(v);
+          if (r < nt && c0 < p.dim && (SG < 16 || s < 8)) y[static_cast<long long>(t0 + r) * p.dim + l0] = from_f<T>(v);
         }
+      };
+      if (nt == kTile) {  // in one piece: a group's first loads and last exchanges overlap with its neighbours' arithmetic
+#pragma unroll
+        for (int t = 0; t < kTile; t += 4) group(t);
+      } else {
+        for (int t = 0; t < nt; t += 4) group(t);
       }
+      __syncwarp();
     }
-    __syncwarp();
-  }
   };
   if (full && p.softplus) {
     if (!CARRY && z)
@@ -529,14 +498,10 @@ __global__ void __launch_bounds__(32) scan_forward_kernel(const ScanParams p) {
   copy_wait<0>();
   if (CARRY) {
     store_pair_state(p.carry + (q * per_chunk + b * p.dim) * p.N, h, c0, c1, p.dim, n0, p.N);
-#pragma unroll
-    for (int m = 0; m < kMine; ++m) {
-      float v = total[m];  // this lane's tokens; the others of the channel lie in the other lanes of the same parity
-      if (SG >= 4) v += __shfl_xor_sync(0xffffffffu, v, 2);
-      if (SG >= 8) v += __shfl_xor_sync(0xffffffffu, v, 4);
-      const int ch = m ? c1 : c0;
-      if (s < 2 && ch < p.dim) totals[q * per_chunk + b * p.dim + ch] = v;
-    }
+    // this lane's tokens; the others of the channel lie in the other lanes of the same parity
+    if (SG >= 4) total += __shfl_xor_sync(0xffffffffu, total, 2);
+    if (SG >= 8) total += __shfl_xor_sync(0xffffffffu, total, 4);
+    if (s < 2 && c0 < p.dim) totals[q * per_chunk + b * p.dim + c0] = total;
     return;
   }
   for (int t = max(first, live); t < end; ++t)

@@ -13,29 +13,27 @@ using namespace btp_scan;
 int state_groups(int N) { return N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
 
 struct Split {
-  int kn;      // states per lane of the forward
   int splits;
   int chunk;
 };
+// Chunks that the tokens are split into, by a model of the time in cycles.  With w warps on the fullest scheduler a token takes
+// 60 + 112 w cycles (measured 285 at w = 2, 1570 at w = 14), in the pass for the carries 60 + 75 w; every chunk before its own costs a
+// warp about 300 cycles.  So a split pays where one pass leaves schedulers with one or two warps over a long stretch.
 Split split_tokens(long long batch, int L, int dim, int N, int sms) {
+  const int wc = 64 / state_groups(N);
+  const long long units = batch * ((dim + wc - 1) / wc), schedulers = static_cast<long long>(sms) * 4;
+  const auto warps = [&](long long n) { return static_cast<double>((n + schedulers - 1) / schedulers); };
   Split best{};
   double best_cost = 0;
-  const char* ek = getenv("TUNE_KN"); const char* es = getenv("TUNE_S");
-  for (int kn = 8; kn >= 4; kn -= 4) {
-    if (ek && atoi(ek) != kn) continue;
-    const int wc = 64 * kn / (4 * state_groups(N));
-    const long long units = batch * ((dim + wc - 1) / wc), slots = static_cast<long long>(sms) * 4;
-    for (int s = 1; s <= 256; s = s < 4 ? s + 1 : s * 5 / 4) {
-      const int chunk = es ? ((L + atoi(es) - 1) / atoi(es) + 31) / 32 * 32 : ((L + s - 1) / s + 31) / 32 * 32;
-      if (s > 1 && chunk < 64) break;
-      const int n = (L + chunk - 1) / chunk;
-      const double per = (kn == 8 ? 130.0 : 75.0), lat = kn == 8 ? 300.0 : 200.0;
-      const double w = static_cast<double>((units * n + slots - 1) / slots);
-      const double cost = (w * per > lat ? w * per : lat) * (chunk + 24) * (n > 1 ? 1.8 : 1.0);
-      if (best.kn == 0 || cost < best_cost) {
-        best_cost = cost;
-        best = Split{kn, n, chunk};
-      }
+  for (int s = 1; s <= 256; s = s < 4 ? s + 1 : s * 5 / 4) {
+    const int chunk = ((L + s - 1) / s + 31) / 32 * 32;
+    if (s > 1 && chunk < 64) break;
+    const int n = (L + chunk - 1) / chunk;
+    double cost = (60 + 112 * warps(units * n)) * (chunk + 16);
+    if (n > 1) cost += (60 + 75 * warps(units * (n - 1))) * (chunk + 16) + 300.0 * n + 8000;
+    if (s == 1 || cost < best_cost) {
+      best_cost = cost;
+      best = Split{n, chunk};
     }
   }
   return best;
@@ -47,7 +45,7 @@ Split split_backward(long long batch, int L, int dim, int N, int sms) {
   const int sg = state_groups(N), wc = 128 / sg, cw = (sg == 2 ? 2 : 4) * wc;
   const long long ctas = batch * ((dim + cw - 1) / cw), warps = batch * ((dim + wc - 1) / wc);
   const long long slots = static_cast<long long>(sms) * 2, wslots = static_cast<long long>(sms) * 8;
-  Split best{4, 1, (L + 31) / 32 * 32};
+  Split best{1, (L + 31) / 32 * 32};
   double best_cost = static_cast<double>((ctas + slots - 1) / slots) * 2.6 * best.chunk;
   for (int s = 2; s <= 256; s = s * 3 / 2 + (s == 2)) {
     const int chunk = ((L + s - 1) / s + 31) / 32 * 32;
@@ -59,7 +57,7 @@ Split split_backward(long long batch, int L, int dim, int N, int sms) {
     const double cost = main + carry + n * 4.0;
     if (cost < best_cost) {
       best_cost = cost;
-      best = Split{4, n, chunk};
+      best = Split{n, chunk};
     }
   }
   return best;
@@ -153,19 +151,17 @@ int btp_sm100_scan_forward(const void* x, const void* delta, const float* A, con
   p.al_B = copies16(Bm, B_b, B_t, e, N);
   p.al_C = copies16(Cm, C_b, C_t, e, N);
   p.al_y = dim % 2 == 0 && aligned16(y);
-  const int wc = 64 * s.kn / (4 * state_groups(N));
+  const int wc = 64 / state_groups(N);
   const long long per_split = static_cast<long long>(B) * ((dim + wc - 1) / wc);
   if (per_split * s.splits > 0x7fffffffll) return fail(BTP_ERR_BAD_SHAPE, "%s: too many elements for one launch", fn);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const auto run = [&](auto tag, auto groups, auto carry_pass) {
     using T = decltype(tag);
-    constexpr int SG = decltype(groups)::value;  // lanes per channel pair at 4 states each
+    constexpr int SG = decltype(groups)::value;
     constexpr bool kCarry = decltype(carry_pass)::value;
-    static_assert(sizeof(FwdTile<T, 8, SG / 2>) <= 48 * 1024 && sizeof(FwdTile<T, 4, SG>) <= 48 * 1024, "fits without a larger limit");
-    const int grid = static_cast<int>(per_split * (kCarry ? s.splits - 1 : s.splits));
-    if (s.kn == 8)
-      return launch_kernel(scan_forward_kernel<T, 8, SG / 2, kCarry>, grid, 32, static_cast<int>(sizeof(FwdTile<T, 8, SG / 2>)), st, p);
-    return launch_kernel(scan_forward_kernel<T, 4, SG, kCarry>, grid, 32, static_cast<int>(sizeof(FwdTile<T, 4, SG>)), st, p);
+    static_assert(sizeof(FwdTile<T, SG>) <= 48 * 1024, "fits without a larger limit");
+    return launch_kernel(scan_forward_kernel<T, SG, kCarry>, static_cast<int>(per_split * (kCarry ? s.splits - 1 : s.splits)), 32,
+                         static_cast<int>(sizeof(FwdTile<T, SG>)), st, p);
   };
   if (s.splits > 1) {
     rc = launched(fn, dispatch(dtype, N, [&](auto tag, auto groups) { return run(tag, groups, std::true_type{}); }));
