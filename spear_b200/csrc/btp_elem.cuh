@@ -159,11 +159,89 @@ __device__ __forceinline__ f32x2 word_pair(unsigned w, __half) {
   const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
   return pack2(f.x, f.y);
 }
+// Four consecutive elements, aligned to all of them, as pairs of floats.
+__device__ __forceinline__ void load_quad(f32x2 (&out)[2], const float* p) {
+  const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(p);
+  out[0] = w.x, out[1] = w.y;
+}
+template <class T>
+__device__ __forceinline__ void load_quad(f32x2 (&out)[2], const T* p) {
+  const uint2 w = *reinterpret_cast<const uint2*>(p);
+  out[0] = word_pair(w.x, T{}), out[1] = word_pair(w.y, T{});
+}
+
+// 2 PAIRS consecutive elements as pairs; `aligned`: one word of all of them may be read, else element by element, `count` of them.
+template <int PAIRS, class T>
+__device__ __forceinline__ void load_channels(f32x2 (&out)[PAIRS], const T* p, bool aligned, int count) {
+  if (aligned) {
+    if constexpr (PAIRS == 2)
+      load_quad(out, p);
+    else
+      out[0] = load_pair(p);
+  } else {
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) out[i] = pack2(2 * i < count ? to_f(p[2 * i]) : 0.f, 2 * i + 1 < count ? to_f(p[2 * i + 1]) : 0.f);
+  }
+}
+template <int PAIRS, class T>
+__device__ __forceinline__ void store_channels(T* p, const f32x2 (&in)[PAIRS], bool aligned, int count) {
+  float f[2 * PAIRS];
+#pragma unroll
+  for (int i = 0; i < PAIRS; ++i) unpack2(f[2 * i], f[2 * i + 1], in[i]);
+  store_run<T, 2 * PAIRS>(p, f, aligned, count);
+}
 template <class T>
 __device__ __forceinline__ void store_pair(T* p, f32x2 v, bool aligned, int count) {
   float f[2];
   unpack2(f[0], f[1], v);
   store_run<T, 2>(p, f, aligned, count);
+}
+
+// Asynchronous copies into shared memory.
+__device__ __forceinline__ void copy16(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy8(void* to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy4(void* to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// ROWS rows of COLS elements (row pitch `pitch`, `cols` of them there) into dst[ROWS][COLS], by the threads of a group of
+// GROUP threads.  Rows from `rows` on and columns from `cols` on are not touched.
+template <class T, int ROWS, int COLS, int GROUP>
+__device__ __forceinline__ void fetch(T (*dst)[COLS], const T* src, long long pitch, int rows, int cols, bool aligned, int tid) {
+  constexpr int kBytes = COLS * static_cast<int>(sizeof(T)) < 16 ? 8 : 16, E = kBytes / static_cast<int>(sizeof(T)), CPR = COLS / E;
+  static_assert(COLS % E == 0 && CPR >= 1, "a row is whole copies");
+  if (aligned) {
+#pragma unroll
+    for (int i0 = 0; i0 < ROWS * CPR; i0 += GROUP) {
+      const int i = i0 + tid, r = i / CPR, c = (i - r * CPR) * E;
+      if ((ROWS * CPR % GROUP == 0 || i < ROWS * CPR) && r < rows && c < cols) {
+        if (kBytes == 16)
+          copy16(&dst[r][c], src + r * pitch + c);
+        else
+          copy8(&dst[r][c], src + r * pitch + c);
+      }
+    }
+  } else {
+#pragma unroll 4
+    for (int i0 = 0; i0 < ROWS * COLS; i0 += GROUP) {
+      const int i = i0 + tid, r = i / COLS, c = i - r * COLS;
+      if (i < ROWS * COLS && r < rows && c < cols) {
+        if (sizeof(T) == 4)
+          copy4(&dst[r][c], src + r * pitch + c);
+        else
+          dst[r][c] = src[r * pitch + c];
+      }
+    }
+  }
 }
 
 // Tokens of sequence b that are there: `lengths` may be null (all L), its values are held to 0 ... L.

@@ -2,26 +2,26 @@
 #include "conv_kernels.cuh"
 #include "elem_host.cuh"
 
+#include <initializer_list>
+
 namespace {
 
 using namespace btp_host;
 using namespace btp_conv;
 
-// Tokens per thread: as long as the device still gets about two threads per slot (148 SMs x 2048), since every run reads W-1
-// tokens of the one before it again; 4 to 64.
-int forward_run(long long B, int L, int dim, int vec, int sms) {
-  const long long want = B * L * (dim / vec) / (static_cast<long long>(sms) * 2048 * 2);
-  int run = 4;
-  while (run < 64 && run < want) run *= 2;
-  return run;
+constexpr int kStepChannels = 4;  // per thread of the step
+
+// Tokens per CTA: whole tiles, as many as leave the device about `per_sm` CTAs per SM (each reads W-1 tokens of its neighbour's run
+// again and fills its ring anew); at least 4 tiles.
+int tokens_per_run(long long B, int L, int dim, int sms, int per_sm) {
+  const long long cblocks = (dim + kCols - 1) / kCols, slots = static_cast<long long>(sms) * per_sm;
+  long long runs = slots / (B * cblocks);
+  if (runs < 1) runs = 1;
+  long long run = ((L + runs - 1) / runs + kTile - 1) / kTile * kTile;
+  if (run < 4 * kTile) run = 4 * kTile;
+  return static_cast<int>(run);
 }
-// Backward: a CTA takes 8 runs of 32 lanes' channels.
-int backward_run(long long B, int L, int dim, int vec, int sms) {
-  const long long want = B * L * (dim / vec) / (static_cast<long long>(sms) * 512 * 2);
-  int run = 8;
-  while (run < 64 && run < want) run *= 2;
-  return run;
-}
+constexpr int kForwardCtas = 20, kBackwardCtas = 8;  // per SM; measured best of 10 ... 40 and 6 ... 16
 
 int check(const char* fn, long long B, int L, int dim, int width, int dtype, int weight_dtype) {
   if (B <= 0 || L <= 0 || dim <= 0) return fail(BTP_ERR_BAD_SHAPE, "%s: B, L and dim must be positive (got %lld, %d, %d)", fn, B, L, dim);
@@ -34,10 +34,14 @@ int check(const char* fn, long long B, int L, int dim, int width, int dtype, int
   return BTP_OK;
 }
 
-template <class T>
-constexpr int vec_of() { return 16 / static_cast<int>(sizeof(T)); }
-
-// f(value of the type, vector width, taps)
+// Whether `n` channels are one word everywhere: rows `dim` and the given strides apart, from each of the pointers.
+bool one_word(int n, int e, int dim, long long sb, long long st, std::initializer_list<const void*> ptrs) {
+  if (dim % n || sb % n || st % n) return false;
+  for (const void* q : ptrs)
+    if (q && (reinterpret_cast<uintptr_t>(q) & static_cast<uintptr_t>(n * e - 1))) return false;
+  return true;
+}
+// f(value of the type, taps)
 template <class F>
 cudaError_t dispatch(int dtype, int width, F&& f) {
   return by_type(dtype, [&](auto tag) {
@@ -62,23 +66,22 @@ int btp_sm100_causal_conv_forward(const void* x, const void* weight, const void*
   int dev;
   DeviceInfo info;
   if ((rc = device_info(&dev, &info))) return rc;
-  const int e = elem_bytes(dtype), vec = 16 / e;
-  const bool al = dim % vec == 0 && (sx_b * e) % 16 == 0 && (sx_t * e) % 16 == 0 && aligned16(x) && aligned16(y) &&
-                  (!initial || aligned16(initial)) && (!state || aligned16(state));
   ConvParams p{};
+  const int e = elem_bytes(dtype);
+  p.aligned = one_word(2, e, dim, sx_b, sx_t, {x, y, initial, state});
+  p.copies = one_word(16 / e, e, dim, sx_b, sx_t, {x});
+  p.whole_w = aligned16(weight);
   p.x = x; p.weight = weight; p.bias = bias; p.initial = initial; p.lengths = lengths; p.y = y; p.state = state;
   p.sx_b = sx_b; p.sx_t = sx_t; p.B = B; p.L = L; p.dim = dim; p.silu = silu != 0; p.weight_f32 = weight_dtype == BTP_DTYPE_F32;
-  const int v = al ? vec : 1;
-  p.run = forward_run(B, L, dim, v, info.sms);
+  p.run = tokens_per_run(B, L, dim, info.sms, kForwardCtas);
   p.runs = (L + p.run - 1) / p.run;
-  const long long ctas = (static_cast<long long>(B) * p.runs * (dim / v) + 255) / 256;
+  const long long ctas = static_cast<long long>(B) * p.runs * ((dim + kCols - 1) / kCols);
   if (ctas > 0x7fffffffll) return fail(BTP_ERR_BAD_SHAPE, "%s: too many elements for one launch", fn);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return launched(fn, dispatch(dtype, width, [&](auto tag, auto taps) {
     using T = decltype(tag);
     constexpr int W = decltype(taps)::value;
-    if (al) return launch_kernel(conv_forward_kernel<T, vec_of<T>(), W>, static_cast<int>(ctas), 256, 0, st, p);
-    return launch_kernel(conv_forward_kernel<T, 1, W>, static_cast<int>(ctas), 256, 0, st, p);
+    return launch_kernel(conv_forward_kernel<T, W>, static_cast<int>(ctas), kThreads, static_cast<int>(sizeof(ConvTile<T, 1>)), st, p);
   }));
 }
 
@@ -89,15 +92,10 @@ int btp_sm100_causal_conv_partial_rows(int B, int L, int dim) {
   int dev;
   DeviceInfo info;
   if ((rc = device_info(&dev, &info))) return rc;
-  // the most that either vector width takes
-  long long most = 0;
-  for (int v : {1, 4}) {
-    const int run = backward_run(B, L, dim, v, info.sms);
-    const long long parts = static_cast<long long>(B) * ((L + run * kRunsPerCta - 1) / (run * kRunsPerCta));
-    if (parts > most) most = parts;
-  }
-  if (most > 0x7fffffffll) return fail(BTP_ERR_BAD_SHAPE, "%s: too many elements for one launch", fn);
-  return static_cast<int>(most);
+  const int run = tokens_per_run(B, L, dim, info.sms, kBackwardCtas);
+  const long long parts = static_cast<long long>(B) * ((L + run - 1) / run);
+  if (parts > 0x7fffffffll) return fail(BTP_ERR_BAD_SHAPE, "%s: too many elements for one launch", fn);
+  return static_cast<int>(parts);
 }
 
 int btp_sm100_causal_conv_backward(const void* x, const void* weight, const void* bias, const void* initial, const int* lengths,
@@ -113,26 +111,29 @@ int btp_sm100_causal_conv_backward(const void* x, const void* weight, const void
   int dev;
   DeviceInfo info;
   if ((rc = device_info(&dev, &info))) return rc;
-  // four channels per thread (8 bytes at 16 bits): filter, windows and sums of W = 4 taps are 20 registers a channel
-  const int e = elem_bytes(dtype);
-  const auto al4 = [&](const void* q) { return !q || (reinterpret_cast<uintptr_t>(q) & static_cast<uintptr_t>(4 * e - 1)) == 0; };
-  const bool al = dim % 4 == 0 && sx_b % 4 == 0 && sx_t % 4 == 0 && al4(x) && al4(dy) && al4(dx) && al4(initial) && al4(dstate) && al4(dinitial);
   ConvParams p{};
   p.x = x; p.weight = weight; p.bias = bias; p.initial = initial; p.lengths = lengths; p.dy = dy; p.dstate = dstate; p.dx = dx;
   p.dinitial = dinitial; p.partial = dweight || dbias ? partial : nullptr;
   p.sx_b = sx_b; p.sx_t = sx_t; p.B = B; p.L = L; p.dim = dim; p.silu = silu != 0; p.weight_f32 = weight_dtype == BTP_DTYPE_F32;
-  const int v = al ? 4 : 1;
-  p.run = backward_run(B, L, dim, v, info.sms);
+  const int e = elem_bytes(dtype);
+  p.aligned = one_word(2, e, dim, sx_b, sx_t, {x, dy, dx, initial, dstate, dinitial});
+  p.copies = one_word(16 / e, e, dim, sx_b, sx_t, {x});
+  p.copies_dy = one_word(16 / e, e, dim, 0, 0, {dy});
+  p.whole_w = aligned16(weight);
+  p.run = tokens_per_run(B, L, dim, info.sms, kBackwardCtas);
   p.runs = (L + p.run - 1) / p.run;
-  const long long parts = static_cast<long long>(B) * ((p.runs + kRunsPerCta - 1) / kRunsPerCta);
-  const long long ctas = parts * ((dim + 32 * v - 1) / (32 * v));
+  const long long parts = static_cast<long long>(B) * p.runs;
+  const long long ctas = parts * ((dim + kCols - 1) / kCols);
   if (ctas > 0x7fffffffll) return fail(BTP_ERR_BAD_SHAPE, "%s: too many elements for one launch", fn);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   rc = launched(fn, dispatch(dtype, width, [&](auto tag, auto taps) {
     using T = decltype(tag);
     constexpr int W = decltype(taps)::value;
-    if (al) return launch_kernel(conv_backward_kernel<T, 4, W>, static_cast<int>(ctas), 256, 0, st, p);
-    return launch_kernel(conv_backward_kernel<T, 1, W>, static_cast<int>(ctas), 256, 0, st, p);
+    constexpr int kSmem = static_cast<int>(sizeof(ConvTile<T, 2>));
+    // per device and process: the same value every time, so a race of two threads is harmless
+    const cudaError_t err = cudaFuncSetAttribute(conv_backward_kernel<T, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (err != cudaSuccess) return err;
+    return launch_kernel(conv_backward_kernel<T, W>, static_cast<int>(ctas), kThreads, kSmem, st, p);
   }));
   if (rc || !p.partial) return rc;
   const long long cols = static_cast<long long>(width + 1) * dim;
@@ -153,19 +154,18 @@ int btp_sm100_causal_conv_step(const void* x, const void* state, const void* wei
   int dev;
   DeviceInfo info;
   if ((rc = device_info(&dev, &info))) return rc;
-  const int e = elem_bytes(dtype), vec = 16 / e;
-  const bool al = dim % vec == 0 && (ld_x * e) % 16 == 0 && aligned16(x) && aligned16(y) && aligned16(state) && aligned16(state_out);
   ConvStepParams p{};
+  p.aligned = one_word(kStepChannels, elem_bytes(dtype), dim, ld_x, 0, {x, y, state, state_out});
+  p.whole_w = aligned16(weight);
   p.x = x; p.state = state; p.weight = weight; p.bias = bias; p.y = y; p.state_out = state_out;
   p.ld_x = ld_x; p.B = B; p.dim = dim; p.silu = silu != 0; p.weight_f32 = weight_dtype == BTP_DTYPE_F32;
-  const long long ctas = (static_cast<long long>(B) * (dim / (al ? vec : 1)) + 127) / 128;
+  const long long ctas = (static_cast<long long>(B) * ((dim + kStepChannels - 1) / kStepChannels) + 127) / 128;
   if (ctas > 0x7fffffffll) return fail(BTP_ERR_BAD_SHAPE, "%s: too many elements for one launch", fn);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return launched(fn, dispatch(dtype, width, [&](auto tag, auto taps) {
     using T = decltype(tag);
     constexpr int W = decltype(taps)::value;
-    if (al) return launch_kernel(conv_step_kernel<T, vec_of<T>(), W>, static_cast<int>(ctas), 128, 0, st, p);
-    return launch_kernel(conv_step_kernel<T, 1, W>, static_cast<int>(ctas), 128, 0, st, p);
+    return launch_kernel(conv_step_kernel<T, W>, static_cast<int>(ctas), 128, 0, st, p);
   }));
 }
 

@@ -68,52 +68,6 @@ struct Tile {
   float C2[kTile][kStates * 2];
 };
 
-__device__ __forceinline__ void copy16(void* to, const void* from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from) : "memory");
-}
-__device__ __forceinline__ void copy8(void* to, const void* from) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from) : "memory");
-}
-__device__ __forceinline__ void copy4(void* to, const void* from) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
-// ROWS rows of COLS elements (row pitch `pitch`, `cols` of them there) into dst[ROWS][COLS], by the threads of a group of
-// GROUP threads.  Rows from `rows` on and columns from `cols` on are not touched.
-template <class T, int ROWS, int COLS, int GROUP>
-__device__ __forceinline__ void fetch(T (*dst)[COLS], const T* src, long long pitch, int rows, int cols, bool aligned, int tid) {
-  constexpr int kBytes = COLS * static_cast<int>(sizeof(T)) < 16 ? 8 : 16, E = kBytes / static_cast<int>(sizeof(T)), CPR = COLS / E;
-  static_assert(COLS % E == 0 && CPR >= 1, "a row is whole copies");
-  if (aligned) {
-#pragma unroll
-    for (int i0 = 0; i0 < ROWS * CPR; i0 += GROUP) {
-      const int i = i0 + tid, r = i / CPR, c = (i - r * CPR) * E;
-      if ((ROWS * CPR % GROUP == 0 || i < ROWS * CPR) && r < rows && c < cols) {
-        if (kBytes == 16)
-          copy16(&dst[r][c], src + r * pitch + c);
-        else
-          copy8(&dst[r][c], src + r * pitch + c);
-      }
-    }
-  } else {
-#pragma unroll 4
-    for (int i0 = 0; i0 < ROWS * COLS; i0 += GROUP) {
-      const int i = i0 + tid, r = i / COLS, c = i - r * COLS;
-      if (i < ROWS * COLS && r < rows && c < cols) {
-        if (sizeof(T) == 4)
-          copy4(&dst[r][c], src + r * pitch + c);
-        else
-          dst[r][c] = src[r * pitch + c];
-      }
-    }
-  }
-}
-
 // Sums four values over the SG lanes of a state group.  SG >= 4: lane s ends with value s & 3; SG == 2: lane s with values
 // 2s and 2s + 1.  v[0], v[1] are the pairs (0, 1) and (2, 3).
 template <int SG>
@@ -235,17 +189,6 @@ struct FwdTile {
   T B[2][kTile][kStates];
   T C[2][kTile][kStates];
 };
-
-// Four consecutive elements, aligned to all of them, as pairs of floats.
-__device__ __forceinline__ void load_quad(f32x2 (&out)[2], const float* p) {
-  const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(p);
-  out[0] = w.x, out[1] = w.y;
-}
-template <class T>
-__device__ __forceinline__ void load_quad(f32x2 (&out)[2], const T* p) {
-  const uint2 w = *reinterpret_cast<const uint2*>(p);
-  out[0] = word_pair(w.x, T{}), out[1] = word_pair(w.y, T{});
-}
 
 // Four consecutive states of the channels c0, c1 as pairs of states; a channel or state that is not there is 0.
 struct PairState {
@@ -525,63 +468,100 @@ struct ScanStepParams {
   long long ld_x, ld_d, ld_z, ld_B, ld_C;
   int batch, dim, N;
   bool softplus;
+  bool al_B, al_C;     // four states of B and C are one word
+  int ctas;            // CTAs over the channels
 };
 
-constexpr int kStepBatch = 4;  // sequences per thread: they share A, D and the bias
+constexpr int kStepBatch = 4;  // sequences per thread
 
-// SG lanes share a channel, 4 states each.  The states' traffic bounds it: 8 bytes per state.
+// SG lanes share a channel, 4 states each, for four sequences at a time: four states' loads are under way together, A is read once, and
+// each lane prepares (step size, input, later gate and output) its share of the four and hands it to the others, as the prompt's
+// kernel does with four tokens.  Bound by the states' traffic, 8 bytes per state.
+// Measured at 256 sequences x 4096 channels x 16 states: STEPUS; with every lane preparing for itself 54 us (four times the instructions).
 template <class T, int SG>
 __global__ void __launch_bounds__(128) scan_step_kernel(const ScanStepParams p) {
+  constexpr int kOwn = SG >= 4 ? 1 : 4 / SG;
   grid_dependency_wait();
-  const long long idx = static_cast<long long>(blockIdx.x) * 128 + threadIdx.x;
-  const long long per_group = (static_cast<long long>(p.dim) * SG + 31) / 32 * 32;  // whole warps: the exchange below needs all lanes
-  const long long bg = idx / per_group;
-  const int in = static_cast<int>(idx - bg * per_group);
-  const int d = in / SG, s = in % SG, n0 = 4 * s;
-  if (bg * kStepBatch >= p.batch) return;
+  const int in = static_cast<int>(blockIdx.x % p.ctas) * 128 + threadIdx.x;
+  const int lane = threadIdx.x & 31, d = in / SG, s = in % SG, n0 = 4 * s;
   const bool ok = d < p.dim;
-  const int dd = ok ? d : p.dim - 1;
-  float A[4], h[kStepBatch][4], Bn[kStepBatch][4], Cn[kStepBatch][4], x[kStepBatch], v[kStepBatch], z[kStepBatch];
-  const int nb = min(kStepBatch, p.batch - static_cast<int>(bg) * kStepBatch);
-  const long long b0 = bg * kStepBatch;
+  const int dd = ok ? d : p.dim - 1;  // lanes without a channel follow the last one: the exchanges below need whole warps
+  const int b0 = static_cast<int>(blockIdx.x / p.ctas) * kStepBatch, nb = min(kStepBatch, p.batch - b0);
+  float h[kStepBatch][4], A[4];
+  f32x2 Bn[kStepBatch][2], Cn[kStepBatch][2];
 #pragma unroll
   for (int i = 0; i < kStepBatch; ++i) {
-    if (i >= nb) break;
-    const long long b = b0 + i;
+    const long long b = b0 + (i < nb ? i : 0);
     load_states(h[i], p.state + (b * p.dim + dd) * p.N, n0, p.N);
+    load_channels<2>(Bn[i], static_cast<const T*>(p.B) + b * p.ld_B + n0, p.al_B && n0 < p.N, p.N - n0);
+    load_channels<2>(Cn[i], static_cast<const T*>(p.C) + b * p.ld_C + n0, p.al_C && n0 < p.N, p.N - n0);
+  }
+  const int mine = SG >= 4 ? (s & 3) : s * kOwn;  // first sequence of the four that this lane prepares
+  float x[kOwn], v[kOwn], z[kOwn];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      Bn[i][k] = n0 + k < p.N ? to_f(static_cast<const T*>(p.B)[b * p.ld_B + n0 + k]) : 0.f;
-      Cn[i][k] = n0 + k < p.N ? to_f(static_cast<const T*>(p.C)[b * p.ld_C + n0 + k]) : 0.f;
-    }
-    x[i] = to_f(static_cast<const T*>(p.x)[b * p.ld_x + dd]);
-    v[i] = to_f(static_cast<const T*>(p.delta)[b * p.ld_d + dd]);
-    z[i] = p.z ? to_f(static_cast<const T*>(p.z)[b * p.ld_z + dd]) : 0.f;
+  for (int k = 0; k < kOwn; ++k) {
+    const long long b = b0 + (mine + k < nb ? mine + k : 0);
+    x[k] = to_f(static_cast<const T*>(p.x)[b * p.ld_x + dd]);
+    v[k] = to_f(static_cast<const T*>(p.delta)[b * p.ld_d + dd]);
+    z[k] = p.z ? to_f(static_cast<const T*>(p.z)[b * p.ld_z + dd]) : 0.f;
   }
   load_states(A, p.A + static_cast<long long>(dd) * p.N, n0, p.N);
   const float bias = p.bias ? p.bias[dd] : 0.f, skip = p.D ? p.D[dd] : 0.f;
+  f32x2 A2[2];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    A[k] *= kLog2e;
+    A[k] = A[k] < -3e38f ? -3e38f : A[k];  // held above -inf as in the prompt's kernel; NaN stays
+  }
+  A2[0] = pack2(A[0], A[1]), A2[1] = pack2(A[2], A[3]);
+  float u[kOwn];
+#pragma unroll
+  for (int k = 0; k < kOwn; ++k) {
+    v[k] += bias;
+    if (p.softplus) v[k] = softplus(v[k]);
+    u[k] = v[k] * x[k];
+  }
+  float y[kStepBatch];
 #pragma unroll
   for (int i = 0; i < kStepBatch; ++i) {
-    if (i >= nb) break;
-    const long long b = b0 + i;
-    float de = v[i] + bias;
-    if (p.softplus) de = softplus(de);
-    const float u = de * x[i];
-    float y = 0.f;
+    const int from = lane - s + i / kOwn;
+    const f32x2 d2 = both(__shfl_sync(0xffffffffu, v[i % kOwn], from)), u2 = both(__shfl_sync(0xffffffffu, u[i % kOwn], from));
+    f32x2 g[2];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      h[i][k] = fmaf(ex2(de * (A[k] * kLog2e)), h[i][k], u * Bn[i][k]);
-      if (n0 + k < p.N) y = fmaf(Cn[i][k], h[i][k], y);
+    for (int k = 0; k < 2; ++k) {
+      g[k] = fma2(ex2_2(mul2(d2, A2[k])), pack2(h[i][2 * k], h[i][2 * k + 1]), mul2(u2, Bn[i][k]));
+      if (n0 + 2 * k >= p.N) g[k] = 0ull;  // states that are not there
+      if (n0 + 2 * k + 1 >= p.N) g[k] = pack2(lo2(g[k]), 0.f);
+      unpack2(h[i][2 * k], h[i][2 * k + 1], g[k]);
     }
+    const f32x2 sum = fma2(Cn[i][1], g[1], mul2(Cn[i][0], g[0]));
+    y[i] = lo2(sum) + hi2(sum);
+  }
+  if (ok) {
 #pragma unroll
-    for (int o = SG / 2; o; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-    if (!ok) continue;
-    store_states(p.state_out + (b * p.dim + dd) * p.N, h[i], n0, p.N);
-    if (s == 0) {
-      y = fmaf(skip, x[i], y);
-      if (p.z) y *= z[i] * sigmoid(z[i]);
-      static_cast<T*>(p.y)[b * p.dim + d] = from_f<T>(y);
-    }
+    for (int i = 0; i < kStepBatch; ++i)
+      if (i < nb) store_states(p.state_out + (static_cast<long long>(b0 + i) * p.dim + d) * p.N, h[i], n0, p.N);
+  }
+  // sums over the channel's lanes: each ends with the sequences that it has prepared
+  float out[kOwn];
+  if constexpr (SG == 2) {
+    const bool up = s & 1;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) out[k] = (up ? y[2 + k] : y[k]) + __shfl_xor_sync(0xffffffffu, up ? y[k] : y[2 + k], 1);
+  } else {
+    const bool hi = s & 2, odd = s & 1;
+    float a[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) a[k] = (hi ? y[2 + k] : y[k]) + __shfl_xor_sync(0xffffffffu, hi ? y[k] : y[2 + k], 2);
+    out[0] = (odd ? a[1] : a[0]) + __shfl_xor_sync(0xffffffffu, odd ? a[0] : a[1], 1);
+#pragma unroll
+    for (int o = 4; o < SG; o *= 2) out[0] += __shfl_xor_sync(0xffffffffu, out[0], o);
+  }
+#pragma unroll
+  for (int k = 0; k < kOwn; ++k) {
+    float r = fmaf(skip, x[k], out[k]);
+    if (p.z) r *= z[k] * sigmoid(z[k]);
+    if (ok && mine + k < nb && (SG < 8 || s < 4)) static_cast<T*>(p.y)[static_cast<long long>(b0 + mine + k) * p.dim + d] = from_f<T>(r);
   }
 }
 

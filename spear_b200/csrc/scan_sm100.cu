@@ -272,9 +272,14 @@ int btp_sm100_scan_step(const void* x, const void* delta, const float* A, const 
   p.x = x; p.delta = delta; p.B = Bm; p.C = Cm; p.z = z; p.A = A; p.D = D; p.bias = delta_bias; p.state = state; p.state_out = state_out; p.y = y;
   p.ld_x = ld_x; p.ld_d = ld_d; p.ld_z = ld_z; p.ld_B = ld_B; p.ld_C = ld_C;
   p.batch = B; p.dim = dim; p.N = N; p.softplus = delta_softplus != 0;
-  const long long groups_b = (B + kStepBatch - 1) / kStepBatch;
-  const long long threads = (static_cast<long long>(dim) * state_groups(N) + 31) / 32 * 32 * groups_b;
-  const long long ctas = (threads + 127) / 128;
+  const auto quads = [&](const void* q, long long ld) {
+    return N % 4 == 0 && ld % 4 == 0 && (reinterpret_cast<uintptr_t>(q) & static_cast<uintptr_t>(4 * elem_bytes(dtype) - 1)) == 0;
+  };
+  p.al_B = quads(Bm, ld_B);
+  p.al_C = quads(Cm, ld_C);
+  const long long over = (static_cast<long long>(dim) * state_groups(N) + 127) / 128;
+  const long long ctas = over * ((B + kStepBatch - 1) / kStepBatch);
+  p.ctas = static_cast<int>(over);
   if (ctas > 0x7fffffffll || static_cast<long long>(dim) * 16 > 0x7fffffffll) return fail(BTP_ERR_BAD_SHAPE, "%s: too many elements for one launch", fn);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return launched(fn, dispatch(dtype, N, [&](auto tag, auto groups) {
