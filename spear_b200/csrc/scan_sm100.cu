@@ -249,7 +249,7 @@ int btp_sm100_scan_backward(const void* x, const void* delta, const float* A, co
                          static_cast<const float*>(bp.partial_bc), dB, dC, lengths, B, L, N, w.blocks);
   }));
   if (rc) return rc;
-  return launched(fn, launch_kernel(column_sum_kernel<float>, static_cast<int>((cols + 31) / 32), 256, 0, st,
+  return launched(fn, launch_kernel(column_sum_kernel<float, 8>, static_cast<int>((cols + 31) / 32), 256, 0, st,
                                     static_cast<const float*>(bp.partial_par), static_cast<void*>(dparams), s.splits * B, cols, true));
 }
 

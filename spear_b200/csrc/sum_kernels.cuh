@@ -5,24 +5,24 @@
 
 namespace btp_elem {
 
-// out[j] = sum over i of part[i][j], in the order of i within each of 8 strands and then of the strands; out in float or T.
-// CTA: 32 columns x 8 strands.
-template <class T>
-__global__ void __launch_bounds__(256) column_sum_kernel(const float* part, void* out, int parts, long long cols, bool out_f32) {
-  __shared__ float s[8][33];
+// out[j] = sum over i of part[i][j], in the order of i within each strand and then of the strands; out in float or T.
+// CTA: 32 columns x STRANDS (8 for a few rows, 32 for hundreds).
+template <class T, int STRANDS>
+__global__ void __launch_bounds__(32 * STRANDS) column_sum_kernel(const float* part, void* out, int parts, long long cols, bool out_f32) {
+  __shared__ float s[STRANDS][33];
   const int lane = threadIdx.x & 31, strand = threadIdx.x >> 5;
   const long long j = static_cast<long long>(blockIdx.x) * 32 + lane;
   grid_dependency_wait();
   float a = 0.f;
   if (j < cols)
 #pragma unroll 4
-    for (int i = strand; i < parts; i += 8) a += part[i * cols + j];
+    for (int i = strand; i < parts; i += STRANDS) a += part[i * cols + j];
   s[strand][lane] = a;
   __syncthreads();
   if (strand == 0 && j < cols) {
     a = s[0][lane];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) a += s[i][lane];
+    for (int i = 1; i < STRANDS; ++i) a += s[i][lane];
     if (out_f32)
       static_cast<float*>(out)[j] = a;
     else

@@ -172,7 +172,8 @@ def rms_norm_8bit(x: torch.Tensor, weight: torch.Tensor | None = None, residual:
         block: None for one scale per row, 128 for one scale per 128 columns (the last may hold fewer).
     Returns:
         (q, scale) or, with a residual, (q, scale, h): q [..., D] float8_e4m3fn, scale [...] or
-        [..., ceil(D / 128)] with y = q * scale; scale = max|y| / 448, or 1 where that maximum is 0 or NaN.
+        [..., ceil(D / 128)] with y = q * scale; scale = max|y| / 448, or 1 where that is NaN or below 1e-37
+        (a row of zeros).
     """
     if block not in _OUT:
         raise ValueError(f"rms_norm_8bit: block must be None or {SCALE_BLOCK} (got {block})")
