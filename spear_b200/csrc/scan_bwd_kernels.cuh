@@ -64,44 +64,41 @@ struct BwdTile {
   float4 park[kTile / kStep][4][BwdShape<SG>::kThreads];
 };
 
-// dB, dC of this lane's channels, v = (dB of states n0..n0+3, dC of the same), summed over the warp's channel groups and stored.
+// dB, dC of this lane's channels, v = (dB of states n0..n0+3, dC of the same), summed over the warp's channel groups: lanes exchange halves
+// until each holds kHeld of the eight sums, at place channel_slot() of a row (dB of all states, dC of all states).
 template <int SG>
-__device__ __forceinline__ void reduce_channels(float* row, const float (&v)[8], int lane, int n0) {
-  constexpr int NP = 4 * SG;
+struct ChannelSums {
+  static constexpr int kHeld = SG == 16 ? 4 : SG == 8 ? 2 : 1;
+  float v[kHeld];
+};
+template <int SG>
+__device__ __forceinline__ int channel_slot(int lane, int n0) {
+  return (lane & 16 ? 4 * SG : 0) + n0 + (SG <= 8 && lane & 8 ? 2 : 0) + (SG <= 4 && lane & 4 ? 1 : 0);
+}
+template <int SG>
+__device__ __forceinline__ ChannelSums<SG> reduce_channels(const float (&v)[8], int lane) {
+  ChannelSums<SG> r;
   float a[4];
   const bool hi = lane & 16;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const float keep = hi ? v[4 + k] : v[k], give = hi ? v[k] : v[4 + k];
-    a[k] = keep + __shfl_xor_sync(0xffffffffu, give, 16);
-  }
-  float* to = row + (hi ? NP : 0) + n0;
-  if (SG == 16) {
-    *reinterpret_cast<float4*>(to) = make_float4(a[0], a[1], a[2], a[3]);
-    return;
-  }
-  const bool b3 = lane & 8;
-  float c[2];
+  for (int k = 0; k < 4; ++k) a[k] = (hi ? v[4 + k] : v[k]) + __shfl_xor_sync(0xffffffffu, hi ? v[k] : v[4 + k], 16);
+  if constexpr (SG == 16) {
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const float keep = b3 ? a[2 + k] : a[k], give = b3 ? a[k] : a[2 + k];
-    c[k] = keep + __shfl_xor_sync(0xffffffffu, give, 8);
-  }
-  to += b3 ? 2 : 0;
-  if (SG == 8) {
-    *reinterpret_cast<float2*>(to) = make_float2(c[0], c[1]);
-    return;
-  }
-  const bool b2 = lane & 4;
-  const float keep = b2 ? c[1] : c[0], give = b2 ? c[0] : c[1];
-  float r = keep + __shfl_xor_sync(0xffffffffu, give, 4);
-  to += b2 ? 1 : 0;
-  if (SG == 2) {
-    r += __shfl_xor_sync(0xffffffffu, r, 2);
-    if (!(lane & 2)) *to = r;
+    for (int k = 0; k < 4; ++k) r.v[k] = a[k];
   } else {
-    *to = r;
+    const bool b3 = lane & 8;
+    float c[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) c[k] = (b3 ? a[2 + k] : a[k]) + __shfl_xor_sync(0xffffffffu, b3 ? a[k] : a[2 + k], 8);
+    if constexpr (SG == 8) {
+      r.v[0] = c[0], r.v[1] = c[1];
+    } else {
+      const bool b2 = lane & 4;
+      r.v[0] = (b2 ? c[1] : c[0]) + __shfl_xor_sync(0xffffffffu, b2 ? c[0] : c[1], 4);
+      if (SG == 2) r.v[0] += __shfl_xor_sync(0xffffffffu, r.v[0], 2);
+    }
   }
+  return r;
 }
 
 // One warp per (channels, chunk from the second on, sequence): the gradient that the chunk hands to the state before it when none
@@ -126,13 +123,15 @@ __global__ void __launch_bounds__(32) scan_backward_carry_kernel(const ScanBwdPa
   const int cols = min(WC, p.dim - cw);
   const bool full = p.N == NP;
   LaneState A2, G;
-  load_lane(A2, p.A, c0, p.dim, n0, p.N, kLog2e);
+  load_rates(A2, p.A, c0, p.dim, n0, p.N);
 #pragma unroll
   for (int n = 0; n < 4; ++n) G.r[0][n] = G.r[1][n] = 0ull;
   const int cp = lane % CP, row0 = lane / CP, pc = cw + 2 * cp;
-  float bias[2];
-#pragma unroll
-  for (int k = 0; k < 2; ++k) bias[k] = p.bias && pc + k < p.dim ? p.bias[pc + k] : 0.f;
+  const f32x2 bias = channel_pair(p.bias, pc, p.dim);
+  for (int i = lane; i < 2 * kTile * (WC - cols); i += 32) {  // channels that are not there: never copied, read as zeros
+    const int at = i / (WC - cols) * WC + cols + i % (WC - cols);
+    (&sm.x[0][0][0])[at] = (&sm.d[0][0][0])[at] = (&sm.z[0][0][0])[at] = from_f<T>(0.f);
+  }
   const T* dl = static_cast<const T*>(p.delta) + b * p.d_b + cw;
   const T* z = p.z ? static_cast<const T*>(p.z) + b * p.z_b + cw : nullptr;
   const T* Cm = static_cast<const T*>(p.C) + b * p.C_b;
@@ -158,22 +157,15 @@ __global__ void __launch_bounds__(32) scan_backward_carry_kernel(const ScanBwdPa
 #pragma unroll
     for (int i = 0; i < kTile; i += RPI) {
       const int r = i + row0;
-      float de[2], gy[2];
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const bool ok = r < nt && pc + k < p.dim;
-        float v = ok ? to_f(sm.d[st][r][2 * cp + k]) + bias[k] : 0.f;
-        if (p.softplus) v = softplus(v);
-        de[k] = ok ? v : 0.f;
-        float e = ok ? to_f(sm.x[st][r][2 * cp + k]) : 0.f;
-        if (z && ok) {
-          const float zz = to_f(sm.z[st][r][2 * cp + k]);
-          e *= zz * sigmoid(zz);
-        }
-        gy[k] = e;
+      f32x2 v = add2(load_pair(&sm.d[st][r][2 * cp]), bias), e = load_pair(&sm.x[st][r][2 * cp]);
+      if (p.softplus) v = softplus2(v);
+      if (z) {
+        const f32x2 zz = load_pair(&sm.z[st][r][2 * cp]);
+        e = mul2(e, mul2(zz, sigmoid2(zz)));
       }
-      *reinterpret_cast<float2*>(&sm.delta[r][2 * cp]) = make_float2(de[0], de[1]);
-      *reinterpret_cast<float2*>(&sm.u[r][2 * cp]) = make_float2(gy[0], gy[1]);
+      if (r >= nt) v = e = 0ull;
+      *reinterpret_cast<f32x2*>(&sm.delta[r][2 * cp]) = v;
+      *reinterpret_cast<f32x2*>(&sm.u[r][2 * cp]) = e;
     }
 #pragma unroll
     for (int i = 0; i < kTile * NP / 2; i += 32) {
@@ -182,22 +174,30 @@ __global__ void __launch_bounds__(32) scan_backward_carry_kernel(const ScanBwdPa
       *reinterpret_cast<float4*>(&sm.C2[r][2 * n]) = make_float4(e0, e0, e1, e1);
     }
     __syncwarp();
-#pragma unroll 4
-    for (int t = nt - 1; t >= 0; --t) {
-      const ulonglong2 d2 = *reinterpret_cast<const ulonglong2*>(&sm.delta[t][4 * g]);
-      const ulonglong2 e2 = *reinterpret_cast<const ulonglong2*>(&sm.u[t][4 * g]);
-      const ulonglong2 ca = *reinterpret_cast<const ulonglong2*>(&sm.C2[t][8 * s]);
-      const ulonglong2 cc = *reinterpret_cast<const ulonglong2*>(&sm.C2[t][8 * s + 4]);
-      const f32x2 cn[4] = {ca.x, ca.y, cc.x, cc.y};
+    const auto walk = [&](auto usual) {
+      for (int t = (nt - 1) & ~3; t >= 0; t -= 4) {
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        G.r[0][n] = mul2(ex2_2(mul2(d2.x, A2.r[0][n])), fma2(cn[n], e2.x, G.r[0][n]));
-        G.r[1][n] = mul2(ex2_2(mul2(d2.y, A2.r[1][n])), fma2(cn[n], e2.y, G.r[1][n]));
+        for (int j = 3; j >= 0; --j) {  // rows behind the last token hold zeros: they leave the gradient as it is
+          const ulonglong2 d2 = *reinterpret_cast<const ulonglong2*>(&sm.delta[t + j][4 * g]);
+          const ulonglong2 e2 = *reinterpret_cast<const ulonglong2*>(&sm.u[t + j][4 * g]);
+          const ulonglong2 ca = *reinterpret_cast<const ulonglong2*>(&sm.C2[t + j][8 * s]);
+          const ulonglong2 cc = *reinterpret_cast<const ulonglong2*>(&sm.C2[t + j][8 * s + 4]);
+          const f32x2 cn[4] = {ca.x, ca.y, cc.x, cc.y};
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            G.r[0][n] = mul2(ex2_2(mul2(d2.x, A2.r[0][n])), fma2(cn[n], e2.x, G.r[0][n]));
+            G.r[1][n] = mul2(ex2_2(mul2(d2.y, A2.r[1][n])), fma2(cn[n], e2.y, G.r[1][n]));
+          }
+          if (!decltype(usual)::value) clear_padding(G, n0, p.N);
+          sum0 = add2(sum0, d2.x);
+          sum1 = add2(sum1, d2.y);
+        }
       }
-      if (!full) clear_padding(G, n0, p.N);
-      sum0 = add2(sum0, d2.x);
-      sum1 = add2(sum1, d2.y);
-    }
+    };
+    if (full)
+      walk(std::true_type{});
+    else
+      walk(std::false_type{});
     __syncwarp();
   }
   copy_wait<0>();
@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(BwdShape<SG>::kThreads) scan_backward_kernel(c
   const bool full = p.N == NP;
 
   LaneState A2, G, dA;
-  load_lane(A2, p.A, c0, p.dim, n0, p.N, kLog2e);
+  load_rates(A2, p.A, c0, p.dim, n0, p.N);
 #pragma unroll
   for (int n = 0; n < 4; ++n) G.r[0][n] = G.r[1][n] = dA.r[0][n] = dA.r[1][n] = 0ull;
   const long long per_chunk = static_cast<long long>(p.batch) * p.dim;
@@ -251,11 +251,11 @@ __global__ void __launch_bounds__(BwdShape<SG>::kThreads) scan_backward_kernel(c
     }
   }
   const int cp = tid % CP, row0 = tid / CP, pc = cw + 2 * cp;
-  float bias[2], skip[2], sum_d[2] = {}, sum_b[2] = {};
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    bias[k] = p.bias && pc + k < p.dim ? p.bias[pc + k] : 0.f;
-    skip[k] = p.D && pc + k < p.dim ? p.D[pc + k] : 0.f;
+  const f32x2 bias = channel_pair(p.bias, pc, p.dim), skip = channel_pair(p.D, pc, p.dim);
+  f32x2 sum_d = 0ull, sum_b = 0ull;
+  for (int i = tid; i < 2 * kTile * (CW - cols); i += NT) {  // channels that are not there: never copied, read as zeros
+    const int at = i / (CW - cols) * CW + cols + i % (CW - cols);
+    (&sm.x[0][0][0])[at] = (&sm.d[0][0][0])[at] = (&sm.z[0][0][0])[at] = (&sm.dy[0][0][0])[at] = from_f<T>(0.f);
   }
   const T* x = static_cast<const T*>(p.x) + b * p.x_b + cw;
   const T* dl = static_cast<const T*>(p.delta) + b * p.d_b + cw;
@@ -292,24 +292,17 @@ __global__ void __launch_bounds__(BwdShape<SG>::kThreads) scan_backward_kernel(c
 #pragma unroll
     for (int i = 0; i < kTile; i += RPI) {
       const int r = i + row0;
-      float de[2], uu[2], gy[2];
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const bool ok = r < nt && pc + k < p.dim;
-        float v = ok ? to_f(sm.d[st][r][2 * cp + k]) + bias[k] : 0.f;
-        if (p.softplus) v = softplus(v);
-        de[k] = ok ? v : 0.f;
-        uu[k] = ok ? v * to_f(sm.x[st][r][2 * cp + k]) : 0.f;
-        float e = ok ? to_f(sm.dy[st][r][2 * cp + k]) : 0.f;
-        if (z && ok) {
-          const float zz = to_f(sm.z[st][r][2 * cp + k]);
-          e *= zz * sigmoid(zz);
-        }
-        gy[k] = e;
+      f32x2 v = add2(load_pair(&sm.d[st][r][2 * cp]), bias), e = load_pair(&sm.dy[st][r][2 * cp]);
+      if (p.softplus) v = softplus2(v);
+      f32x2 w = mul2(v, load_pair(&sm.x[st][r][2 * cp]));
+      if (z) {
+        const f32x2 zz = load_pair(&sm.z[st][r][2 * cp]);
+        e = mul2(e, mul2(zz, sigmoid2(zz)));
       }
-      *reinterpret_cast<float2*>(&sm.delta[r][2 * cp]) = make_float2(de[0], de[1]);
-      *reinterpret_cast<float2*>(&sm.u[r][2 * cp]) = make_float2(uu[0], uu[1]);
-      *reinterpret_cast<float2*>(&sm.gy[r][2 * cp]) = make_float2(gy[0], gy[1]);
+      if (r >= nt) v = w = e = 0ull;  // rows behind the last token: zeros leave the state and its gradient as they are
+      *reinterpret_cast<f32x2*>(&sm.delta[r][2 * cp]) = v;
+      *reinterpret_cast<f32x2*>(&sm.u[r][2 * cp]) = w;
+      *reinterpret_cast<f32x2*>(&sm.gy[r][2 * cp]) = e;
     }
     for (int i = tid; i < kTile * NP / 2; i += NT) {
       const int r = i / (NP / 2), n = i % (NP / 2) * 2;
@@ -320,117 +313,138 @@ __global__ void __launch_bounds__(BwdShape<SG>::kThreads) scan_backward_kernel(c
       *reinterpret_cast<float4*>(&sm.C2[r][2 * n]) = make_float4(e0, e0, e1, e1);
     }
     __syncthreads();
-    // forward over the tile: park the state before each step of 4 tokens
     const int steps = (nt + kStep - 1) / kStep;
-    for (int k = 0; k < steps; ++k) {
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        float4 v;
-        unpack2(v.x, v.y, h.r[0][n]);
-        unpack2(v.z, v.w, h.r[1][n]);
-        sm.park[k][n][tid] = v;
-      }
-      if (k + 1 == steps) break;
-#pragma unroll
-      for (int j = 0; j < kStep; ++j) {
-        const int t = k * kStep + j;
-        const ulonglong2 d2 = *reinterpret_cast<const ulonglong2*>(&sm.delta[t][cl]);
-        const ulonglong2 u2 = *reinterpret_cast<const ulonglong2*>(&sm.u[t][cl]);
-        const ulonglong2 ba = *reinterpret_cast<const ulonglong2*>(&sm.B2[t][8 * s]);
-        const ulonglong2 bb = *reinterpret_cast<const ulonglong2*>(&sm.B2[t][8 * s + 4]);
-        const f32x2 bn[4] = {ba.x, ba.y, bb.x, bb.y};
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          h.r[0][n] = fma2(ex2_2(mul2(d2.x, A2.r[0][n])), h.r[0][n], mul2(u2.x, bn[n]));
-          h.r[1][n] = fma2(ex2_2(mul2(d2.y, A2.r[1][n])), h.r[1][n], mul2(u2.y, bn[n]));
-        }
-        if (!full) clear_padding(h, n0, p.N);
-      }
-    }
     LaneState dA_tile;
 #pragma unroll
     for (int n = 0; n < 4; ++n) dA_tile.r[0][n] = dA_tile.r[1][n] = 0ull;
-    for (int k = steps - 1; k >= 0; --k) {
-      LaneState a[kStep], w[kStep];  // decays, decayed states before the token's own input
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const float4 v = sm.park[k][n][tid];
-        h.r[0][n] = pack2(v.x, v.y);
-        h.r[1][n] = pack2(v.z, v.w);
-      }
-#pragma unroll
-      for (int j = 0; j < kStep; ++j) {
-        const int t = k * kStep + j;  // rows behind the last token hold zeros: they leave the state as it is
-        const ulonglong2 d2 = *reinterpret_cast<const ulonglong2*>(&sm.delta[t][cl]);
-        const ulonglong2 u2 = *reinterpret_cast<const ulonglong2*>(&sm.u[t][cl]);
-        const ulonglong2 ba = *reinterpret_cast<const ulonglong2*>(&sm.B2[t][8 * s]);
-        const ulonglong2 bb = *reinterpret_cast<const ulonglong2*>(&sm.B2[t][8 * s + 4]);
-        const f32x2 bn[4] = {ba.x, ba.y, bb.x, bb.y};
+    const auto walk = [&](auto usual, auto gated) {
+      constexpr bool kFull = decltype(usual)::value, kGate = decltype(gated)::value;
+      // forward over the tile: park the state before each step of 4 tokens
+      for (int k = 0; k < steps; ++k) {
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-          a[j].r[0][n] = ex2_2(mul2(d2.x, A2.r[0][n]));
-          a[j].r[1][n] = ex2_2(mul2(d2.y, A2.r[1][n]));
-          w[j].r[0][n] = mul2(a[j].r[0][n], h.r[0][n]);
-          w[j].r[1][n] = mul2(a[j].r[1][n], h.r[1][n]);
-          h.r[0][n] = fma2(u2.x, bn[n], w[j].r[0][n]);
-          h.r[1][n] = fma2(u2.y, bn[n], w[j].r[1][n]);
+          float4 v;
+          unpack2(v.x, v.y, h.r[0][n]);
+          unpack2(v.z, v.w, h.r[1][n]);
+          sm.park[k][n][tid] = v;
         }
-        if (!full) {
-          clear_padding(h, n0, p.N);
-          clear_padding(w[j], n0, p.N);
-        }
-      }
+        if (k + 1 == steps) break;
 #pragma unroll
-      for (int j = kStep - 1; j >= 0; --j) {
-        const int t = k * kStep + j;
-        if (t >= nt) continue;
-        const ulonglong2 d2 = *reinterpret_cast<const ulonglong2*>(&sm.delta[t][cl]);
-        const ulonglong2 u2 = *reinterpret_cast<const ulonglong2*>(&sm.u[t][cl]);
-        const ulonglong2 e2 = *reinterpret_cast<const ulonglong2*>(&sm.gy[t][cl]);
-        const ulonglong2 ba = *reinterpret_cast<const ulonglong2*>(&sm.B2[t][8 * s]);
-        const ulonglong2 bb = *reinterpret_cast<const ulonglong2*>(&sm.B2[t][8 * s + 4]);
-        const ulonglong2 ca = *reinterpret_cast<const ulonglong2*>(&sm.C2[t][8 * s]);
-        const ulonglong2 cc = *reinterpret_cast<const ulonglong2*>(&sm.C2[t][8 * s + 4]);
-        const f32x2 bn[4] = {ba.x, ba.y, bb.x, bb.y}, cn[4] = {ca.x, ca.y, cc.x, cc.y};
-        const f32x2 dp[2] = {d2.x, d2.y}, up[2] = {u2.x, u2.y}, ep[2] = {e2.x, e2.y};
-        f32x2 y[2] = {}, du[2] = {}, wa[2] = {};
-        float bc[8];
+        for (int j = 0; j < kStep; ++j) {
+          const int t = k * kStep + j;
+          const ulonglong2 d2 = *reinterpret_cast<const ulonglong2*>(&sm.delta[t][cl]);
+          const ulonglong2 u2 = *reinterpret_cast<const ulonglong2*>(&sm.u[t][cl]);
+          const ulonglong2 ba = *reinterpret_cast<const ulonglong2*>(&sm.B2[t][8 * s]);
+          const ulonglong2 bb = *reinterpret_cast<const ulonglong2*>(&sm.B2[t][8 * s + 4]);
+          const f32x2 bn[4] = {ba.x, ba.y, bb.x, bb.y};
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          f32x2 db = 0ull, dc = 0ull;
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            f32x2 gg = fma2(cn[n], ep[c], G.r[c][n]);
-            if (!full && n0 + n >= p.N) gg = 0ull;
-            const f32x2 hh = fma2(up[c], bn[n], w[j].r[c][n]);
-            y[c] = fma2(cn[n], hh, y[c]);
-            dc = fma2(ep[c], hh, dc);
-            db = fma2(gg, up[c], db);
-            du[c] = fma2(gg, bn[n], du[c]);
-            const f32x2 ww = mul2(gg, w[j].r[c][n]);
-            dA_tile.r[c][n] = fma2(ww, dp[c], dA_tile.r[c][n]);
-            wa[c] = fma2(ww, A2.r[c][n], wa[c]);
-            G.r[c][n] = mul2(gg, a[j].r[c][n]);
+          for (int n = 0; n < 4; ++n) {
+            h.r[0][n] = fma2(ex2_2(mul2(d2.x, A2.r[0][n])), h.r[0][n], mul2(u2.x, bn[n]));
+            h.r[1][n] = fma2(ex2_2(mul2(d2.y, A2.r[1][n])), h.r[1][n], mul2(u2.y, bn[n]));
           }
-          bc[n] = lo2(db) + hi2(db);
-          bc[4 + n] = lo2(dc) + hi2(dc);
-        }
-        reduce_channels<SG>(sm.red[warp][t], bc, lane, n0);
-        float oy[2], ou[2], ow[2];
-        reduce_states<SG>(oy, y[0], y[1], s);
-        reduce_states<SG>(ou, du[0], du[1], s);
-        reduce_states<SG>(ow, wa[0], wa[1], s);
-        __syncwarp();  // all lanes have read the token's u and dy: their places take du and sum C h
-        if (SG == 2) {
-          *reinterpret_cast<float2*>(&sm.gy[t][cl + 2 * s]) = make_float2(oy[0], oy[1]);
-          *reinterpret_cast<float2*>(&sm.u[t][cl + 2 * s]) = make_float2(ou[0], ou[1]);
-          *reinterpret_cast<float2*>(&sm.wa[t][cl + 2 * s]) = make_float2(ow[0], ow[1]);
-        } else if (SG == 4 || s < 4) {
-          sm.gy[t][cl + (s & 3)] = oy[0];
-          sm.u[t][cl + (s & 3)] = ou[0];
-          sm.wa[t][cl + (s & 3)] = ow[0];
+          if (!kFull) clear_padding(h, n0, p.N);
         }
       }
+      for (int k = steps - 1; k >= 0; --k) {
+        LaneState a[kStep], w[kStep];  // decays, decayed states before the token's own input
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const float4 v = sm.park[k][n][tid];
+          h.r[0][n] = pack2(v.x, v.y);
+          h.r[1][n] = pack2(v.z, v.w);
+        }
+#pragma unroll
+        for (int j = 0; j < kStep; ++j) {
+          const int t = k * kStep + j;
+          const ulonglong2 d2 = *reinterpret_cast<const ulonglong2*>(&sm.delta[t][cl]);
+          const ulonglong2 u2 = *reinterpret_cast<const ulonglong2*>(&sm.u[t][cl]);
+          const ulonglong2 ba = *reinterpret_cast<const ulonglong2*>(&sm.B2[t][8 * s]);
+          const ulonglong2 bb = *reinterpret_cast<const ulonglong2*>(&sm.B2[t][8 * s + 4]);
+          const f32x2 bn[4] = {ba.x, ba.y, bb.x, bb.y};
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            a[j].r[0][n] = ex2_2(mul2(d2.x, A2.r[0][n]));
+            a[j].r[1][n] = ex2_2(mul2(d2.y, A2.r[1][n]));
+            w[j].r[0][n] = mul2(a[j].r[0][n], h.r[0][n]);
+            w[j].r[1][n] = mul2(a[j].r[1][n], h.r[1][n]);
+            h.r[0][n] = fma2(u2.x, bn[n], w[j].r[0][n]);
+            h.r[1][n] = fma2(u2.y, bn[n], w[j].r[1][n]);
+          }
+          if (!kFull) {
+            clear_padding(h, n0, p.N);
+            clear_padding(w[j], n0, p.N);
+          }
+        }
+        // the step's results stay in registers until its last token: a store in between would order the next token's loads behind it
+        float oy[kStep][2], ou[kStep][2], ow[kStep][2];
+        ChannelSums<SG> sums[kStep];
+#pragma unroll
+        for (int j = kStep - 1; j >= 0; --j) {
+          const int t = k * kStep + j;
+          const ulonglong2 d2 = *reinterpret_cast<const ulonglong2*>(&sm.delta[t][cl]);
+          const ulonglong2 u2 = *reinterpret_cast<const ulonglong2*>(&sm.u[t][cl]);
+          const ulonglong2 e2 = *reinterpret_cast<const ulonglong2*>(&sm.gy[t][cl]);
+          const ulonglong2 ba = *reinterpret_cast<const ulonglong2*>(&sm.B2[t][8 * s]);
+          const ulonglong2 bb = *reinterpret_cast<const ulonglong2*>(&sm.B2[t][8 * s + 4]);
+          const ulonglong2 ca = *reinterpret_cast<const ulonglong2*>(&sm.C2[t][8 * s]);
+          const ulonglong2 cc = *reinterpret_cast<const ulonglong2*>(&sm.C2[t][8 * s + 4]);
+          const f32x2 bn[4] = {ba.x, ba.y, bb.x, bb.y}, cn[4] = {ca.x, ca.y, cc.x, cc.y};
+          const f32x2 dp[2] = {d2.x, d2.y}, up[2] = {u2.x, u2.y}, ep[2] = {e2.x, e2.y};
+          f32x2 y[2] = {}, du[2] = {}, wa[2] = {};
+          float bc[8];
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            f32x2 db = 0ull, dc = 0ull;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              f32x2 gg = fma2(cn[n], ep[c], G.r[c][n]);
+              if (!kFull && n0 + n >= p.N) gg = 0ull;
+              const f32x2 hh = fma2(up[c], bn[n], w[j].r[c][n]);
+              if (kGate) y[c] = fma2(cn[n], hh, y[c]);
+              dc = fma2(ep[c], hh, dc);
+              db = fma2(gg, up[c], db);
+              du[c] = fma2(gg, bn[n], du[c]);
+              const f32x2 ww = mul2(gg, w[j].r[c][n]);
+              dA_tile.r[c][n] = fma2(ww, dp[c], dA_tile.r[c][n]);
+              wa[c] = fma2(ww, A2.r[c][n], wa[c]);
+              G.r[c][n] = mul2(gg, a[j].r[c][n]);
+            }
+            bc[n] = lo2(db) + hi2(db);
+            bc[4 + n] = lo2(dc) + hi2(dc);
+          }
+          sums[j] = reduce_channels<SG>(bc, lane);
+          if (kGate) reduce_states<SG>(oy[j], y[0], y[1], s);
+          reduce_states<SG>(ou[j], du[0], du[1], s);
+          reduce_states<SG>(ow[j], wa[0], wa[1], s);
+        }
+        __syncwarp();  // all lanes have read the step's u and dy: their places take du and sum C h
+        const int slot = channel_slot<SG>(lane, n0);
+#pragma unroll
+        for (int j = 0; j < kStep; ++j) {
+          const int t = k * kStep + j;
+          if (SG > 2 || !(lane & 2)) {
+#pragma unroll
+            for (int i = 0; i < ChannelSums<SG>::kHeld; ++i) sm.red[warp][t][slot + i] = sums[j].v[i];
+          }
+          if (SG == 2) {
+            if (kGate) *reinterpret_cast<float2*>(&sm.gy[t][cl + 2 * s]) = make_float2(oy[j][0], oy[j][1]);
+            *reinterpret_cast<float2*>(&sm.u[t][cl + 2 * s]) = make_float2(ou[j][0], ou[j][1]);
+            *reinterpret_cast<float2*>(&sm.wa[t][cl + 2 * s]) = make_float2(ow[j][0], ow[j][1]);
+          } else if (SG == 4 || s < 4) {
+            if (kGate) sm.gy[t][cl + (s & 3)] = oy[j][0];
+            sm.u[t][cl + (s & 3)] = ou[j][0];
+            sm.wa[t][cl + (s & 3)] = ow[j][0];
+          }
+        }
+      }
+    };
+    if (full) {
+      if (z)
+        walk(std::true_type{}, std::true_type{});
+      else
+        walk(std::true_type{}, std::false_type{});
+    } else {
+      walk(std::false_type{}, std::true_type{});
     }
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
@@ -438,41 +452,32 @@ __global__ void __launch_bounds__(BwdShape<SG>::kThreads) scan_backward_kernel(c
       dA.r[1][n] = add2(dA.r[1][n], dA_tile.r[1][n]);
     }
     __syncthreads();
-    float tile_d[2] = {}, tile_b[2] = {};
+    f32x2 tile_d = 0ull, tile_b = 0ull;
 #pragma unroll
     for (int i = 0; i < kTile; i += RPI) {
-      const int r = i + row0;
+      const int r = i + row0, c = 2 * cp;
       if (r >= nt || pc >= p.dim) continue;
-      float ox[2], od[2], oz[2];
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int c = 2 * cp + k;
-        const bool ok = pc + k < p.dim;
-        const float xx = ok ? to_f(sm.x[st][r][c]) : 0.f, up = ok ? to_f(sm.dy[st][r][c]) : 0.f;
-        float e = up;
-        if (z) {
-          const float zz = ok ? to_f(sm.z[st][r][c]) : 0.f, sg = sigmoid(zz);
-          e = up * (zz * sg);
-          oz[k] = up * fmaf(skip[k], xx, sm.gy[r][c]) * (sg * fmaf(zz, 1.f - sg, 1.f));
-        }
-        const float du = sm.u[r][c];
-        ox[k] = fmaf(du, sm.delta[r][c], e * skip[k]);
-        float v = fmaf(du, xx, sm.wa[r][c] * kLn2);
-        if (p.softplus) v *= sigmoid((ok ? to_f(sm.d[st][r][c]) : 0.f) + bias[k]);
-        od[k] = v;
-        tile_d[k] = fmaf(e, xx, tile_d[k]);
-        tile_b[k] += v;
+      const f32x2 xx = load_pair(&sm.x[st][r][c]), up = load_pair(&sm.dy[st][r][c]);
+      const f32x2 du = *reinterpret_cast<const f32x2*>(&sm.u[r][c]), one = both(1.f);
+      const long long at = static_cast<long long>(t0 + r) * p.dim + c;
+      f32x2 e = up;
+      if (z) {
+        const f32x2 zz = load_pair(&sm.z[st][r][c]), sg = sigmoid2(zz);
+        e = mul2(up, mul2(zz, sg));
+        const f32x2 y0 = fma2(skip, xx, *reinterpret_cast<const f32x2*>(&sm.gy[r][c]));
+        const f32x2 slope = mul2(sg, fma2(zz, fma2(sg, both(-1.f), one), one));
+        store_pair<T>(dz + at, mul2(mul2(up, y0), slope), bp.al_out, p.dim - pc);
       }
-      const long long at = static_cast<long long>(t0 + r) * p.dim + 2 * cp;
-      store_run<T, 2>(dx + at, ox, bp.al_out, p.dim - pc);
-      store_run<T, 2>(dd + at, od, bp.al_out, p.dim - pc);
-      if (z) store_run<T, 2>(dz + at, oz, bp.al_out, p.dim - pc);
+      const f32x2 ox = fma2(du, *reinterpret_cast<const f32x2*>(&sm.delta[r][c]), mul2(e, skip));
+      f32x2 v = fma2(du, xx, mul2(*reinterpret_cast<const f32x2*>(&sm.wa[r][c]), both(kLn2)));
+      if (p.softplus) v = mul2(v, sigmoid2(add2(load_pair(&sm.d[st][r][c]), bias)));
+      store_pair<T>(dx + at, ox, bp.al_out, p.dim - pc);
+      store_pair<T>(dd + at, v, bp.al_out, p.dim - pc);
+      tile_d = fma2(e, xx, tile_d);
+      tile_b = add2(tile_b, v);
     }
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      sum_d[k] += tile_d[k];
-      sum_b[k] += tile_b[k];
-    }
+    sum_d = add2(sum_d, tile_d);
+    sum_b = add2(sum_b, tile_b);
     float* bc = bp.partial_bc + ((cb * static_cast<long long>(p.batch) + b) * p.L + t0) * 2 * p.N;
     for (int i = tid; i < nt * 2 * NP; i += NT) {
       const int r = i / (2 * NP), j = i % (2 * NP), n = j % NP;
@@ -498,11 +503,8 @@ __global__ void __launch_bounds__(BwdShape<SG>::kThreads) scan_backward_kernel(c
   __syncthreads();
   // the threads of one channel pair add up their rows
   float* strip = &sm.delta[0][0];  // [RPI][CW] and again for the bias
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    strip[row0 * CW + 2 * cp + k] = sum_d[k];
-    strip[(RPI + row0) * CW + 2 * cp + k] = sum_b[k];
-  }
+  *reinterpret_cast<f32x2*>(&strip[row0 * CW + 2 * cp]) = sum_d;
+  *reinterpret_cast<f32x2*>(&strip[(RPI + row0) * CW + 2 * cp]) = sum_b;
   __syncthreads();
   for (int c = tid; c < cols; c += NT) {
     float a = 0.f, e = 0.f;

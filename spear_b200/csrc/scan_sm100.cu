@@ -49,12 +49,18 @@ Split split_backward(long long batch, int L, int dim, int N, int sms) {
   double best_cost = static_cast<double>((ctas + slots - 1) / slots) * 2.6 * best.chunk;
   for (int s = 2; s <= 256; s = s * 3 / 2 + (s == 2)) {
     const int chunk = ((L + s - 1) / s + 31) / 32 * 32;
+#ifdef BS
+    if (s != BS) continue;
+#endif
     if (chunk < 64) break;
     const int n = (L + chunk - 1) / chunk;
     if (n < 2) continue;
     const double main = static_cast<double>((ctas * n + slots - 1) / slots) * 2.6 * (chunk + 16);
     const double carry = static_cast<double>((warps * (n - 1) + wslots - 1) / wslots) * (chunk + 24);
     const double cost = main + carry + n * 4.0;
+#ifdef BS
+    best_cost = 1e30;
+#endif
     if (cost < best_cost) {
       best_cost = cost;
       best = Split{n, chunk};
