@@ -14,22 +14,29 @@ from .. import _lib
 TAG = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16, torch.float32: _lib.DTYPE_F32}
 
 
+_current_device, _raw_stream = _native._current_device, _native._raw_stream
+_fns: dict = {}  # the library's functions by name, looked up once
+
+
+def _entry(name: str):
+    _fns[name] = fn = getattr(_lib.load(), name)
+    return fn
+
+
 def activation(t: torch.Tensor, what: str) -> None:
     if t.dtype not in TAG:
         raise RuntimeError(f"{what} must be bfloat16, float16 or float32 (got {t.dtype})")
 
 
-def on_gpu(what: str, *tensors) -> int:
+def on_gpu(what: str, first: torch.Tensor, *others) -> int:
     """All tensors (None is skipped) on one CUDA device; returns its index."""
-    index = -1
-    for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise RuntimeError(f"{what} needs CUDA tensors: this package has no CPU path and no fallback")
-        if index < 0:
-            index = t.device.index
-        elif t.device.index != index:
+    index = first.get_device()
+    if index < 0:
+        raise RuntimeError(f"{what} needs CUDA tensors: this package has no CPU path and no fallback")
+    for t in others:
+        if t is not None and t.get_device() != index:
+            if t.get_device() < 0:
+                raise RuntimeError(f"{what} needs CUDA tensors: this package has no CPU path and no fallback")
             raise RuntimeError(f"{what}: all tensors must be on one device (got cuda:{index} and {t.device})")
     return index
 
@@ -40,9 +47,9 @@ def ptr(t: torch.Tensor | None):
 
 def call(name: str, index: int, *args) -> None:
     """Enqueues a launch on the current stream of device `index`; the stream is the entry's last argument."""
-    fn = getattr(_lib._lib or _lib.load(), name)
-    if index == _native._current_device():
-        rc = fn(*args, _native._raw_stream(index))
+    fn = _fns.get(name) or _entry(name)
+    if index == _current_device():
+        rc = fn(*args, _raw_stream(index))
     else:
         with _native._OnDevice(index) as stream:
             rc = fn(*args, stream)
@@ -52,8 +59,8 @@ def call(name: str, index: int, *args) -> None:
 
 def query(name: str, index: int, *args) -> int:
     """A size that depends on the device's launch shape."""
-    fn = getattr(_lib._lib or _lib.load(), name)
-    if index == _native._current_device():
+    fn = _fns.get(name) or _entry(name)
+    if index == _current_device():
         n = fn(*args)
     else:
         with _native._OnDevice(index):

@@ -29,7 +29,7 @@ def _check(what, x, weight, residual, eps) -> int:
         raise ValueError(f"{what}: x must be [..., D] with 1 <= D <= {MAX_DIM}, got {tuple(x.shape)}")
     _call.activation(x, f"{what}: x")
     if weight is not None:
-        if tuple(weight.shape) != (x.shape[-1],):
+        if weight.shape != x.shape[-1:]:
             raise ValueError(f"{what}: weight must be [{x.shape[-1]}], got {tuple(weight.shape)}")
         if weight.dtype != x.dtype and weight.dtype != torch.float32:
             raise RuntimeError(f"{what}: weight must have x's dtype ({x.dtype}) or be float32 (got {weight.dtype})")
@@ -46,6 +46,8 @@ def _check(what, x, weight, residual, eps) -> int:
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """t as [rows, D] with dense rows at one pitch; copied only where its strides allow no such view."""
     d = t.shape[-1]
+    if t.dim() == 2 and t.is_contiguous():
+        return t
     r = t.reshape(-1, d)
     if (d > 1 and r.stride(1) != 1) or (r.shape[0] > 1 and r.stride(0) < d):
         r = r.contiguous()
@@ -60,7 +62,7 @@ def _launch_forward(x, residual, weight, y, h, rstd, scale, eps, mode) -> None:
     rows, dim = x.shape
     if rows == 0:
         return
-    _call.call("btp_sm100_rms_norm_forward", x.device.index, x.data_ptr(), _call.ptr(residual), _call.ptr(weight), y.data_ptr(),
+    _call.call("btp_sm100_rms_norm_forward", x.get_device(), x.data_ptr(), _call.ptr(residual), _call.ptr(weight), y.data_ptr(),
                _call.ptr(h), _call.ptr(rstd), _call.ptr(scale), rows, dim, _pitch(x), dim if residual is None else _pitch(residual),
                eps, _call.TAG[x.dtype], 0 if residual is None else _call.TAG[residual.dtype],
                0 if weight is None else _call.TAG[weight.dtype], mode)
@@ -151,18 +153,16 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, residual: torc
     if torch.compiler.is_compiling() or (torch.is_grad_enabled() and any(
             t is not None and t.requires_grad for t in (x, weight, residual))):
         return _RMSNorm.apply(x, weight, residual, float(eps))
-    d = x.shape[-1]
     x2 = _rows(x)
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     if residual is None:
-        _launch_forward(x2, None, weight, y.view(-1, d), None, None, None, float(eps), 0)
+        _launch_forward(x2, None, weight, y, None, None, None, float(eps), 0)
         return y
-    h = torch.empty(x.shape, device=x.device, dtype=residual.dtype)
-    _launch_forward(x2, _rows(residual), weight, y.view(-1, d), h.view(-1, d), None, None, float(eps), 0)
+    h = torch.empty_like(residual, memory_format=torch.contiguous_format)
+    _launch_forward(x2, _rows(residual), weight, y, h, None, None, float(eps), 0)
     return y, h
 
 
-@torch.no_grad()
 def rms_norm_8bit(x: torch.Tensor, weight: torch.Tensor | None = None, residual: torch.Tensor | None = None, *,
                   eps: float = 1e-6, block: int | None = None):
     """rms_norm whose output is e4m3 with float32 scales, the operand of an 8-bit product.  No gradient.
@@ -179,11 +179,9 @@ def rms_norm_8bit(x: torch.Tensor, weight: torch.Tensor | None = None, residual:
         raise ValueError(f"rms_norm_8bit: block must be None or {SCALE_BLOCK} (got {block})")
     _check("rms_norm_8bit", x, weight, residual, eps)
     weight = weight if weight is None or weight.is_contiguous() else weight.contiguous()
-    d = x.shape[-1]
-    x2 = _rows(x)
-    q = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn)
-    scale = torch.empty(x.shape[:-1] if block is None else (*x.shape[:-1], -(-d // SCALE_BLOCK)), device=x.device, dtype=torch.float32)
-    h = None if residual is None else torch.empty(x.shape, device=x.device, dtype=residual.dtype)
-    _launch_forward(x2, None if residual is None else _rows(residual), weight, q.view(-1, d), None if h is None else h.view(-1, d),
-                    None, scale, float(eps), _OUT[block])
+    x2 = _rows(x)  # no output below is computed from a tensor that autograd follows
+    q = torch.empty_like(x, dtype=torch.float8_e4m3fn, memory_format=torch.contiguous_format)
+    scale = torch.empty(x.shape[:-1] if block is None else (*x.shape[:-1], -(-x.shape[-1] // SCALE_BLOCK)), device=x.device, dtype=torch.float32)
+    h = None if residual is None else torch.empty_like(residual, memory_format=torch.contiguous_format)
+    _launch_forward(x2, None if residual is None else _rows(residual), weight, q, h, None, scale, float(eps), _OUT[block])
     return (q, scale) if h is None else (q, scale, h)

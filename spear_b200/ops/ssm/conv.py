@@ -22,18 +22,19 @@ WIDTHS = (2, 3, 4)
 
 
 def _check_filter(what, dim, dtype, weight, bias, activation) -> int:
-    if weight.dim() != 2 or weight.shape[0] != dim or weight.shape[1] not in WIDTHS:
+    shape = weight.shape
+    if len(shape) != 2 or shape[0] != dim or shape[1] not in WIDTHS:
         raise ValueError(f"{what}: weight must be [{dim}, W] with W in {WIDTHS}, got {tuple(weight.shape)}")
     if weight.dtype != dtype and weight.dtype != torch.float32:
         raise RuntimeError(f"{what}: weight must have x's dtype ({dtype}) or be float32 (got {weight.dtype})")
     if bias is not None:
-        if tuple(bias.shape) != (dim,):
+        if bias.shape != (dim,):
             raise ValueError(f"{what}: bias must be [{dim}], got {tuple(bias.shape)}")
         if bias.dtype != weight.dtype:
             raise RuntimeError(f"{what}: bias must have the weight's dtype ({weight.dtype}), got {bias.dtype}")
     if activation not in (None, "silu"):
         raise ValueError(f"{what}: activation must be None or 'silu' (got {activation!r})")
-    return weight.shape[1]
+    return shape[1]
 
 
 def check_lengths(what, lengths, batch) -> None:
@@ -48,7 +49,17 @@ def dense(t: torch.Tensor | None) -> torch.Tensor | None:
 
 
 def dense_last(t: torch.Tensor | None) -> torch.Tensor | None:
-    return t if t is None or t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+    return t if t is None or t.is_contiguous() or t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def row(t: torch.Tensor | None):
+    """[B, D] with dense rows, and its pitch."""
+    if t is None:
+        return None, 0
+    if t.is_contiguous():
+        return t, t.shape[1]
+    t = dense_last(t)
+    return t, t.stride(0)
 
 
 def strides(t: torch.Tensor) -> tuple[int, int]:
@@ -172,7 +183,7 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None
 def check_state_out(what, state, state_out) -> torch.Tensor:
     """Where the new state goes: fresh memory, or the caller's tensor, which may be the old state itself."""
     if state_out is None:
-        return torch.empty(state.shape, device=state.device, dtype=state.dtype)
+        return torch.empty_like(state, memory_format=torch.contiguous_format)
     if state_out is state:
         return state_out
     if state_out.shape != state.shape or state_out.dtype != state.dtype or state_out.device != state.device or not state_out.is_contiguous():
@@ -183,7 +194,6 @@ def check_state_out(what, state, state_out) -> torch.Tensor:
     return state_out
 
 
-@torch.no_grad()
 def causal_conv_step(x_t: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
                      activation: str | None = None, state_out: torch.Tensor | None = None):
     """One token of ``causal_conv``: returns (y_t [B, D], new state [B, W-1, D]).
@@ -197,15 +207,15 @@ def causal_conv_step(x_t: torch.Tensor, state: torch.Tensor, weight: torch.Tenso
     B, D = x_t.shape
     _call.activation(x_t, f"{what}: x_t")
     W = _check_filter(what, D, x_t.dtype, weight, bias, activation)
-    if tuple(state.shape) != (B, W - 1, D) or state.dtype != x_t.dtype or not state.is_contiguous():
+    if state.shape != (B, W - 1, D) or state.dtype != x_t.dtype or not state.is_contiguous():
         raise ValueError(f"{what}: state must be contiguous {(B, W - 1, D)} of x_t's dtype, got {state.dtype} {tuple(state.shape)}")
     index = _call.on_gpu(what, x_t, state, weight, bias)
     out = check_state_out(what, state, state_out)
-    y = torch.empty(B, D, device=x_t.device, dtype=x_t.dtype)
+    y = torch.empty_like(x_t, memory_format=torch.contiguous_format)
     if B == 0:
         return y, out
-    x_t, weight, bias = dense_last(x_t), dense(weight), dense(bias)
+    (x_t, pitch), weight, bias = row(x_t), dense(weight), dense(bias)
     _call.call("btp_sm100_causal_conv_step", index, x_t.data_ptr(), state.data_ptr(), weight.data_ptr(), _call.ptr(bias), y.data_ptr(),
-               out.data_ptr(), B, D, W, x_t.stride(0) if B > 1 else D, int(activation is not None), _call.TAG[x_t.dtype],
+               out.data_ptr(), B, D, W, pitch, int(activation is not None), _call.TAG[x_t.dtype],
                _call.TAG[weight.dtype])
     return y, out

@@ -17,7 +17,7 @@ from torch.autograd.function import once_differentiable
 
 from ..btp import interface as _iface
 from .. import _call
-from .conv import check_lengths, check_state_out, dense, dense_last, strides
+from .conv import check_lengths, check_state_out, dense, dense_last, row, strides
 
 __all__ = ["selective_scan", "selective_scan_step", "MAX_STATES"]
 
@@ -31,26 +31,30 @@ def _aligned(t: torch.Tensor | None) -> torch.Tensor | None:
 
 
 def _check_params(what, dim, A, D, delta_bias) -> int:
-    if A.dim() != 2 or A.shape[0] != dim or not 1 <= A.shape[1] <= MAX_STATES:
-        raise ValueError(f"{what}: A must be [{dim}, N] with 1 <= N <= {MAX_STATES}, got {tuple(A.shape)}")
-    for t, name in ((A, "A"), (D, "D"), (delta_bias, "delta_bias")):
+    shape = A.shape
+    if len(shape) != 2 or shape[0] != dim or not 1 <= shape[1] <= MAX_STATES:
+        raise ValueError(f"{what}: A must be [{dim}, N] with 1 <= N <= {MAX_STATES}, got {tuple(shape)}")
+    if A.dtype != torch.float32:
+        raise RuntimeError(f"{what}: A must be float32 (got {A.dtype})")
+    for t, name in ((D, "D"), (delta_bias, "delta_bias")):
         if t is None:
             continue
-        if name != "A" and tuple(t.shape) != (dim,):
+        if t.shape != (dim,):
             raise ValueError(f"{what}: {name} must be [{dim}], got {tuple(t.shape)}")
         if t.dtype != torch.float32:
             raise RuntimeError(f"{what}: {name} must be float32 (got {t.dtype})")
-    return A.shape[1]
+    return shape[1]
 
 
 def _check_tokens(what, x, others) -> None:
+    dtype = x.dtype
     for t, name, shape in others:
         if t is None:
             continue
-        if tuple(t.shape) != shape:
-            raise ValueError(f"{what}: {name} must be {shape}, got {tuple(t.shape)}")
-        if t.dtype != x.dtype:
-            raise RuntimeError(f"{what}: {name} must have x's dtype ({x.dtype}), got {t.dtype}")
+        if t.shape != shape:
+            raise ValueError(f"{what}: {name} must be {tuple(shape)}, got {tuple(t.shape)}")
+        if t.dtype != dtype:
+            raise RuntimeError(f"{what}: {name} must have x's dtype ({dtype}), got {t.dtype}")
 
 
 def _shape_args(x, delta, A, B, C, z):
@@ -189,7 +193,6 @@ def selective_scan(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: tor
     return (y, state) if return_state else y
 
 
-@torch.no_grad()
 def selective_scan_step(x_t: torch.Tensor, delta_t: torch.Tensor, A: torch.Tensor, B_t: torch.Tensor, C_t: torch.Tensor,
                         state: torch.Tensor, D: torch.Tensor | None = None, z_t: torch.Tensor | None = None, *,
                         delta_bias: torch.Tensor | None = None, delta_softplus: bool = False, state_out: torch.Tensor | None = None):
@@ -205,20 +208,20 @@ def selective_scan_step(x_t: torch.Tensor, delta_t: torch.Tensor, A: torch.Tenso
     Bsz, dim = x_t.shape
     _call.activation(x_t, f"{what}: x_t")
     N = _check_params(what, dim, A, D, delta_bias)
-    _check_tokens(what, x_t, ((delta_t, "delta_t", (Bsz, dim)), (z_t, "z_t", (Bsz, dim)), (B_t, "B_t", (Bsz, N)), (C_t, "C_t", (Bsz, N))))
-    if tuple(state.shape) != (Bsz, dim, N) or state.dtype != torch.float32 or not state.is_contiguous():
+    _check_tokens(what, x_t, ((delta_t, "delta_t", x_t.shape), (z_t, "z_t", x_t.shape), (B_t, "B_t", (Bsz, N)), (C_t, "C_t", (Bsz, N))))
+    if state.shape != (Bsz, dim, N) or state.dtype != torch.float32 or not state.is_contiguous():
         raise ValueError(f"{what}: state must be contiguous float32 {(Bsz, dim, N)}, got {state.dtype} {tuple(state.shape)}")
     index = _call.on_gpu(what, x_t, delta_t, A, B_t, C_t, state, D, z_t, delta_bias)
     out = check_state_out(what, state, state_out)
-    y = torch.empty(Bsz, dim, device=x_t.device, dtype=x_t.dtype)
+    y = torch.empty_like(x_t, memory_format=torch.contiguous_format)
     if Bsz == 0:
         return y, out
     if (state.data_ptr() | out.data_ptr()) % 16:
         raise ValueError(f"{what}: state and state_out must be 16-byte aligned")
-    x_t, delta_t, B_t, C_t, z_t = dense_last(x_t), dense_last(delta_t), dense_last(B_t), dense_last(C_t), dense_last(z_t)
+    (x_t, px), (delta_t, pd), (B_t, pB), (C_t, pC), (z_t, pz) = row(x_t), row(delta_t), row(B_t), row(C_t), row(z_t)
     A, D, delta_bias = _aligned(dense(A)), dense(D), dense(delta_bias)
     p = _call.ptr
     _call.call("btp_sm100_scan_step", index, x_t.data_ptr(), delta_t.data_ptr(), A.data_ptr(), B_t.data_ptr(), C_t.data_ptr(), p(D),
-               p(z_t), p(delta_bias), state.data_ptr(), y.data_ptr(), out.data_ptr(), Bsz, dim, N, x_t.stride(0), delta_t.stride(0),
-               B_t.stride(0), C_t.stride(0), 0 if z_t is None else z_t.stride(0), int(bool(delta_softplus)), _call.TAG[x_t.dtype])
+               p(z_t), p(delta_bias), state.data_ptr(), y.data_ptr(), out.data_ptr(), Bsz, dim, N, px, pd, pB, pC, pz,
+               1 if delta_softplus else 0, _call.TAG[x_t.dtype])
     return y, out
