@@ -2,13 +2,17 @@
 
     from spear_b200.ops.btp import btp          # same signature as spear.ops.btp.btp
     from spear_b200.nn.phalanx import Phalanx   # same constructor / state_dict as spear.nn.phalanx.Phalanx
+    from spear_b200.ops.ssm import causal_conv, selective_scan    # selective state space operators, and their token forms
+    from spear_b200.ops.norm import rms_norm, rms_norm_8bit       # norm with the residual's addition
+    from spear_b200.nn.ssm import SelectiveSSM                    # the layer of these operators
+    from spear_b200.nn.block import MixerBlock                    # pre-norm residual block around either layer
 
 The native library is loaded on first use; there is no CPU or PyTorch fallback.
 """
 
 __version__ = "0.1.0"
 
-__all__ = ["btp", "Phalanx", "SigmoidA", "install_as_spear_backend"]
+__all__ = ["btp", "Phalanx", "SigmoidA", "SelectiveSSM", "MixerBlock", "install_as_spear_backend"]
 
 
 def install_as_spear_backend():
@@ -38,4 +42,12 @@ def __getattr__(name):  # lazy: importing the package must not require torch ops
         from .nn import phalanx
 
         return getattr(phalanx, name)
+    if name == "SelectiveSSM":
+        from .nn.ssm import SelectiveSSM
+
+        return SelectiveSSM
+    if name == "MixerBlock":
+        from .nn.block import MixerBlock
+
+        return MixerBlock
     raise AttributeError(name)

@@ -68,3 +68,18 @@ def query(name: str, index: int, *args) -> int:
     if n < 0:
         _lib.check(int(n), name)
     return int(n)
+
+
+def traceable(name: str, direct):
+    """The registered op `spear_btp::name` while torch.compile traces, the function behind it otherwise (the dispatcher takes
+    longer than a small launch)."""
+    op = getattr(torch.ops.spear_btp, name)
+    compiling = torch.compiler.is_compiling
+
+    def run(*args):
+        if compiling():
+            op(*args)
+        else:
+            direct(*args)
+
+    return run

@@ -96,6 +96,8 @@ def _fake(*args) -> None:
 
 _iface._register(_iface._LIB, "spear_btp", "rms_norm_forward", _op_forward, _fake, ["y", "h", "rstd"])
 _iface._register(_iface._LIB, "spear_btp", "rms_norm_backward", _op_backward, _fake, ["dx", "dresidual", "dweight"])
+_forward = _call.traceable("rms_norm_forward", _op_forward)
+_backward = _call.traceable("rms_norm_backward", _op_backward)
 
 
 class _RMSNorm(torch.autograd.Function):
@@ -107,7 +109,7 @@ class _RMSNorm(torch.autograd.Function):
         h = None if residual is None else torch.empty(x.shape, device=x.device, dtype=residual.dtype)
         rstd = torch.empty(x2.shape[0], device=x.device, dtype=torch.float32)
         d = x.shape[-1]
-        torch.ops.spear_btp.rms_norm_forward(x2, r2, weight, y.view(-1, d), None if h is None else h.view(-1, d), rstd, eps)
+        _forward(x2, r2, weight, y.view(-1, d), None if h is None else h.view(-1, d), rstd, eps)
         ctx.save_for_backward(x2 if h is None else h, weight, rstd)
         ctx.has_residual = h is not None
         ctx.dtype = x.dtype
@@ -131,7 +133,7 @@ class _RMSNorm(torch.autograd.Function):
         dres = torch.empty(shape, device=dy.device, dtype=h.dtype) if need_r and not one else None
         dw = torch.empty_like(weight, memory_format=torch.contiguous_format) if need_w and weight is not None else None
         if dx is not None or dres is not None or dw is not None:
-            torch.ops.spear_btp.rms_norm_backward(h2, weight, dy2, dh2, rstd, None if dx is None else dx.view(-1, d),
+            _backward(h2, weight, dy2, dh2, rstd, None if dx is None else dx.view(-1, d),
                                                   None if dres is None else dres.view(-1, d), dw)
         return dx if need_x else None, dw, (dx if one else dres) if need_r else None, None
 

@@ -103,6 +103,8 @@ def _fake(*args) -> None:
 
 _iface._register(_iface._LIB, "spear_btp", "causal_conv_forward", _op_forward, _fake, ["y", "state"])
 _iface._register(_iface._LIB, "spear_btp", "causal_conv_backward", _op_backward, _fake, ["dx", "dweight", "dbias", "dinitial"])
+_forward = _call.traceable("causal_conv_forward", _op_forward)
+_backward = _call.traceable("causal_conv_backward", _op_backward)
 
 
 class _CausalConv(torch.autograd.Function):
@@ -111,7 +113,7 @@ class _CausalConv(torch.autograd.Function):
         B, L, D = x.shape
         y = torch.empty(B, L, D, device=x.device, dtype=x.dtype)
         state = torch.empty(B, weight.shape[1] - 1, D, device=x.device, dtype=x.dtype) if want_state else None
-        torch.ops.spear_btp.causal_conv_forward(x, weight, bias, initial, lengths, y, state, silu)
+        _forward(x, weight, bias, initial, lengths, y, state, silu)
         ctx.save_for_backward(x, weight, bias, initial, lengths)
         ctx.silu = silu
         ctx.set_materialize_grads(False)
@@ -130,7 +132,7 @@ class _CausalConv(torch.autograd.Function):
         dw = torch.empty(weight.shape, device=x.device, dtype=weight.dtype) if need_w else None
         db = torch.empty(bias.shape, device=x.device, dtype=bias.dtype) if need_b and bias is not None else None
         di = torch.empty(initial.shape, device=x.device, dtype=x.dtype) if need_i and initial is not None else None
-        torch.ops.spear_btp.causal_conv_backward(x, weight, bias, initial, lengths, dy, dstate, dx, dw, db, di, ctx.silu)
+        _backward(x, weight, bias, initial, lengths, dy, dstate, dx, dw, db, di, ctx.silu)
         return dx if need_x else None, dw, db, di, None, None, None
 
 

@@ -103,6 +103,8 @@ def _fake(*args) -> None:
 
 _iface._register(_iface._LIB, "spear_btp", "scan_forward", _op_forward, _fake, ["y", "state", "checkpoints"])
 _iface._register(_iface._LIB, "spear_btp", "scan_backward", _op_backward, _fake, ["dx", "ddelta", "dparams", "dB", "dC", "dz", "dinitial"])
+_forward = _call.traceable("scan_forward", _op_forward)
+_backward = _call.traceable("scan_backward", _op_backward)
 
 
 class _SelectiveScan(torch.autograd.Function):
@@ -113,7 +115,7 @@ class _SelectiveScan(torch.autograd.Function):
         y = torch.empty(Bsz, L, dim, device=x.device, dtype=x.dtype)
         state = torch.empty(Bsz, dim, N, device=x.device, dtype=torch.float32) if want_state else None
         checkpoints = torch.empty(Bsz, -(-L // _CHECKPOINT), dim, N, device=x.device, dtype=torch.float32)
-        torch.ops.spear_btp.scan_forward(x, delta, A, B, C, D, z, delta_bias, initial, lengths, y, state, checkpoints, softplus)
+        _forward(x, delta, A, B, C, D, z, delta_bias, initial, lengths, y, state, checkpoints, softplus)
         ctx.save_for_backward(x, delta, A, B, C, D, z, delta_bias, lengths, checkpoints)
         ctx.softplus = softplus
         ctx.set_materialize_grads(False)
@@ -136,7 +138,7 @@ class _SelectiveScan(torch.autograd.Function):
         dB, dC = (torch.empty(B.shape, device=dev, dtype=dtype) for _ in range(2))
         dparams = torch.empty(-(-dim * (N + 2) // 4) * 4, device=dev, dtype=torch.float32)
         dinitial = torch.empty(Bsz, dim, N, device=dev, dtype=torch.float32) if need[8] else None
-        torch.ops.spear_btp.scan_backward(x, delta, A, B, C, D, z, delta_bias, lengths, checkpoints, dy, dstate, dx, ddelta, dparams,
+        _backward(x, delta, A, B, C, D, z, delta_bias, lengths, checkpoints, dy, dstate, dx, ddelta, dparams,
                                           dB, dC, dz, dinitial, ctx.softplus)
         dA, dD, dbias = dparams[:dim * N].view(dim, N), dparams[dim * N:dim * (N + 1)], dparams[dim * (N + 1):dim * (N + 2)]
         grads = (dx, ddelta, dA, dB, dC, None if D is None else dD, dz, None if delta_bias is None else dbias, dinitial)
