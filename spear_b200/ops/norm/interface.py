@@ -104,14 +104,11 @@ class _RMSNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
         x2 = _rows(x)
-        r2 = None if residual is None else _rows(residual)
-        y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-        h = None if residual is None else torch.empty(x.shape, device=x.device, dtype=residual.dtype)
+        y = torch.empty_like(x, memory_format=torch.contiguous_format)
+        h = None if residual is None else torch.empty_like(residual, memory_format=torch.contiguous_format)
         rstd = torch.empty(x2.shape[0], device=x.device, dtype=torch.float32)
-        d = x.shape[-1]
-        _forward(x2, r2, weight, y.view(-1, d), None if h is None else h.view(-1, d), rstd, eps)
+        _forward(x2, None if residual is None else _rows(residual), weight, y, h, rstd, eps)
         ctx.save_for_backward(x2 if h is None else h, weight, rstd)
-        ctx.has_residual = h is not None
         ctx.dtype = x.dtype
         ctx.set_materialize_grads(False)
         return y if h is None else (y, h)
@@ -124,17 +121,14 @@ class _RMSNorm(torch.autograd.Function):
         if dy is None:  # y was not used: the sum passes its gradient on
             dx = dh.to(ctx.dtype) if dh is not None and need_x else None
             return dx, None, dh if need_r else None, None
-        shape, d = dy.shape, dy.shape[-1]
-        dy2 = dy.reshape(-1, d).contiguous()
-        h2 = _rows(h)
-        dh2 = None if dh is None else dh.reshape(-1, d).contiguous()
+        dy = dy.contiguous()
+        dh = None if dh is None else dh.contiguous()
         one = h.dtype == ctx.dtype  # one tensor serves as the gradient of both terms of the sum
-        dx = torch.empty(shape, device=dy.device, dtype=ctx.dtype) if need_x or (one and need_r) else None
-        dres = torch.empty(shape, device=dy.device, dtype=h.dtype) if need_r and not one else None
-        dw = torch.empty_like(weight, memory_format=torch.contiguous_format) if need_w and weight is not None else None
+        dx = torch.empty_like(dy) if need_x or (one and need_r) else None
+        dres = torch.empty_like(dy, dtype=h.dtype) if need_r and not one else None
+        dw = torch.empty_like(weight) if need_w and weight is not None else None
         if dx is not None or dres is not None or dw is not None:
-            _backward(h2, weight, dy2, dh2, rstd, None if dx is None else dx.view(-1, d),
-                                                  None if dres is None else dres.view(-1, d), dw)
+            _backward(_rows(h), weight, dy, dh, rstd, dx, dres, dw)
         return dx if need_x else None, dw, (dx if one else dres) if need_r else None, None
 
 
