@@ -49,7 +49,6 @@ constexpr int kCols = 2 * kThreads;        // channels of a CTA
 constexpr int kTile = 16;                  // tokens per tile
 constexpr int kStages = 3;                 // tiles in the ring
 
-
 // 2 PAIRS channels of row `t` of xx (t may be negative: the initial state).
 template <class T, int PAIRS, int W>
 __device__ __forceinline__ void load_xx(f32x2 (&out)[PAIRS], const ConvParams& p, const T* x, long long b, int t, int d) {

@@ -13,7 +13,9 @@
 // lanes of a state group by exchanging halves (7 exchanges for 8 sums), the warps in shared memory.  Sums over the CTAs' channels
 // and over sequences go through a buffer and a second kernel in a fixed order: the same call gives the same bits.
 //
-// Bound: the two-wide multiply-adds (about 13 per token, channel and state) and two exponentials.
+// Bound: the two-wide multiply-adds (about 13 per token, channel and state) and two exponentials.  Measured at 8 x 2048 tokens x 2048
+// channels x 16 states, bfloat16: 800 us, and 180 us for the carries of its 16 chunks; 385 instructions per token and warp at 0.44 per
+// cycle with the two warps that registers (255) and shared memory leave a scheduler.
 #pragma once
 
 #include "scan_kernels.cuh"

@@ -12,7 +12,10 @@
 // Measured against lanes of 4 channels x 4 states with step sizes and y staged in shared memory (8 x 2048 tokens x 2048
 // channels x 16 states): 298 us against 520; 2 channels x 8 states 372 (half the warps), 2 x 2 states 343 (more exchanges).
 //
-// Bound: one exponential per (token, channel, state) on the special-function unit, 16 per clock and SM.
+// Bound: one exponential per (token, channel, state) on the special-function unit, 16 per clock and SM: 119 us for those 5.4e8.  At
+// that shape a scheduler has two warps and issues half of the time; with the tokens split 16 times (many warps) the same kernel
+// takes 212 us, two thirds of the special-function unit's rate.  Taking a share of the exponentials by a polynomial on the multiply-add
+// pipe was slower (the instructions it adds count more).
 //
 // Few channels or sequences: the tokens are split over `splits` chunks.  A first kernel runs each chunk from state zero and
 // keeps its last state and its sum of step sizes (the product of its decays is exp(A times that sum), one exponential); the second
@@ -50,9 +53,10 @@ struct ScanParams {
   int batch, L, dim, N;
   int splits, chunk;      // chunk: tokens per split, a multiple of 32
   bool softplus;
-  bool al_x, al_d, al_z, al_B, al_C, al_y;  // 16-byte copies (y: pairs) are possible
+  bool al_x, al_d, al_z, al_B, al_C;  // 16-byte copies are possible
 };
 
+// A tile of the backward's carries: lanes of 4 channels x 4 states, step sizes and inputs in float, C given twice.
 template <class T, int SG>
 struct Tile {
   static constexpr int kStates = 4 * SG;
@@ -493,6 +497,7 @@ __global__ void __launch_bounds__(128, 7) scan_step_kernel(const ScanStepParams 
   constexpr int kOwn = SG >= 4 ? 1 : 4 / SG;
   grid_dependency_wait();
   const int in = static_cast<int>(blockIdx.x % p.ctas) * 128 + threadIdx.x;
+  if ((in & ~31) / SG >= p.dim) return;  // a warp without a channel: it must not even read, another may be writing in place
   const int lane = threadIdx.x & 31, d = in / SG, s = in % SG, n0 = 4 * s;
   const bool ok = d < p.dim;
   const int dd = ok ? d : p.dim - 1;  // lanes without a channel follow the last one: the exchanges below need whole warps

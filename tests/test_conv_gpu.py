@@ -295,3 +295,6 @@ def test_compiled_and_repeatable():
         y = causal_conv(*leaves, activation="silu")
         runs.append(torch.autograd.grad(y, leaves, torch.ones_like(y)))
     assert all(torch.equal(a, b) for a, b in zip(*runs))
+    leaves = [v[n].clone().requires_grad_(True) for n in ("x", "weight", "bias")]
+    y = torch.compile(causal_conv, backend="aot_eager")(*leaves, activation="silu")
+    assert all(torch.equal(a, b) for a, b in zip(runs[0], torch.autograd.grad(y, leaves, torch.ones_like(y))))

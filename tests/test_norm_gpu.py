@@ -282,3 +282,10 @@ def test_compiled():
     x, w, r = inputs((9, 320), torch.bfloat16, torch.float32, torch.bfloat16, seed=8)
     f = torch.compile(lambda a, b, c: rms_norm(a, b, c), backend="eager", fullgraph=True)
     assert all(torch.equal(a, b) for a, b in zip(f(x, w, r), rms_norm(x, w, r)))
+
+    dy, dh = torch.randn_like(x), torch.randn_like(r)
+    out = []
+    for fn in (rms_norm, torch.compile(rms_norm, backend="aot_eager")):
+        leaves = [t.clone().requires_grad_(True) for t in (x, w, r)]
+        out.append(torch.autograd.grad(list(fn(*leaves)), leaves, [dy, dh]))
+    assert all(torch.equal(a, b) for a, b in zip(*out))

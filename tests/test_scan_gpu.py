@@ -58,7 +58,7 @@ def check(got, want, dtype, name):
 # lengths around the tile of 16 and the step of 4, one token, long enough to be split; channel counts and states that fill no warp
 SHAPES = [(1, 1, 1, 1), (1, 1, 32, 16), (2, 2, 8, 4), (1, 3, 33, 16), (2, 15, 40, 16), (3, 16, 64, 8), (2, 17, 130, 16), (1, 31, 24, 32),
           (2, 33, 20, 64), (1, 64, 7, 3), (2, 65, 12, 13), (1, 100, 36, 17), (2, 40, 19, 33), (1, 50, 9, 61), (3, 300, 16, 16), (1, 777, 40, 16),
-          (2, 1000, 6, 8), (1, 520, 10, 64), (1, 640, 66, 32)]
+          (2, 1000, 6, 8), (1, 520, 10, 64), (1, 640, 66, 32), (2, 37, 24, 64), (1, 50, 48, 20), (2, 20, 136, 7)]
 VARIANTS = [dict(), dict(skip=False, gate=False, bias=False), dict(initial=True, gate=False), dict(lengths=True, initial=True)]
 
 
@@ -367,3 +367,15 @@ def test_more_than_2_31_elements():
     y = selective_scan(x, d, A, B, C)
     small = selective_scan(x[..., -40:].contiguous(), d[..., -40:].contiguous(), A[-40:].clone(), B, C)
     assert torch.equal(y[..., -40:], small) and (y[..., :40] == 0).all()
+
+
+def test_compiled_training_step():
+    v = inputs(2, 70, 40, 16, torch.bfloat16, seed=15)
+    names = [n for n in NAMES if v[n] is not None]
+    dy = torch.randn(2, 70, 40, device="cuda").bfloat16()
+    out = []
+    for fn in (run, torch.compile(run, backend="aot_eager")):
+        leaves = {n: v[n].clone().requires_grad_(True) for n in names}
+        y = fn({**v, **leaves}, state=False)
+        out.append([y.detach(), *torch.autograd.grad(y, list(leaves.values()), dy)])
+    assert all(torch.equal(a, b) for a, b in zip(*out))
