@@ -70,14 +70,41 @@ def query(name: str, index: int, *args) -> int:
     return int(n)
 
 
+def dense(t: torch.Tensor | None) -> torch.Tensor | None:
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+def dense_last(t: torch.Tensor | None) -> torch.Tensor | None:
+    return t if t is None or t.is_contiguous() or t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def buffers(what: str, index: int, *wanted) -> None:
+    """Refuses buffers of a registered op, each (tensor or None, name, elements, dtype), that a launch would reach past."""
+    for t, name, n, dtype in wanted:
+        if t is not None and (t.numel() != n or t.dtype != dtype or not t.is_contiguous() or t.get_device() != index):
+            raise ValueError(f"{what}: {name} must hold {n} contiguous {dtype} on cuda:{index}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def pass_on(into: torch.Tensor | None, given: torch.Tensor | None) -> None:
+    """No tokens: a state (or its gradient) goes through as it came, zeros where none came."""
+    if into is not None:
+        into.zero_() if given is None else into.copy_(given)
+
+
+_modes, _tracing = torch._C._len_torch_dispatch_stack, torch._C._get_tracing_state
+_DIRECT = frozenset((torch.Tensor, torch.nn.Parameter, type(None), bool, int, float))
+
+
 def traceable(name: str, direct):
-    """The registered op `spear_btp::name` while torch.compile traces, the function behind it otherwise (the dispatcher takes
-    longer than a small launch)."""
+    """The registered op `spear_btp::name` where somebody records or interprets the call (torch.compile, make_fx and other dispatch
+    modes, torch.jit.trace, a tensor subclass), the function `direct` otherwise (the dispatcher takes longer than a small launch).
+
+    A recorded op is replayed on tensors that no public function has looked at, so the op itself checks its arguments."""
     op = getattr(torch.ops.spear_btp, name)
     compiling = torch.compiler.is_compiling
 
     def run(*args):
-        if compiling():
+        if compiling() or _modes() or _tracing() is not None or not _DIRECT.issuperset(map(type, args)):
             op(*args)
         else:
             direct(*args)

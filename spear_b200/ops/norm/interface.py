@@ -58,23 +58,44 @@ def _pitch(r: torch.Tensor) -> int:
     return r.stride(0) if r.shape[0] > 1 else r.shape[1]
 
 
-def _launch_forward(x, residual, weight, y, h, rstd, scale, eps, mode) -> None:
+def _launch_forward(x, residual, weight, y, h, rstd, eps, scale=None, out_mode=0) -> None:
     rows, dim = x.shape
     if rows == 0:
         return
     _call.call("btp_sm100_rms_norm_forward", x.get_device(), x.data_ptr(), _call.ptr(residual), _call.ptr(weight), y.data_ptr(),
                _call.ptr(h), _call.ptr(rstd), _call.ptr(scale), rows, dim, _pitch(x), dim if residual is None else _pitch(residual),
                eps, _call.TAG[x.dtype], 0 if residual is None else _call.TAG[residual.dtype],
-               0 if weight is None else _call.TAG[weight.dtype], mode)
+               0 if weight is None else _call.TAG[weight.dtype], out_mode)
 
 
 def _op_forward(x: torch.Tensor, residual: Optional[torch.Tensor], weight: Optional[torch.Tensor], y: torch.Tensor,
-                h: Optional[torch.Tensor], rstd: torch.Tensor, eps: float) -> None:
-    _launch_forward(x, residual, weight, y, h, rstd, None, eps, 0)
+                h: Optional[torch.Tensor], rstd: Optional[torch.Tensor], eps: float, scale: Optional[torch.Tensor] = None,
+                out_mode: int = 0) -> None:
+    what = "spear_btp::rms_norm_forward"
+    index = _check(what, x, weight, residual, eps)
+    n, dim = x.numel(), x.shape[-1]
+    blocks = {0: 0, 1: 1, 2: -(-dim // SCALE_BLOCK)}.get(out_mode)
+    if blocks is None or (blocks and scale is None) or (residual is not None and h is None):
+        raise ValueError(f"{what}: out_mode must be 0, or 1 or 2 with a scale, and a residual comes with h")
+    _call.buffers(what, index, (y, "y", n, torch.float8_e4m3fn if out_mode else x.dtype), (rstd, "rstd", n // dim, torch.float32),
+                  (h, "h", n, x.dtype if residual is None else residual.dtype), (scale, "scale", n // dim * blocks, torch.float32))
+    _launch_forward(_rows(x), None if residual is None else _rows(residual), _call.dense(weight), y, h, rstd, eps, scale, out_mode)
 
 
 def _op_backward(h: torch.Tensor, weight: Optional[torch.Tensor], dy: torch.Tensor, dh: Optional[torch.Tensor], rstd: torch.Tensor,
                  dx: Optional[torch.Tensor], dresidual: Optional[torch.Tensor], dweight: Optional[torch.Tensor]) -> None:
+    what = "spear_btp::rms_norm_backward"
+    index = _check(what, _rows(dy), weight, _rows(h), 0.0)
+    n, dim = dy.numel(), dy.shape[-1]
+    if dweight is not None and weight is None:
+        raise ValueError(f"{what}: dweight needs the weight")
+    _call.buffers(what, index, (rstd, "rstd", n // dim, torch.float32), (dh, "dh", n, h.dtype), (dx, "dx", n, dy.dtype),
+                  (dresidual, "dresidual", n, h.dtype), (dweight, "dweight", dim, None if weight is None else weight.dtype))
+    _launch_backward(_rows(h), _call.dense(weight), dy.contiguous(), dh, rstd, dx, dresidual, dweight)
+
+
+def _launch_backward(h: torch.Tensor, weight: Optional[torch.Tensor], dy: torch.Tensor, dh: Optional[torch.Tensor], rstd: torch.Tensor,
+                     dx: Optional[torch.Tensor], dresidual: Optional[torch.Tensor], dweight: Optional[torch.Tensor]) -> None:
     rows, dim = h.shape
     if rows == 0:
         if dweight is not None:
@@ -94,10 +115,10 @@ def _fake(*args) -> None:
     return None
 
 
-_iface._register(_iface._LIB, "spear_btp", "rms_norm_forward", _op_forward, _fake, ["y", "h", "rstd"])
+_iface._register(_iface._LIB, "spear_btp", "rms_norm_forward", _op_forward, _fake, ["y", "h", "rstd", "scale"])
 _iface._register(_iface._LIB, "spear_btp", "rms_norm_backward", _op_backward, _fake, ["dx", "dresidual", "dweight"])
-_forward = _call.traceable("rms_norm_forward", _op_forward)
-_backward = _call.traceable("rms_norm_backward", _op_backward)
+_forward = _call.traceable("rms_norm_forward", _launch_forward)
+_backward = _call.traceable("rms_norm_backward", _launch_backward)
 
 
 class _RMSNorm(torch.autograd.Function):
@@ -106,7 +127,7 @@ class _RMSNorm(torch.autograd.Function):
         x2 = _rows(x)
         y = torch.empty_like(x, memory_format=torch.contiguous_format)
         h = None if residual is None else torch.empty_like(residual, memory_format=torch.contiguous_format)
-        rstd = torch.empty(x2.shape[0], device=x.device, dtype=torch.float32)
+        rstd = x.new_empty(x2.shape[0], dtype=torch.float32)
         _forward(x2, None if residual is None else _rows(residual), weight, y, h, rstd, eps)
         ctx.save_for_backward(x2 if h is None else h, weight, rstd)
         ctx.dtype = x.dtype
@@ -152,10 +173,10 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, residual: torc
     x2 = _rows(x)
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
     if residual is None:
-        _launch_forward(x2, None, weight, y, None, None, None, float(eps), 0)
+        _forward(x2, None, weight, y, None, None, float(eps))
         return y
     h = torch.empty_like(residual, memory_format=torch.contiguous_format)
-    _launch_forward(x2, _rows(residual), weight, y, h, None, None, float(eps), 0)
+    _forward(x2, _rows(residual), weight, y, h, None, float(eps))
     return y, h
 
 
@@ -177,7 +198,7 @@ def rms_norm_8bit(x: torch.Tensor, weight: torch.Tensor | None = None, residual:
     weight = weight if weight is None or weight.is_contiguous() else weight.contiguous()
     x2 = _rows(x)  # no output below is computed from a tensor that autograd follows
     q = torch.empty_like(x, dtype=torch.float8_e4m3fn, memory_format=torch.contiguous_format)
-    scale = torch.empty(x.shape[:-1] if block is None else (*x.shape[:-1], -(-x.shape[-1] // SCALE_BLOCK)), device=x.device, dtype=torch.float32)
+    scale = x.new_empty(x.shape[:-1] if block is None else (*x.shape[:-1], -(-x.shape[-1] // SCALE_BLOCK)), dtype=torch.float32)
     h = None if residual is None else torch.empty_like(residual, memory_format=torch.contiguous_format)
-    _launch_forward(x2, None if residual is None else _rows(residual), weight, q, h, None, scale, float(eps), _OUT[block])
+    _forward(x2, None if residual is None else _rows(residual), weight, q, h, None, float(eps), scale, _OUT[block])
     return (q, scale) if h is None else (q, scale, h)

@@ -15,6 +15,7 @@ from torch.autograd.function import once_differentiable
 
 from ..btp import interface as _iface
 from .. import _call
+from .._call import dense, dense_last
 
 __all__ = ["causal_conv", "causal_conv_step"]
 
@@ -44,12 +45,32 @@ def check_lengths(what, lengths, batch) -> None:
         raise ValueError(f"{what}: lengths must be int32 [{batch}], got {lengths.dtype} {tuple(lengths.shape)}")
 
 
-def dense(t: torch.Tensor | None) -> torch.Tensor | None:
-    return t if t is None or t.is_contiguous() else t.contiguous()
+def _check(what, x, weight, bias, activation, initial, lengths) -> tuple[int, int]:
+    """(taps, device) of a convolution over [B, L, D]."""
+    if x.dim() != 3 or x.shape[2] < 1:
+        raise ValueError(f"{what}: x must be [B, L, D], got {tuple(x.shape)}")
+    B, L, D = x.shape
+    _call.activation(x, f"{what}: x")
+    W = _check_filter(what, D, x.dtype, weight, bias, activation)
+    if initial is not None:
+        if tuple(initial.shape) != (B, W - 1, D):
+            raise ValueError(f"{what}: initial_state must be {(B, W - 1, D)}, got {tuple(initial.shape)}")
+        if initial.dtype != x.dtype:
+            raise RuntimeError(f"{what}: initial_state must have x's dtype ({x.dtype}), got {initial.dtype}")
+    check_lengths(what, lengths, B)
+    return W, _call.on_gpu(what, x, weight, bias, initial, lengths)
 
 
-def dense_last(t: torch.Tensor | None) -> torch.Tensor | None:
-    return t if t is None or t.is_contiguous() or t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+def _check_step(what, x_t, state, weight, bias, activation) -> int:
+    """The device of a single token's convolution."""
+    if x_t.dim() != 2 or x_t.shape[1] < 1:
+        raise ValueError(f"{what}: x_t must be [B, D], got {tuple(x_t.shape)}")
+    B, D = x_t.shape
+    _call.activation(x_t, f"{what}: x_t")
+    W = _check_filter(what, D, x_t.dtype, weight, bias, activation)
+    if state.shape != (B, W - 1, D) or state.dtype != x_t.dtype or not state.is_contiguous():
+        raise ValueError(f"{what}: state must be contiguous {(B, W - 1, D)} of x_t's dtype, got {state.dtype} {tuple(state.shape)}")
+    return _call.on_gpu(what, x_t, state, weight, bias)
 
 
 def row(t: torch.Tensor | None):
@@ -78,12 +99,33 @@ def _launch_forward(x, weight, bias, initial, lengths, y, state, silu) -> None:
 
 def _op_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], initial: Optional[torch.Tensor],
                 lengths: Optional[torch.Tensor], y: torch.Tensor, state: Optional[torch.Tensor], silu: bool) -> None:
-    _launch_forward(x, weight, bias, initial, lengths, y, state, silu)
+    what = "spear_btp::causal_conv_forward"
+    W, index = _check(what, x, weight, bias, None, initial, lengths)
+    B, L, D = x.shape
+    _call.buffers(what, index, (y, "y", B * L * D, x.dtype), (state, "state", B * (W - 1) * D, x.dtype))
+    if x.numel():
+        _launch_forward(dense_last(x), dense(weight), dense(bias), dense(initial), dense(lengths), y, state, silu)
+    else:
+        _call.pass_on(state, initial)
 
 
 def _op_backward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], initial: Optional[torch.Tensor],
                  lengths: Optional[torch.Tensor], dy: torch.Tensor, dstate: Optional[torch.Tensor], dx: torch.Tensor,
                  dweight: Optional[torch.Tensor], dbias: Optional[torch.Tensor], dinitial: Optional[torch.Tensor], silu: bool) -> None:
+    what = "spear_btp::causal_conv_backward"
+    W, index = _check(what, x, weight, bias, None, initial, lengths)
+    B, L, D = x.shape
+    n, m = B * L * D, B * (W - 1) * D
+    _call.buffers(what, index, (dy, "dy", n, x.dtype), (dstate, "dstate", m, x.dtype), (dx, "dx", n, x.dtype),
+                  (dweight, "dweight", D * W, weight.dtype), (dbias, "dbias", D, weight.dtype), (dinitial, "dinitial", m, x.dtype))
+    if n:
+        _launch_backward(dense_last(x), dense(weight), dense(bias), dense(initial), dense(lengths), dy, dstate, dx, dweight, dbias,
+                         dinitial, silu)
+    else:
+        _call.pass_on(dinitial, dstate), _call.pass_on(dweight, None), _call.pass_on(dbias, None)
+
+
+def _launch_backward(x, weight, bias, initial, lengths, dy, dstate, dx, dweight, dbias, dinitial, silu) -> None:
     B, L, D = x.shape
     W = weight.shape[1]
     index = x.device.index
@@ -97,22 +139,42 @@ def _op_backward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
                _call.ptr(dinitial), _call.ptr(partial), B, L, D, W, sb, st, int(silu), _call.TAG[x.dtype], _call.TAG[weight.dtype])
 
 
+def _launch_step(x_t, state, weight, bias, y, state_out, silu) -> None:
+    B, D = x_t.shape
+    (x_t, pitch), weight, bias = row(x_t), dense(weight), dense(bias)
+    _call.call("btp_sm100_causal_conv_step", x_t.get_device(), x_t.data_ptr(), state.data_ptr(), weight.data_ptr(), _call.ptr(bias),
+               y.data_ptr(), state_out.data_ptr(), B, D, weight.shape[1], pitch, int(silu), _call.TAG[x_t.dtype],
+               _call.TAG[weight.dtype])
+
+
+def _op_step(x_t: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], y: torch.Tensor,
+             state_out: torch.Tensor, silu: bool) -> None:
+    what = "spear_btp::causal_conv_step"
+    index = _check_step(what, x_t, state, weight, bias, None)
+    check_state_out(what, state, state_out)
+    _call.buffers(what, index, (y, "y", x_t.numel(), x_t.dtype))
+    if x_t.numel():
+        _launch_step(x_t, state, weight, bias, y, state_out, silu)
+
+
 def _fake(*args) -> None:
     return None
 
 
 _iface._register(_iface._LIB, "spear_btp", "causal_conv_forward", _op_forward, _fake, ["y", "state"])
 _iface._register(_iface._LIB, "spear_btp", "causal_conv_backward", _op_backward, _fake, ["dx", "dweight", "dbias", "dinitial"])
-_forward = _call.traceable("causal_conv_forward", _op_forward)
-_backward = _call.traceable("causal_conv_backward", _op_backward)
+_iface._register(_iface._LIB, "spear_btp", "causal_conv_step", _op_step, _fake, ["y", "state_out"])
+_forward = _call.traceable("causal_conv_forward", _launch_forward)
+_backward = _call.traceable("causal_conv_backward", _launch_backward)
+_step = _call.traceable("causal_conv_step", _launch_step)
 
 
 class _CausalConv(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, initial, lengths, silu, want_state):
         B, L, D = x.shape
-        y = torch.empty(B, L, D, device=x.device, dtype=x.dtype)
-        state = torch.empty(B, weight.shape[1] - 1, D, device=x.device, dtype=x.dtype) if want_state else None
+        y = x.new_empty((B, L, D))
+        state = x.new_empty((B, weight.shape[1] - 1, D)) if want_state else None
         _forward(x, weight, bias, initial, lengths, y, state, silu)
         ctx.save_for_backward(x, weight, bias, initial, lengths)
         ctx.silu = silu
@@ -126,12 +188,12 @@ class _CausalConv(torch.autograd.Function):
         need_x, need_w, need_b, need_i = ctx.needs_input_grad[:4]
         if dy is None and dstate is None:
             return (None,) * 7
-        dy = torch.zeros(x.shape, device=x.device, dtype=x.dtype) if dy is None else dy.contiguous()
+        dy = x.new_zeros(x.shape) if dy is None else dy.contiguous()
         dstate = None if dstate is None else dstate.contiguous()
-        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-        dw = torch.empty(weight.shape, device=x.device, dtype=weight.dtype) if need_w else None
-        db = torch.empty(bias.shape, device=x.device, dtype=bias.dtype) if need_b and bias is not None else None
-        di = torch.empty(initial.shape, device=x.device, dtype=x.dtype) if need_i and initial is not None else None
+        dx = x.new_empty(x.shape)
+        dw = weight.new_empty(weight.shape) if need_w else None
+        db = bias.new_empty(bias.shape) if need_b and bias is not None else None
+        di = x.new_empty(initial.shape) if need_i and initial is not None else None
         _backward(x, weight, bias, initial, lengths, dy, dstate, dx, dw, db, di, ctx.silu)
         return dx if need_x else None, dw, db, di, None, None, None
 
@@ -152,19 +214,8 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None
     Returns:
         y [B, L, D], or (y, state [B, W-1, D]).  Gradients for x, weight, bias and initial_state.
     """
-    what = "causal_conv"
-    if x.dim() != 3 or x.shape[2] < 1:
-        raise ValueError(f"{what}: x must be [B, L, D], got {tuple(x.shape)}")
+    W, _ = _check("causal_conv", x, weight, bias, activation, initial_state, lengths)
     B, L, D = x.shape
-    _call.activation(x, f"{what}: x")
-    W = _check_filter(what, D, x.dtype, weight, bias, activation)
-    if initial_state is not None:
-        if tuple(initial_state.shape) != (B, W - 1, D):
-            raise ValueError(f"{what}: initial_state must be {(B, W - 1, D)}, got {tuple(initial_state.shape)}")
-        if initial_state.dtype != x.dtype:
-            raise RuntimeError(f"{what}: initial_state must have x's dtype ({x.dtype}), got {initial_state.dtype}")
-    check_lengths(what, lengths, B)
-    _call.on_gpu(what, x, weight, bias, initial_state, lengths)
     if B == 0 or L == 0:  # nothing to compute; the state passes through
         y = x * 1
         if not return_state:
@@ -176,9 +227,9 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None
     if torch.compiler.is_compiling() or (torch.is_grad_enabled() and any(
             t is not None and t.requires_grad for t in (x, weight, bias, initial_state))):
         return _CausalConv.apply(x, weight, bias, initial_state, lengths, silu, bool(return_state))
-    y = torch.empty(B, L, D, device=x.device, dtype=x.dtype)
-    state = torch.empty(B, W - 1, D, device=x.device, dtype=x.dtype) if return_state else None
-    _launch_forward(x, weight, bias, initial_state, lengths, y, state, silu)
+    y = x.new_empty((B, L, D))
+    state = x.new_empty((B, W - 1, D)) if return_state else None
+    _forward(x, weight, bias, initial_state, lengths, y, state, silu)
     return (y, state) if return_state else y
 
 
@@ -204,20 +255,9 @@ def causal_conv_step(x_t: torch.Tensor, state: torch.Tensor, weight: torch.Tenso
     write it: passing the state itself updates it in place (the form for a captured graph).
     """
     what = "causal_conv_step"
-    if x_t.dim() != 2 or x_t.shape[1] < 1:
-        raise ValueError(f"{what}: x_t must be [B, D], got {tuple(x_t.shape)}")
-    B, D = x_t.shape
-    _call.activation(x_t, f"{what}: x_t")
-    W = _check_filter(what, D, x_t.dtype, weight, bias, activation)
-    if state.shape != (B, W - 1, D) or state.dtype != x_t.dtype or not state.is_contiguous():
-        raise ValueError(f"{what}: state must be contiguous {(B, W - 1, D)} of x_t's dtype, got {state.dtype} {tuple(state.shape)}")
-    index = _call.on_gpu(what, x_t, state, weight, bias)
+    _check_step(what, x_t, state, weight, bias, activation)
     out = check_state_out(what, state, state_out)
     y = torch.empty_like(x_t, memory_format=torch.contiguous_format)
-    if B == 0:
-        return y, out
-    (x_t, pitch), weight, bias = row(x_t), dense(weight), dense(bias)
-    _call.call("btp_sm100_causal_conv_step", index, x_t.data_ptr(), state.data_ptr(), weight.data_ptr(), _call.ptr(bias), y.data_ptr(),
-               out.data_ptr(), B, D, W, pitch, int(activation is not None), _call.TAG[x_t.dtype],
-               _call.TAG[weight.dtype])
+    if x_t.shape[0]:
+        _step(x_t, state, weight, bias, y, out, activation is not None)
     return y, out

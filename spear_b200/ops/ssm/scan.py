@@ -17,7 +17,8 @@ from torch.autograd.function import once_differentiable
 
 from ..btp import interface as _iface
 from .. import _call
-from .conv import check_lengths, check_state_out, dense, dense_last, row, strides
+from .._call import dense, dense_last
+from .conv import check_lengths, check_state_out, row, strides
 
 __all__ = ["selective_scan", "selective_scan_step", "MAX_STATES"]
 
@@ -57,6 +58,33 @@ def _check_tokens(what, x, others) -> None:
             raise RuntimeError(f"{what}: {name} must have x's dtype ({dtype}), got {t.dtype}")
 
 
+def _check(what, x, delta, A, B, C, D, z, delta_bias, initial, lengths) -> tuple[int, int]:
+    """(states, device) of a scan over [B, L, D]."""
+    if x.dim() != 3 or x.shape[2] < 1:
+        raise ValueError(f"{what}: x must be [B, L, D], got {tuple(x.shape)}")
+    Bsz, L, dim = x.shape
+    _call.activation(x, f"{what}: x")
+    N = _check_params(what, dim, A, D, delta_bias)
+    _check_tokens(what, x, ((delta, "delta", (Bsz, L, dim)), (z, "z", (Bsz, L, dim)), (B, "B", (Bsz, L, N)), (C, "C", (Bsz, L, N))))
+    if initial is not None and (tuple(initial.shape) != (Bsz, dim, N) or initial.dtype != torch.float32):
+        raise ValueError(f"{what}: initial_state must be float32 {(Bsz, dim, N)}, got {initial.dtype} {tuple(initial.shape)}")
+    check_lengths(what, lengths, Bsz)
+    return N, _call.on_gpu(what, x, delta, A, B, C, D, z, delta_bias, initial, lengths)
+
+
+def _check_step(what, x_t, delta_t, A, B_t, C_t, state, D, z_t, delta_bias) -> int:
+    """The device of a single token's scan."""
+    if x_t.dim() != 2 or x_t.shape[1] < 1:
+        raise ValueError(f"{what}: x_t must be [B, D], got {tuple(x_t.shape)}")
+    Bsz, dim = x_t.shape
+    _call.activation(x_t, f"{what}: x_t")
+    N = _check_params(what, dim, A, D, delta_bias)
+    _check_tokens(what, x_t, ((delta_t, "delta_t", x_t.shape), (z_t, "z_t", x_t.shape), (B_t, "B_t", (Bsz, N)), (C_t, "C_t", (Bsz, N))))
+    if state.shape != (Bsz, dim, N) or state.dtype != torch.float32 or not state.is_contiguous():
+        raise ValueError(f"{what}: state must be contiguous float32 {(Bsz, dim, N)}, got {state.dtype} {tuple(state.shape)}")
+    return _call.on_gpu(what, x_t, delta_t, A, B_t, C_t, state, D, z_t, delta_bias)
+
+
 def _shape_args(x, delta, A, B, C, z):
     zb, zt = (0, 0) if z is None else strides(z)
     return (x.shape[0], x.shape[1], x.shape[2], A.shape[1], *strides(x), *strides(delta), *strides(B), *strides(C), zb, zt)
@@ -76,9 +104,18 @@ def _launch_forward(x, delta, A, B, C, D, z, delta_bias, initial, lengths, y, st
 
 def _op_forward(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, D: Optional[torch.Tensor],
                 z: Optional[torch.Tensor], delta_bias: Optional[torch.Tensor], initial: Optional[torch.Tensor],
-                lengths: Optional[torch.Tensor], y: torch.Tensor, state: Optional[torch.Tensor], checkpoints: torch.Tensor,
+                lengths: Optional[torch.Tensor], y: torch.Tensor, state: Optional[torch.Tensor], checkpoints: Optional[torch.Tensor],
                 softplus: bool) -> None:
-    _launch_forward(x, delta, A, B, C, D, z, delta_bias, initial, lengths, y, state, checkpoints, softplus)
+    what = "spear_btp::scan_forward"
+    N, index = _check(what, x, delta, A, B, C, D, z, delta_bias, initial, lengths)
+    Bsz, L, dim = x.shape
+    _call.buffers(what, index, (y, "y", x.numel(), x.dtype), (state, "state", Bsz * dim * N, torch.float32),
+                  (checkpoints, "checkpoints", Bsz * -(-L // _CHECKPOINT) * dim * N, torch.float32))
+    if x.numel():
+        _launch_forward(dense_last(x), dense_last(delta), dense(A), dense_last(B), dense_last(C), dense(D), dense_last(z),
+                        dense(delta_bias), dense(initial), dense(lengths), y, state, checkpoints, softplus)
+    else:
+        _call.pass_on(state, initial)
 
 
 def _op_backward(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, D: Optional[torch.Tensor],
@@ -86,6 +123,30 @@ def _op_backward(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch
                  checkpoints: torch.Tensor, dy: torch.Tensor, dstate: Optional[torch.Tensor], dx: torch.Tensor, ddelta: torch.Tensor,
                  dparams: torch.Tensor, dB: torch.Tensor, dC: torch.Tensor, dz: Optional[torch.Tensor],
                  dinitial: Optional[torch.Tensor], softplus: bool) -> None:
+    what = "spear_btp::scan_backward"
+    N, index = _check(what, x, delta, A, B, C, D, z, delta_bias, None, lengths)
+    Bsz, L, dim = x.shape
+    n, m, f32 = x.numel(), Bsz * dim * N, torch.float32
+    if z is not None and dz is None:
+        raise ValueError(f"{what}: z comes with dz")
+    _call.buffers(what, index, (checkpoints, "checkpoints", Bsz * -(-L // _CHECKPOINT) * dim * N, f32), (dy, "dy", n, x.dtype),
+                  (dstate, "dstate", m, f32), (dx, "dx", n, x.dtype), (ddelta, "ddelta", n, x.dtype),
+                  (dparams, "dparams", _parameter_floats(dim, N), f32), (dB, "dB", B.numel(), x.dtype), (dC, "dC", C.numel(), x.dtype),
+                  (dz, "dz", n, x.dtype), (dinitial, "dinitial", m, f32))
+    if n:
+        _launch_backward(dense_last(x), dense_last(delta), dense(A), dense_last(B), dense_last(C), dense(D), dense_last(z),
+                         dense(delta_bias), dense(lengths), checkpoints, dy, dstate, dx, ddelta, dparams, dB, dC, dz, dinitial, softplus)
+    else:
+        _call.pass_on(dinitial, dstate), _call.pass_on(dparams, None)
+
+
+def _parameter_floats(dim: int, N: int) -> int:
+    """Elements of dA, dD and dbias, one after the other, up to a whole 16 bytes."""
+    return -(-dim * (N + 2) // 4) * 4
+
+
+def _launch_backward(x, delta, A, B, C, D, z, delta_bias, lengths, checkpoints, dy, dstate, dx, ddelta, dparams, dB, dC, dz, dinitial,
+                     softplus) -> None:
     index = x.device.index
     A, dstate = _aligned(A), _aligned(dstate)
     shape = _shape_args(x, delta, A, B, C, z)
@@ -97,14 +158,39 @@ def _op_backward(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch
                _call.TAG[x.dtype])
 
 
+def _launch_step(x_t, delta_t, A, B_t, C_t, state, D, z_t, delta_bias, y, state_out, softplus) -> None:
+    Bsz, dim = x_t.shape
+    if (state.data_ptr() | state_out.data_ptr()) % 16:
+        raise ValueError("selective_scan_step: state and state_out must be 16-byte aligned")
+    (x_t, px), (delta_t, pd), (B_t, pB), (C_t, pC), (z_t, pz) = row(x_t), row(delta_t), row(B_t), row(C_t), row(z_t)
+    A, D, delta_bias = _aligned(dense(A)), dense(D), dense(delta_bias)
+    p = _call.ptr
+    _call.call("btp_sm100_scan_step", x_t.get_device(), x_t.data_ptr(), delta_t.data_ptr(), A.data_ptr(), B_t.data_ptr(), C_t.data_ptr(),
+               p(D), p(z_t), p(delta_bias), state.data_ptr(), y.data_ptr(), state_out.data_ptr(), Bsz, dim, A.shape[1], px, pd, pB, pC, pz,
+               1 if softplus else 0, _call.TAG[x_t.dtype])
+
+
+def _op_step(x_t: torch.Tensor, delta_t: torch.Tensor, A: torch.Tensor, B_t: torch.Tensor, C_t: torch.Tensor, state: torch.Tensor,
+             D: Optional[torch.Tensor], z_t: Optional[torch.Tensor], delta_bias: Optional[torch.Tensor], y: torch.Tensor,
+             state_out: torch.Tensor, softplus: bool) -> None:
+    what = "spear_btp::scan_step"
+    index = _check_step(what, x_t, delta_t, A, B_t, C_t, state, D, z_t, delta_bias)
+    check_state_out(what, state, state_out)
+    _call.buffers(what, index, (y, "y", x_t.numel(), x_t.dtype))
+    if x_t.numel():
+        _launch_step(x_t, delta_t, A, B_t, C_t, state, D, z_t, delta_bias, y, state_out, softplus)
+
+
 def _fake(*args) -> None:
     return None
 
 
 _iface._register(_iface._LIB, "spear_btp", "scan_forward", _op_forward, _fake, ["y", "state", "checkpoints"])
 _iface._register(_iface._LIB, "spear_btp", "scan_backward", _op_backward, _fake, ["dx", "ddelta", "dparams", "dB", "dC", "dz", "dinitial"])
-_forward = _call.traceable("scan_forward", _op_forward)
-_backward = _call.traceable("scan_backward", _op_backward)
+_iface._register(_iface._LIB, "spear_btp", "scan_step", _op_step, _fake, ["y", "state_out"])
+_forward = _call.traceable("scan_forward", _launch_forward)
+_backward = _call.traceable("scan_backward", _launch_backward)
+_step = _call.traceable("scan_step", _launch_step)
 
 
 class _SelectiveScan(torch.autograd.Function):
@@ -112,9 +198,9 @@ class _SelectiveScan(torch.autograd.Function):
     def forward(ctx, x, delta, A, B, C, D, z, delta_bias, initial, lengths, softplus, want_state):
         Bsz, L, dim = x.shape
         N = A.shape[1]
-        y = torch.empty(Bsz, L, dim, device=x.device, dtype=x.dtype)
-        state = torch.empty(Bsz, dim, N, device=x.device, dtype=torch.float32) if want_state else None
-        checkpoints = torch.empty(Bsz, -(-L // _CHECKPOINT), dim, N, device=x.device, dtype=torch.float32)
+        y = x.new_empty((Bsz, L, dim))
+        state = x.new_empty((Bsz, dim, N), dtype=torch.float32) if want_state else None
+        checkpoints = x.new_empty((Bsz, -(-L // _CHECKPOINT), dim, N), dtype=torch.float32)
         _forward(x, delta, A, B, C, D, z, delta_bias, initial, lengths, y, state, checkpoints, softplus)
         ctx.save_for_backward(x, delta, A, B, C, D, z, delta_bias, lengths, checkpoints)
         ctx.softplus = softplus
@@ -128,18 +214,17 @@ class _SelectiveScan(torch.autograd.Function):
         need = ctx.needs_input_grad
         if dy is None and dstate is None:
             return (None,) * 12
-        dev, dtype = x.device, x.dtype
         Bsz, L, dim = x.shape
         N = A.shape[1]
-        dy = torch.zeros(x.shape, device=dev, dtype=dtype) if dy is None else dy.contiguous()
+        dy = x.new_zeros(x.shape) if dy is None else dy.contiguous()
         dstate = dense(dstate)
-        dx, ddelta = (torch.empty(x.shape, device=dev, dtype=dtype) for _ in range(2))
-        dz = None if z is None else torch.empty(x.shape, device=dev, dtype=dtype)
-        dB, dC = (torch.empty(B.shape, device=dev, dtype=dtype) for _ in range(2))
-        dparams = torch.empty(-(-dim * (N + 2) // 4) * 4, device=dev, dtype=torch.float32)
-        dinitial = torch.empty(Bsz, dim, N, device=dev, dtype=torch.float32) if need[8] else None
-        _backward(x, delta, A, B, C, D, z, delta_bias, lengths, checkpoints, dy, dstate, dx, ddelta, dparams,
-                                          dB, dC, dz, dinitial, ctx.softplus)
+        dx, ddelta = (x.new_empty(x.shape) for _ in range(2))
+        dz = None if z is None else x.new_empty(x.shape)
+        dB, dC = (x.new_empty(B.shape) for _ in range(2))
+        dparams = x.new_empty(_parameter_floats(dim, N), dtype=torch.float32)
+        dinitial = x.new_empty((Bsz, dim, N), dtype=torch.float32) if need[8] else None
+        _backward(x, delta, A, B, C, D, z, delta_bias, lengths, checkpoints, dy, dstate, dx, ddelta, dparams, dB, dC, dz, dinitial,
+                  ctx.softplus)
         dA, dD, dbias = dparams[:dim * N].view(dim, N), dparams[dim * N:dim * (N + 1)], dparams[dim * (N + 1):dim * (N + 2)]
         grads = (dx, ddelta, dA, dB, dC, None if D is None else dD, dz, None if delta_bias is None else dbias, dinitial)
         return (*(g if n else None for g, n in zip(grads, need)), None, None, None)
@@ -168,30 +253,21 @@ def selective_scan(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: tor
         y [B, L, D], or (y, state [B, D, N] float32).  Gradients for every floating-point argument; the backward pass
         keeps one state per 16 tokens from the forward.
     """
-    what = "selective_scan"
-    if x.dim() != 3 or x.shape[2] < 1:
-        raise ValueError(f"{what}: x must be [B, L, D], got {tuple(x.shape)}")
+    N, _ = _check("selective_scan", x, delta, A, B, C, D, z, delta_bias, initial_state, lengths)
     Bsz, L, dim = x.shape
-    _call.activation(x, f"{what}: x")
-    N = _check_params(what, dim, A, D, delta_bias)
-    _check_tokens(what, x, ((delta, "delta", (Bsz, L, dim)), (z, "z", (Bsz, L, dim)), (B, "B", (Bsz, L, N)), (C, "C", (Bsz, L, N))))
-    if initial_state is not None and (tuple(initial_state.shape) != (Bsz, dim, N) or initial_state.dtype != torch.float32):
-        raise ValueError(f"{what}: initial_state must be float32 {(Bsz, dim, N)}, got {initial_state.dtype} {tuple(initial_state.shape)}")
-    check_lengths(what, lengths, Bsz)
-    _call.on_gpu(what, x, delta, A, B, C, D, z, delta_bias, initial_state, lengths)
     if Bsz == 0 or L == 0:  # nothing to compute; the state passes through
         y = x * 1
         if not return_state:
             return y
-        return y, (torch.zeros(Bsz, dim, N, device=x.device, dtype=torch.float32) if initial_state is None else initial_state.clone())
+        return y, (x.new_zeros((Bsz, dim, N), dtype=torch.float32) if initial_state is None else initial_state.clone())
     x, delta, B, C, z = dense_last(x), dense_last(delta), dense_last(B), dense_last(C), dense_last(z)
     A, D, delta_bias, initial_state, lengths = dense(A), dense(D), dense(delta_bias), dense(initial_state), dense(lengths)
     if torch.compiler.is_compiling() or (torch.is_grad_enabled() and any(
             t is not None and t.requires_grad for t in (x, delta, A, B, C, D, z, delta_bias, initial_state))):
         return _SelectiveScan.apply(x, delta, A, B, C, D, z, delta_bias, initial_state, lengths, bool(delta_softplus), bool(return_state))
-    y = torch.empty(Bsz, L, dim, device=x.device, dtype=x.dtype)
-    state = torch.empty(Bsz, dim, N, device=x.device, dtype=torch.float32) if return_state else None
-    _launch_forward(x, delta, A, B, C, D, z, delta_bias, initial_state, lengths, y, state, None, bool(delta_softplus))
+    y = x.new_empty((Bsz, L, dim))
+    state = x.new_empty((Bsz, dim, N), dtype=torch.float32) if return_state else None
+    _forward(x, delta, A, B, C, D, z, delta_bias, initial_state, lengths, y, state, None, bool(delta_softplus))
     return (y, state) if return_state else y
 
 
@@ -205,25 +281,9 @@ def selective_scan_step(x_t: torch.Tensor, delta_t: torch.Tensor, A: torch.Tenso
     itself updates it in place (the form for a captured graph).
     """
     what = "selective_scan_step"
-    if x_t.dim() != 2 or x_t.shape[1] < 1:
-        raise ValueError(f"{what}: x_t must be [B, D], got {tuple(x_t.shape)}")
-    Bsz, dim = x_t.shape
-    _call.activation(x_t, f"{what}: x_t")
-    N = _check_params(what, dim, A, D, delta_bias)
-    _check_tokens(what, x_t, ((delta_t, "delta_t", x_t.shape), (z_t, "z_t", x_t.shape), (B_t, "B_t", (Bsz, N)), (C_t, "C_t", (Bsz, N))))
-    if state.shape != (Bsz, dim, N) or state.dtype != torch.float32 or not state.is_contiguous():
-        raise ValueError(f"{what}: state must be contiguous float32 {(Bsz, dim, N)}, got {state.dtype} {tuple(state.shape)}")
-    index = _call.on_gpu(what, x_t, delta_t, A, B_t, C_t, state, D, z_t, delta_bias)
+    _check_step(what, x_t, delta_t, A, B_t, C_t, state, D, z_t, delta_bias)
     out = check_state_out(what, state, state_out)
     y = torch.empty_like(x_t, memory_format=torch.contiguous_format)
-    if Bsz == 0:
-        return y, out
-    if (state.data_ptr() | out.data_ptr()) % 16:
-        raise ValueError(f"{what}: state and state_out must be 16-byte aligned")
-    (x_t, px), (delta_t, pd), (B_t, pB), (C_t, pC), (z_t, pz) = row(x_t), row(delta_t), row(B_t), row(C_t), row(z_t)
-    A, D, delta_bias = _aligned(dense(A)), dense(D), dense(delta_bias)
-    p = _call.ptr
-    _call.call("btp_sm100_scan_step", index, x_t.data_ptr(), delta_t.data_ptr(), A.data_ptr(), B_t.data_ptr(), C_t.data_ptr(), p(D),
-               p(z_t), p(delta_bias), state.data_ptr(), y.data_ptr(), out.data_ptr(), Bsz, dim, N, px, pd, pB, pC, pz,
-               1 if delta_softplus else 0, _call.TAG[x_t.dtype])
+    if x_t.shape[0]:
+        _step(x_t, delta_t, A, B_t, C_t, state, D, z_t, delta_bias, y, out, bool(delta_softplus))
     return y, out
