@@ -7,6 +7,7 @@ machine.  Like the other operators here these have no CPU path and no fallback.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _btp as _native
 from .. import _lib
@@ -29,7 +30,11 @@ def activation(t: torch.Tensor, what: str) -> None:
 
 
 def on_gpu(what: str, first: torch.Tensor, *others) -> int:
-    """All tensors (None is skipped) on one CUDA device; returns its index."""
+    """All tensors (None is skipped) on one CUDA device and without tangents; returns the device's index."""
+    if forward_ad._current_level >= 0:  # a dual tensor does not require grad: nothing else would notice it, and its tangent would be lost
+        for t in (first, *others):
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{what} has no forward-mode derivative")
     index = first.get_device()
     if index < 0:
         raise RuntimeError(f"{what} needs CUDA tensors: this package has no CPU path and no fallback")

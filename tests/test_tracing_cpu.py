@@ -154,6 +154,25 @@ def test_functional_transforms_are_refused(stand_in):
             call()
 
 
+@pytest.mark.parametrize("case", CALLS, ids=str)
+def test_forward_mode_is_refused(case):
+    """A dual tensor in any place; a result without its tangent would be a wrong derivative."""
+    from torch.autograd import forward_ad
+
+    _, fn, make = CALLS[case]
+    for i in range(len(make())):
+        args = list(make())
+        with forward_ad.dual_level():
+            args[i] = forward_ad.make_dual(args[i], torch.ones_like(args[i]))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                fn(*args)
+            with pytest.raises(RuntimeError, match="no CPU path"):  # an open level alone changes nothing
+                fn(*make())
+    args = make()
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(lambda x: fn(x, *args[1:]), args[:1], args[:1])
+
+
 def test_recorded_ops_check_what_they_are_given(monkeypatch):
     """A recorded program runs the op on tensors of other shapes and strides than it was recorded with."""
     from spear_b200.ops.norm import interface as norm
