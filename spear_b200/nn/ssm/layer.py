@@ -59,7 +59,6 @@ class SelectiveSSM(nn.Module):
             raise ValueError(f"need 0 < dt_min <= dt_max (got {dt_min}, {dt_max})")
         self.dim, self.state_size, self.width, self.inner = dim, state_size, width, expand * dim
         self.rank = -(-dim // 16) if rank is None else rank
-        self.dtype = dtype
         self.in_proj = nn.Linear(dim, 2 * self.inner, bias=False, dtype=dtype)
         self.conv_weight = nn.Parameter(torch.empty(self.inner, width, dtype=dtype).uniform_(-1, 1) / math.sqrt(width))
         self.conv_bias = nn.Parameter(torch.zeros(self.inner, dtype=dtype))
@@ -70,6 +69,11 @@ class SelectiveSSM(nn.Module):
         self.A_log = nn.Parameter(torch.arange(1, state_size + 1, dtype=torch.float32).log().repeat(self.inner, 1))
         self.D = nn.Parameter(torch.ones(self.inner))
         self.out_proj = nn.Linear(self.inner, dim, bias=False, dtype=dtype)
+
+    @property
+    def dtype(self) -> torch.dtype:
+        """Type of the projections as they are now: `.to()` may have cast the module."""
+        return self.in_proj.weight.dtype
 
     def _parameters_of_scan(self):
         """Rates, input weight and step bias in float32, also where `.to()` has cast the module."""

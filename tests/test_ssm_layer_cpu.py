@@ -59,3 +59,14 @@ def test_public_names():
     assert spear_b200.SelectiveSSM is SelectiveSSM and spear_b200.MixerBlock is MixerBlock
     for name in ("rms_norm", "rms_norm_8bit", "causal_conv", "causal_conv_step", "selective_scan", "selective_scan_step"):
         assert callable(getattr(ops, name))
+
+
+@pytest.mark.parametrize("built,cast", [(torch.float32, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float32, torch.float16)])
+def test_a_cast_layer_works_in_its_new_type(built, cast):
+    layer = SelectiveSSM(dim=16, dtype=built).to(cast)
+    assert layer.dtype == cast and layer.empty_state(2).conv.dtype == cast and layer.empty_state(2).ssm.dtype == torch.float32
+    for given in (built, cast):  # past the projections, up to the first operator
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            layer(torch.randn(1, 4, 16, dtype=given))
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            layer.step(torch.randn(1, 16, dtype=given), layer.empty_state(1))

@@ -203,3 +203,16 @@ def test_8bit_norm_feeds_a_scaled_product():
     true = y.double() @ weight.double().t()
     off = y.double().abs() @ weight.double().abs().t() * (2 * 2.0 ** -4 + 2.0 ** -8) + 512 * 2.0 ** -10 * scale.double()[:, None] * ws.double().t() * 900
     assert ((exact - true).abs() <= off).all()
+
+
+@pytest.mark.parametrize("built,cast", [(torch.float32, torch.bfloat16), (torch.bfloat16, torch.float32)])
+def test_a_cast_layer_is_a_layer_of_that_type(built, cast):
+    """The same parameters, A, D and the step bias rounded by the cast and used in float32 again: the same bits."""
+    a = layer(dtype=built).to(cast)
+    b = layer(dtype=cast)
+    b.load_state_dict(a.state_dict())
+    u = torch.randn(2, 30, 64, device="cuda")
+    assert torch.equal(a(u), b(u)) and a(u).dtype == cast
+    (ya, sa), (yb, sb) = a.prefill(u), b.prefill(u)
+    assert torch.equal(ya, yb) and torch.equal(sa.conv, sb.conv) and torch.equal(sa.ssm, sb.ssm)
+    assert torch.equal(a.step(u[:, 0], a.empty_state(2))[0], b.step(u[:, 0], b.empty_state(2))[0])
