@@ -87,6 +87,9 @@ class SelectiveSSM(nn.Module):
     def _run(self, u, state, lengths, return_state):
         if u.dim() != 3 or u.shape[2] != self.dim:
             raise ValueError(f"SelectiveSSM takes [B, L, {self.dim}], got {tuple(u.shape)}")
+        if lengths is not None and torch.is_grad_enabled():
+            # in_proj's weight gradient sums over all tokens: behind a sequence's end zero times whatever the padding holds, NaN for NaN
+            u = u.masked_fill((torch.arange(u.shape[1], device=u.device) >= lengths[:, None])[..., None], 0.0)
         x, z = self.in_proj(u.to(self.dtype)).split(self.inner, dim=-1)
         conv = causal_conv(x, self.conv_weight, self.conv_bias, activation="silu", initial_state=None if state is None else state.conv,
                            lengths=lengths, return_state=return_state)

@@ -216,3 +216,21 @@ def test_a_cast_layer_is_a_layer_of_that_type(built, cast):
     (ya, sa), (yb, sb) = a.prefill(u), b.prefill(u)
     assert torch.equal(ya, yb) and torch.equal(sa.conv, sb.conv) and torch.equal(sa.ssm, sb.ssm)
     assert torch.equal(a.step(u[:, 0], a.empty_state(2))[0], b.step(u[:, 0], b.empty_state(2))[0])
+
+
+def test_padding_never_reaches_a_gradient():
+    """NaN and infinities behind the sequences' ends: outputs and every gradient as with any other padding."""
+    m = layer()
+    n = torch.tensor([30, 0, 7], device="cuda", dtype=torch.int32)
+    u = torch.randn(3, 30, 64, device="cuda")
+    up = torch.randn(3, 30, 64, device="cuda")
+    dirty = u.clone()
+    dirty[1], dirty[2, 7:20], dirty[2, 20:] = float("nan"), float("inf"), -1e30
+
+    def run(v):
+        v = v.detach().requires_grad_(True)
+        y = m(v, lengths=n)
+        return [y.detach(), *torch.autograd.grad(y, [v, *m.parameters()], up)]
+
+    for a, b in zip(run(u), run(dirty)):
+        assert torch.equal(a, b) and torch.isfinite(b).all()
