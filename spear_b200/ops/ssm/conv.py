@@ -237,6 +237,8 @@ def check_state_out(what, state, state_out) -> torch.Tensor:
     """Where the new state goes: fresh memory, or the caller's tensor, which may be the old state itself."""
     if state_out is None:
         return torch.empty_like(state, memory_format=torch.contiguous_format)
+    if state_out.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what}: state_out requires grad, and a token has no gradient: detach it, or call under torch.no_grad()")
     if state_out is state:
         return state_out
     if state_out.shape != state.shape or state_out.dtype != state.dtype or state_out.device != state.device or not state_out.is_contiguous():
@@ -247,12 +249,19 @@ def check_state_out(what, state, state_out) -> torch.Tensor:
     return state_out
 
 
+def written(state_out: torch.Tensor | None) -> None:
+    """Tells autograd that the caller's tensor has changed, so that a backward pass that needs its old values fails."""
+    if state_out is not None and not torch.compiler.is_compiling() and not state_out.is_inference():
+        torch.autograd.graph.increment_version(state_out)
+
+
 def causal_conv_step(x_t: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
                      activation: str | None = None, state_out: torch.Tensor | None = None):
     """One token of ``causal_conv``: returns (y_t [B, D], new state [B, W-1, D]).
 
-    One kernel launch.  ``state`` stays valid and the new state is a fresh tensor, unless ``state_out`` says where to
-    write it: passing the state itself updates it in place (the form for a captured graph).
+    One kernel launch, no gradient: neither result requires grad, whatever the inputs do.  ``state`` stays valid and the
+    new state is a fresh tensor, unless ``state_out`` says where to write it: passing the state itself updates it in
+    place (the form for a captured graph).
     """
     what = "causal_conv_step"
     _check_step(what, x_t, state, weight, bias, activation)
@@ -260,4 +269,5 @@ def causal_conv_step(x_t: torch.Tensor, state: torch.Tensor, weight: torch.Tenso
     y = torch.empty_like(x_t, memory_format=torch.contiguous_format)
     if x_t.shape[0]:
         _step(x_t, state, weight, bias, y, out, activation is not None)
+        written(state_out)
     return y, out

@@ -18,7 +18,7 @@ from torch.autograd.function import once_differentiable
 from ..btp import interface as _iface
 from .. import _call
 from .._call import dense, dense_last
-from .conv import check_lengths, check_state_out, row, strides
+from .conv import check_lengths, check_state_out, row, strides, written
 
 __all__ = ["selective_scan", "selective_scan_step", "MAX_STATES"]
 
@@ -276,9 +276,10 @@ def selective_scan_step(x_t: torch.Tensor, delta_t: torch.Tensor, A: torch.Tenso
                         delta_bias: torch.Tensor | None = None, delta_softplus: bool = False, state_out: torch.Tensor | None = None):
     """One token of ``selective_scan``: returns (y_t [B, D], new state [B, D, N] float32).
 
-    x_t, delta_t, z_t [B, D] and B_t, C_t [B, N] as there, without the token dimension.  One kernel launch.  ``state``
-    stays valid and the new state is a fresh tensor, unless ``state_out`` says where to write it: passing the state
-    itself updates it in place (the form for a captured graph).
+    x_t, delta_t, z_t [B, D] and B_t, C_t [B, N] as there, without the token dimension.  One kernel launch, no gradient:
+    neither result requires grad, whatever the inputs do.  ``state`` stays valid and the new state is a fresh tensor,
+    unless ``state_out`` says where to write it: passing the state itself updates it in place (the form for a captured
+    graph).
     """
     what = "selective_scan_step"
     _check_step(what, x_t, delta_t, A, B_t, C_t, state, D, z_t, delta_bias)
@@ -286,4 +287,5 @@ def selective_scan_step(x_t: torch.Tensor, delta_t: torch.Tensor, A: torch.Tenso
     y = torch.empty_like(x_t, memory_format=torch.contiguous_format)
     if x_t.shape[0]:
         _step(x_t, delta_t, A, B_t, C_t, state, D, z_t, delta_bias, y, out, bool(delta_softplus))
+        written(state_out)
     return y, out

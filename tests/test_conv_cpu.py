@@ -78,3 +78,36 @@ def test_entry_refuses_bad_arguments_before_any_launch():
     step = lib.btp_sm100_causal_conv_step
     assert step(p, p, p, None, p, None, 1, 8, 4, 8, 0, 0, 0, None) == -1
     assert step(p, p, p, None, p, p, 1, 8, 9, 8, 0, 0, 0, None) == -3
+
+
+@pytest.mark.parametrize("token", ["conv", "scan"])
+def test_autograd_learns_of_a_state_that_is_updated_in_place(monkeypatch, token):
+    """A tensor that some graph has saved must not change unseen; a tensor with a gradient of its own is not overwritten."""
+    from spear_b200.ops import _call
+    from spear_b200.ops.ssm import selective_scan_step
+
+    monkeypatch.setattr(_call, "call", lambda *args: None)
+    monkeypatch.setattr(_call, "on_gpu", lambda what, first, *others: 0)
+    if token == "conv":
+        state, w = torch.randn(2, 3, 8), torch.nn.Parameter(torch.randn(8, 4))
+        step = lambda **kw: causal_conv_step(Z(2, 8), state, w, **kw)
+    else:
+        state, w = torch.randn(2, 8, 4), torch.nn.Parameter(torch.randn(8, 4))
+        step = lambda **kw: selective_scan_step(Z(2, 8), Z(2, 8), w, Z(2, 4), Z(2, 4), state, **kw)
+    loss = (state * torch.ones_like(state, requires_grad=True)).sum()  # saves the state
+    before = state._version
+    y, new = step()
+    assert state._version == before and not y.requires_grad and not new.requires_grad
+    y, new = step(state_out=state)
+    assert new is state and state._version == before + 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    other = torch.empty_like(state)
+    step(state_out=other)
+    assert other._version == 1
+    with pytest.raises(ValueError, match="requires grad"):
+        step(state_out=torch.empty_like(state).requires_grad_())
+    with torch.no_grad():
+        step(state_out=torch.empty_like(state).requires_grad_())
+    with torch.inference_mode():
+        step(state_out=torch.empty_like(state))
