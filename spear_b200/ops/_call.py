@@ -29,6 +29,12 @@ def activation(t: torch.Tensor, what: str) -> None:
         raise RuntimeError(f"{what} must be bfloat16, float16 or float32 (got {t.dtype})")
 
 
+def sizes(what: str, shape) -> None:
+    """The C entries take 32-bit sizes, and ctypes would cut a larger one off without a word."""
+    if max(shape) > 0x7FFFFFFF:
+        raise ValueError(f"{what}: every size must be below 2^31, got {tuple(shape)}")
+
+
 def on_gpu(what: str, first: torch.Tensor, *others) -> int:
     """All tensors (None is skipped) on one CUDA device and without tangents; returns the device's index."""
     if forward_ad._current_level >= 0:  # a dual tensor does not require grad: nothing else would notice it, and its tangent would be lost

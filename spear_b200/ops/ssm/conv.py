@@ -51,6 +51,7 @@ def _check(what, x, weight, bias, activation, initial, lengths) -> tuple[int, in
         raise ValueError(f"{what}: x must be [B, L, D], got {tuple(x.shape)}")
     B, L, D = x.shape
     _call.activation(x, f"{what}: x")
+    _call.sizes(what, x.shape)
     W = _check_filter(what, D, x.dtype, weight, bias, activation)
     if initial is not None:
         if tuple(initial.shape) != (B, W - 1, D):
@@ -67,6 +68,7 @@ def _check_step(what, x_t, state, weight, bias, activation) -> int:
         raise ValueError(f"{what}: x_t must be [B, D], got {tuple(x_t.shape)}")
     B, D = x_t.shape
     _call.activation(x_t, f"{what}: x_t")
+    _call.sizes(what, x_t.shape)
     W = _check_filter(what, D, x_t.dtype, weight, bias, activation)
     if state.shape != (B, W - 1, D) or state.dtype != x_t.dtype or not state.is_contiguous():
         raise ValueError(f"{what}: state must be contiguous {(B, W - 1, D)} of x_t's dtype, got {state.dtype} {tuple(state.shape)}")

@@ -64,6 +64,7 @@ def _check(what, x, delta, A, B, C, D, z, delta_bias, initial, lengths) -> tuple
         raise ValueError(f"{what}: x must be [B, L, D], got {tuple(x.shape)}")
     Bsz, L, dim = x.shape
     _call.activation(x, f"{what}: x")
+    _call.sizes(what, x.shape)
     N = _check_params(what, dim, A, D, delta_bias)
     _check_tokens(what, x, ((delta, "delta", (Bsz, L, dim)), (z, "z", (Bsz, L, dim)), (B, "B", (Bsz, L, N)), (C, "C", (Bsz, L, N))))
     if initial is not None and (tuple(initial.shape) != (Bsz, dim, N) or initial.dtype != torch.float32):
@@ -78,6 +79,7 @@ def _check_step(what, x_t, delta_t, A, B_t, C_t, state, D, z_t, delta_bias) -> i
         raise ValueError(f"{what}: x_t must be [B, D], got {tuple(x_t.shape)}")
     Bsz, dim = x_t.shape
     _call.activation(x_t, f"{what}: x_t")
+    _call.sizes(what, x_t.shape)
     N = _check_params(what, dim, A, D, delta_bias)
     _check_tokens(what, x_t, ((delta_t, "delta_t", x_t.shape), (z_t, "z_t", x_t.shape), (B_t, "B_t", (Bsz, N)), (C_t, "C_t", (Bsz, N))))
     if state.shape != (Bsz, dim, N) or state.dtype != torch.float32 or not state.is_contiguous():

@@ -111,3 +111,13 @@ def test_autograd_learns_of_a_state_that_is_updated_in_place(monkeypatch, token)
         step(state_out=torch.empty_like(state).requires_grad_())
     with torch.inference_mode():
         step(state_out=torch.empty_like(state))
+
+
+@pytest.mark.parametrize("B,L,D", [(2 ** 32 + 1, 1, 1), (1, 2 ** 32 + 5, 1), (1, 1, 2 ** 32 + 8)])
+def test_sizes_beyond_32_bits_are_refused_not_cut_off(B, L, D):
+    E = lambda *shape: torch.empty(*shape, device="meta")
+    with pytest.raises(ValueError, match="below 2\\^31"):
+        causal_conv(E(B, L, D), E(D, 4))
+    if L == 1:
+        with pytest.raises(ValueError, match="below 2\\^31"):
+            causal_conv_step(E(B, D), E(B, 3, D), E(D, 4))

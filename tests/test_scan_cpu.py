@@ -119,3 +119,15 @@ def test_oracle_agrees_with_autograd():
     assert torch.allclose(got["y"].v, torch.stack(ys)) and torch.allclose(got["state"].v, torch.stack(ends))
     for name, gr in zip(w, grads):
         assert torch.allclose(got["d" + {"delta_bias": "bias"}.get(name, name)].v, gr, atol=1e-12), name
+
+
+@pytest.mark.parametrize("B,L,D", [(2 ** 32 + 1, 1, 1), (1, 2 ** 32 + 5, 1), (1, 1, 2 ** 32 + 8)])
+def test_sizes_beyond_32_bits_are_refused_not_cut_off(B, L, D):
+    from spear_b200.ops.ssm import selective_scan, selective_scan_step
+
+    E = lambda *shape: torch.empty(*shape, device="meta")
+    with pytest.raises(ValueError, match="below 2\\^31"):
+        selective_scan(E(B, L, D), E(B, L, D), E(D, 2), E(B, L, 2), E(B, L, 2))
+    if L == 1:
+        with pytest.raises(ValueError, match="below 2\\^31"):
+            selective_scan_step(E(B, D), E(B, D), E(D, 2), E(B, 2), E(B, 2), E(B, D, 2))
