@@ -161,12 +161,20 @@ __device__ __forceinline__ void load_rates(LaneState& A2, const float* A, int c0
     A2.r[i >> 2][i & 3] = pack2(a < -3e38f ? -3e38f : a, b < -3e38f ? -3e38f : b);
   }
 }
-// h = exp(A total) h + last: the effect of a whole chunk with step sizes that sum up to `total`.
+// h = 2^x h + last: the effect of a whole chunk, x being the rate to the base 2 times the sum of its step sizes.  2^x may leave the range
+// of a float where the token by token product does not: what exceeds 2^+-126 is applied to h first (a factor of exactly 1
+// otherwise), and a state of 0 stays 0 however much the chunk would make it grow.
+__device__ __forceinline__ float outside(float v, float x) { return v == 0.f ? 0.f : ex2(x - fminf(fmaxf(x, -126.f), 126.f)) * v; }
+__device__ __forceinline__ f32x2 over_chunk(f32x2 h, f32x2 x, f32x2 last) {
+  const float x0 = lo2(x), x1 = hi2(x);
+  const f32x2 a = pack2(ex2(fminf(fmaxf(x0, -126.f), 126.f)), ex2(fminf(fmaxf(x1, -126.f), 126.f)));
+  return fma2(a, pack2(outside(lo2(h), x0), outside(hi2(h), x1)), last);
+}
 __device__ __forceinline__ void apply_chunk(LaneState& h, const LaneState& A2, const LaneState& last, f32x2 t0, f32x2 t1) {
 #pragma unroll
   for (int n = 0; n < 4; ++n) {
-    h.r[0][n] = fma2(ex2_2(mul2(A2.r[0][n], t0)), h.r[0][n], last.r[0][n]);
-    h.r[1][n] = fma2(ex2_2(mul2(A2.r[1][n], t1)), h.r[1][n], last.r[1][n]);
+    h.r[0][n] = over_chunk(h.r[0][n], mul2(A2.r[0][n], t0), last.r[0][n]);
+    h.r[1][n] = over_chunk(h.r[1][n], mul2(A2.r[1][n], t1), last.r[1][n]);
   }
 }
 __device__ __forceinline__ void load_totals(f32x2& t0, f32x2& t1, const float* row, int c0, int dim) {
@@ -288,7 +296,7 @@ __global__ void __launch_bounds__(32) scan_forward_kernel(const ScanParams p) {
         const int ch = c ? c1 : c0;
         const f32x2 total = both(ch < p.dim ? row[ch] : 0.f);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) h.r[c][i] = fma2(ex2_2(mul2(A2.r[c][i], total)), h.r[c][i], last.r[c][i]);
+        for (int i = 0; i < 2; ++i) h.r[c][i] = over_chunk(h.r[c][i], mul2(A2.r[c][i], total), last.r[c][i]);
       }
     }
   }

@@ -379,3 +379,57 @@ def test_compiled_training_step():
         y = fn({**v, **leaves}, state=False)
         out.append([y.detach(), *torch.autograd.grad(y, list(leaves.values()), dy)])
     assert all(torch.equal(a, b) for a, b in zip(*out))
+
+
+def split_inputs():
+    """Few channels and many tokens, so that both directions take the tokens in chunks."""
+    from spear_b200.ops import _call
+
+    v = inputs(1, 640, 24, 16, torch.float32, gate=False, bias=False, skip=False, initial=True)
+    assert _call.query("btp_sm100_scan_carry_floats", 0, 1, 640, 24, 16) > 0
+    whole = 2 * 640 * 16 + 24 * 18  # dB and dC of one block of channels and the parameters' row of one chunk
+    assert _call.query("btp_sm100_scan_backward_floats", 0, 1, 640, 24, 16) > whole
+    return v
+
+
+def test_chunks_that_would_make_a_state_grow_beyond_a_float():
+    """No state before the last 3 tokens and no gradient behind the first 3: what lies between would multiply either by e^4000."""
+    v = split_inputs()
+    v["A"] = -v["A"].clamp(-2, -1)
+    v["delta"] = torch.full_like(v["delta"], 4.0)
+    v["initial_state"].zero_()
+    v["x"][:, :-3] = 0
+    dy = torch.zeros_like(v["x"])
+    dy[:, :3] = torch.randn(1, 3, 24, device="cuda")
+    names = [n for n in NAMES if v[n] is not None]
+    for n in names:
+        v[n].requires_grad_(True)
+    y, state = run(v, softplus=False)
+    got = dict(zip(names, torch.autograd.grad(y, [v[n] for n in names], dy)))
+    want = oracle(v, softplus=False, dy=dy)
+    check(y.detach(), want["y"], torch.float32, "y")
+    check(state.detach(), want["state"], torch.float32, "state")
+    assert torch.isfinite(y).all() and torch.isfinite(state).all()
+    for n in names:
+        key = "d" + {"initial_state": "initial"}.get(n, n)
+        check(got[n], want[key], torch.float32, key)
+        assert torch.isfinite(got[n]).all(), key
+
+
+def test_chunks_that_shrink_a_large_state_below_a_floats_reach():
+    """1e30 times e^-102 is 5e-15, though e^-102 by itself is no normal float; the same for the final state's gradient."""
+    v = split_inputs()
+    v["A"] = -1.6 + 0.02 * torch.rand(24, 16, device="cuda")
+    v["x"].zero_(), v["delta"].zero_()
+    for at, name in ((5, "state"), (610, "dinitial")):  # 16 tokens inside one chunk of whole 32
+        v["delta"].detach().zero_()[:, at:at + 16] = 4.0
+        v["initial_state"] = torch.full((1, 24, 16), 1e30 if name == "state" else 0.0, device="cuda", requires_grad=True)
+        y, state = run(v, softplus=False)
+        if name == "state":
+            want = oracle(v, softplus=False)
+            check(y.detach(), want["y"], torch.float32, "y")
+            check(state.detach(), want["state"], torch.float32, name)
+        else:
+            ds = torch.full_like(state, 1e30)
+            got, = torch.autograd.grad(state, [v["initial_state"]], ds)
+            check(got, oracle(v, softplus=False, dy=torch.zeros_like(y), dstate=ds)[name], torch.float32, name)
