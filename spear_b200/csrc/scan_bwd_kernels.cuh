@@ -23,7 +23,6 @@
 namespace btp_scan {
 
 constexpr int kStep = 4;  // tokens whose decays and states are in registers at a time
-constexpr float kLn2 = 0.6931471805599453f;
 
 struct ScanBwdParams {
   ScanParams f;             // inputs; y, state unused; carry: [splits - 1][B][dim][N] gradients, then the sums of step sizes
@@ -187,8 +186,8 @@ __global__ void __launch_bounds__(32) scan_backward_carry_kernel(const ScanBwdPa
           const f32x2 cn[4] = {ca.x, ca.y, cc.x, cc.y};
 #pragma unroll
           for (int n = 0; n < 4; ++n) {
-            G.r[0][n] = mul2(ex2_2(mul2(d2.x, A2.r[0][n])), fma2(cn[n], e2.x, G.r[0][n]));
-            G.r[1][n] = mul2(ex2_2(mul2(d2.y, A2.r[1][n])), fma2(cn[n], e2.y, G.r[1][n]));
+            G.r[0][n] = mul2(decay2(d2.x, A2.r[0][n]), fma2(cn[n], e2.x, G.r[0][n]));
+            G.r[1][n] = mul2(decay2(d2.y, A2.r[1][n]), fma2(cn[n], e2.y, G.r[1][n]));
           }
           if (!decltype(usual)::value) clear_padding(G, n0, p.N);
           sum0 = add2(sum0, d2.x);
@@ -341,8 +340,8 @@ __global__ void __launch_bounds__(BwdShape<SG>::kThreads) scan_backward_kernel(c
           const f32x2 bn[4] = {ba.x, ba.y, bb.x, bb.y};
 #pragma unroll
           for (int n = 0; n < 4; ++n) {
-            h.r[0][n] = fma2(ex2_2(mul2(d2.x, A2.r[0][n])), h.r[0][n], mul2(u2.x, bn[n]));
-            h.r[1][n] = fma2(ex2_2(mul2(d2.y, A2.r[1][n])), h.r[1][n], mul2(u2.y, bn[n]));
+            h.r[0][n] = fma2(decay2(d2.x, A2.r[0][n]), h.r[0][n], mul2(u2.x, bn[n]));
+            h.r[1][n] = fma2(decay2(d2.y, A2.r[1][n]), h.r[1][n], mul2(u2.y, bn[n]));
           }
           if (!kFull) clear_padding(h, n0, p.N);
         }
@@ -365,8 +364,8 @@ __global__ void __launch_bounds__(BwdShape<SG>::kThreads) scan_backward_kernel(c
           const f32x2 bn[4] = {ba.x, ba.y, bb.x, bb.y};
 #pragma unroll
           for (int n = 0; n < 4; ++n) {
-            a[j].r[0][n] = ex2_2(mul2(d2.x, A2.r[0][n]));
-            a[j].r[1][n] = ex2_2(mul2(d2.y, A2.r[1][n]));
+            a[j].r[0][n] = decay2(d2.x, A2.r[0][n]);
+            a[j].r[1][n] = decay2(d2.y, A2.r[1][n]);
             w[j].r[0][n] = mul2(a[j].r[0][n], h.r[0][n]);
             w[j].r[1][n] = mul2(a[j].r[1][n], h.r[1][n]);
             h.r[0][n] = fma2(u2.x, bn[n], w[j].r[0][n]);
@@ -472,7 +471,7 @@ __global__ void __launch_bounds__(BwdShape<SG>::kThreads) scan_backward_kernel(c
       }
       const f32x2 ox = fma2(du, *reinterpret_cast<const f32x2*>(&sm.delta[r][c]), mul2(e, skip));
       f32x2 v = fma2(du, xx, mul2(*reinterpret_cast<const f32x2*>(&sm.wa[r][c]), both(kLn2)));
-      if (p.softplus) v = mul2(v, sigmoid2(add2(load_pair(&sm.d[st][r][c]), bias)));
+      if (p.softplus) v = mul2(v, softplus_slope2(add2(load_pair(&sm.d[st][r][c]), bias)));
       store_pair<T>(dx + at, ox, bp.al_out, p.dim - pc);
       store_pair<T>(dd + at, v, bp.al_out, p.dim - pc);
       tile_d = fma2(e, xx, tile_d);

@@ -433,3 +433,54 @@ def test_chunks_that_shrink_a_large_state_below_a_floats_reach():
             ds = torch.full_like(state, 1e30)
             got, = torch.autograd.grad(state, [v["initial_state"]], ds)
             check(got, oracle(v, softplus=False, dy=torch.zeros_like(y), dstate=ds)[name], torch.float32, name)
+
+
+@pytest.mark.parametrize("lo,hi", [(-30, -12), (-12, -7), (-7, -2), (-2, 0), (0, 3), (3, 30)])
+def test_step_sizes_are_accurate_where_they_are_small(lo, hi):
+    """With a rate of -1e30 nothing is remembered, so y is the step size itself and delta's gradient its slope.
+
+    Relative to 64 bits, u = 2^-24: e^-|v| two units of the special-function unit (4u) and a rounding; the polynomial of
+    log(1 + w) 1e-7 as evaluated, its product or sum one rounding.  The slope: e^-|v| as before, 1 + w one rounding, its
+    reciprocal a unit (2u), two products, and the state's gradient exactly 1."""
+    n, u = 40000, 2.0 ** -24
+    v = torch.linspace(lo, hi, n, device="cuda").view(1, n, 1).requires_grad_(True)
+    one = torch.ones(1, n, 1, device="cuda")
+    from spear_b200.ops.ssm import selective_scan
+
+    y = selective_scan(one, v, torch.full((1, 1), -1e30, device="cuda"), one, one, delta_softplus=True)
+    slope, = torch.autograd.grad(y, v, one)
+    v64 = v.detach().double()
+    want = torch.logaddexp(v64, torch.zeros_like(v64))
+    assert ((y.detach().double() - want).abs() <= (6 * u + 1e-7) * want).all()
+    want = torch.exp(v64 - want)
+    assert ((slope.double() - want).abs() <= 10 * u * want).all()
+
+
+@pytest.mark.parametrize("way", ["prompt", "chunks", "token", "gradient"])
+def test_decays_are_not_off_in_one_direction(way):
+    """The product of 4096 decays between 0.98 and 0.998.  A factor's own rounding is random: 4e-8 rms for the special-function
+    unit's result and 2e-8 for the product, five deviations of their sum are 5 * sqrt(4096) * 5e-8.  On average a factor may be off by
+    4e-9 (the unit alone is low by 2e-8, 8e-5 for the product).  The rate to the base 2 is rounded twice: 2u of the exponent."""
+    from spear_b200.ops import _call
+    from spear_b200.ops.ssm import selective_scan, selective_scan_step
+
+    L, u = 4096, 2.0 ** -24
+    B, D = (1, 8) if way == "chunks" else (64, 512)  # enough warps for all tokens in one piece, or few and so in chunks
+    assert (_call.query("btp_sm100_scan_carry_floats", 0, B, L, D, 4) > 0) == (way == "chunks")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    dt = 0.002 + 0.018 * torch.rand(B, L, D, generator=g, device="cuda")
+    A = torch.full((D, 4), -1.0, device="cuda")
+    z, zn = torch.zeros(B, L, D, device="cuda"), torch.zeros(B, L, 4, device="cuda")
+    one = torch.ones(B, D, 4, device="cuda")
+    if way in ("prompt", "chunks"):
+        got = selective_scan(z, dt, A, zn, zn, initial_state=one, return_state=True)[1]
+    elif way == "token":
+        got = one.clone()
+        for t in range(L):
+            selective_scan_step(z[:, t], dt[:, t], A, zn[:, t], zn[:, t], got, state_out=got)
+    else:
+        start = one.clone().requires_grad_(True)
+        got, = torch.autograd.grad(selective_scan(z, dt, A, zn, zn, initial_state=start, return_state=True)[1], start, one)
+    total = dt.double().sum(1)[..., None].expand(B, D, 4)
+    rel = got.double() / torch.exp(-total) - 1
+    assert (rel.abs() <= 4e-9 * L + 5 * L ** 0.5 * 5e-8 + 2 * u * total).all(), rel.abs().max()
