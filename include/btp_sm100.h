@@ -255,7 +255,7 @@ int btp_sm100_causal_conv_partial_rows(int B, int L, int dim);
  * Backward of btp_sm100_causal_conv_forward, for gradients dy of y and dstate of state (NULL: none).
  *   dy, dx [B, L, dim] x's type, dense (dx is 0 from lengths[b] on);  dstate, dinitial [B, width-1, dim] x's type, dense
  *   dweight [dim, width], dbias [dim] weight's type, either NULL; partial: scratch of
- *   btp_sm100_causal_conv_partial_rows(B, L, dim) * (width + 1) * dim floats, needed for either of the two.
+ *   btp_sm100_causal_conv_partial_rows(B, L, dim) * (width + 1) * dim floats, 8-byte aligned, needed for either of the two.
  * Sums are taken in a fixed order.
  */
 int btp_sm100_causal_conv_backward(const void* x, const void* weight, const void* bias, const void* initial, const int* lengths,

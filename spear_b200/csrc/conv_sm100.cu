@@ -107,6 +107,7 @@ int btp_sm100_causal_conv_backward(const void* x, const void* weight, const void
   if (rc) return rc;
   if (!x || !weight || !dy || !dx) return fail(BTP_ERR_NULL_POINTER, "%s: x, weight, dy and dx must not be NULL", fn);
   if ((dweight || dbias) && !partial) return fail(BTP_ERR_NULL_POINTER, "%s: dweight and dbias need the partial sums", fn);
+  if (partial && (reinterpret_cast<uintptr_t>(partial) & 7u)) return fail(BTP_ERR_MISALIGNED, "%s: the partial sums must be 8-byte aligned", fn);
   if (sx_b < 0 || sx_t < 0) return fail(BTP_ERR_BAD_SHAPE, "%s: strides must not be negative", fn);
   int dev;
   DeviceInfo info;

@@ -121,3 +121,13 @@ def test_sizes_beyond_32_bits_are_refused_not_cut_off(B, L, D):
     if L == 1:
         with pytest.raises(ValueError, match="below 2\\^31"):
             causal_conv_step(E(B, D), E(B, 3, D), E(D, 4))
+
+
+def test_entry_refuses_partial_sums_that_it_cannot_store_in_pairs():
+    from spear_b200 import _lib
+
+    lib = _lib.load()
+    p = ctypes.c_void_p(16)
+    for at in (20, 17):
+        rc = lib.btp_sm100_causal_conv_backward(p, p, None, None, None, p, None, p, p, None, None, ctypes.c_void_p(at), 1, 4, 8, 4, 32, 8, 0, 0, 0, None)
+        assert rc == -5 and "8-byte" in lib.btp_sm100_last_error().decode()
