@@ -208,7 +208,7 @@ int btp_sm100_prefill_state(const void* a, const void* x, void* h_loc, void* r_p
  *   out_mode  BTP_NORM_SAME    y [rows, dim] in x's type, dense; scale may be NULL
  *             BTP_NORM_ROW8    y [rows, dim] e4m3 bytes, scale [rows] float: max|y| / 448 of the row
  *             BTP_NORM_BLOCK8  y [rows, dim] e4m3 bytes, scale [rows, ceil(dim/128)]: the same per 128 columns
- *             The stored byte is e4m3(y / scale), rounded to nearest even; the scale is 1 where the maximum is
+ *             The stored byte is e4m3(y / scale) of the float32 quotient, rounded to nearest even; the scale is 1 where the maximum is
  *             NaN, 0 or so small that the scale would be below 1e-37.
  */
 #define BTP_NORM_SAME 0

@@ -159,7 +159,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, residual: torc
     Args:
         x: [..., D] bfloat16, float16 or float32, D <= 16384; the last dimension is copied to be dense if it is not.
         weight: [D] in x's dtype or float32, or None for ones.
-        residual: [..., D] in x's dtype or float32 (a residual stream kept in 32 bits), or None.
+        residual: [..., D] in x's dtype or float32 (a residual stream kept in 32 bits), or None.  Gradients are taken of
+            the sum as it is stored, so a float16 stream must stay below 65504: a sum beyond that is stored as infinity,
+            and its row's gradients and its column of the weight's are lost, though y is right.
         eps: added to the mean square.
     Returns:
         y [..., D] in x's dtype; with a residual (y, h) where h = x + residual in the residual's dtype.  y is the

@@ -298,3 +298,58 @@ def test_compiled_and_repeatable():
     leaves = [v[n].clone().requires_grad_(True) for n in ("x", "weight", "bias")]
     y = torch.compile(causal_conv, backend="aot_eager")(*leaves, activation="silu")
     assert all(torch.equal(a, b) for a, b in zip(runs[0], torch.autograd.grad(y, leaves, torch.ones_like(y))))
+
+
+# sequences x channels enough for runs of many tiles, so that the ring of three is gone through many times
+@pytest.mark.parametrize("shape", [(8, 1500, 2056), (16, 2999, 1024)], ids=str)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("padded", [False, True])
+def test_long_runs(shape, dtype, padded):
+    from spear_b200.ops.ssm import causal_conv
+
+    B, L, D = shape
+    W = 4
+    v = inputs(B, L, D, W, dtype, initial=True, lengths=padded, seed=6)
+    if padded:
+        v["lengths"][1], v["lengths"][2] = L, L - 1
+    dy = torch.randn(B, L, D, generator=torch.Generator(device="cuda").manual_seed(7), device="cuda").to(dtype)
+    names = ("x", "weight", "bias", "initial_state")
+    for n in names:
+        v[n].requires_grad_(True)
+    y, state = causal_conv(v["x"], v["weight"], v["bias"], activation="silu", initial_state=v["initial_state"], lengths=v["lengths"],
+                           return_state=True)
+    got = dict(zip(names, torch.autograd.grad(y, [v[n] for n in names], dy)))
+    h = half(dtype)
+    for b in range(B):  # sequence by sequence: 64 bits of all of them are tens of GB
+        one = {k: (t if k in ("weight", "bias") else None if t is None else t[b:b + 1]) for k, t in v.items()}
+        w64 = {k: t.requires_grad_(True) if k in names else t for k, t in as64(one).items()}
+        yw, sw, pre, mag = reference(w64, True)
+        tol = (W + 1) * U * mag * 1.1 + (pre.abs() + 4) * 2 * U * yw.abs()  # silu's slope is at most 1.1
+        assert ((y[b:b + 1].double() - yw).abs() <= tol + h * (yw.abs() + tol) + tiny(dtype)).all(), b
+        assert torch.equal(state[b:b + 1], sw.to(dtype)), b
+        dx, dw, db, di = torch.autograd.grad(yw, [w64[n] for n in names], dy[b:b + 1].double())
+        # e = dy act'(pre): act' is off by 2 (|pre| + 4) u twice and by half of the pre-activation's error, its second derivative's bound;
+        # a gradient is the sum of W such terms
+        off = dy[b:b + 1].double().abs() * (4 * (pre.abs() + 4) * U + 0.5 * (W + 1) * U * mag)
+        if v["lengths"] is not None:
+            off = off * (torch.arange(L, device="cuda")[None, :, None] < v["lengths"][b])
+        w = v["weight"].detach().double().abs()
+        ahead = torch.cat([off, off.new_zeros(1, W - 1, D)], 1)
+        size = torch.cat([dy[b:b + 1].double().abs() * 1.1, off.new_zeros(1, W - 1, D)], 1)
+        tol = sum(w[:, k] * (ahead + (W + 1) * U * size)[:, W - 1 - k:W - 1 - k + L] for k in range(W))
+        assert ((got["x"][b:b + 1].double() - dx).abs() <= tol + h * (dx.abs() + tol) + tiny(dtype)).all(), b
+        if b == 0:
+            sums = [dw.clone(), db.clone()]
+        else:
+            sums[0] += dw
+            sums[1] += db
+    # one thread adds up a run, one strand of eight the runs: at most 3000 + 300 roundings, and each term is off as above; the terms'
+    # magnitudes are at most those of dy 1.1 times |xx|
+    x = v["x"].detach().double().abs()
+    live = 1.0 if v["lengths"] is None else (torch.arange(L, device="cuda")[None, :] < v["lengths"][:, None]).double()[..., None]
+    weight = dy.double().abs() * live * (1.1 * 3300 * U + 60 * U)
+    size_b = weight.sum((0, 1))
+    xmax = x.amax((0, 1)).maximum(v["initial_state"].detach().double().abs().amax((0, 1)))
+    assert ((got["bias"].double() - sums[1]).abs() <= size_b + h * (sums[1].abs() + size_b)).all()
+    tol = (size_b * xmax)[:, None]
+    assert ((got["weight"].double() - sums[0]).abs() <= tol + h * (sums[0].abs() + tol)).all()

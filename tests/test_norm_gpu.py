@@ -289,3 +289,87 @@ def test_compiled():
         leaves = [t.clone().requires_grad_(True) for t in (x, w, r)]
         out.append(torch.autograd.grad(list(fn(*leaves)), leaves, [dy, dh]))
     assert all(torch.equal(a, b) for a, b in zip(*out))
+
+
+# several rows per warp or CTA, with a remainder: a row per warp, per CTA of one, two and four runs of columns per thread
+TURNS = [(20001, 40), (20003, 256), (5003, 520), (3001, 2048), (2003, 4104), (701, 8200), (603, 16384)]
+
+
+@pytest.mark.parametrize("shape", TURNS, ids=str)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("residual", ["same", torch.float32])
+def test_rows_in_turn(shape, dtype, residual):
+    """Every row against 64 bits where a warp or CTA takes many of them: the next row fetched ahead, the slots of the sums in turn,
+    the weight's gradient over all of a group's rows."""
+    from spear_b200.ops.norm import rms_norm, rms_norm_8bit
+
+    res = dtype if residual == "same" else residual
+    x, w, r = inputs(shape, dtype, res, torch.float32, seed=3)
+    y, h = rms_norm(x, w, r)
+    check_forward(x, w, r, y, h)
+    check_forward(x, w, None, rms_norm(x, w), None)
+    _, _, yw = reference(x, w, r)
+    for block in (None, 128):
+        q, scale, h8 = rms_norm_8bit(x, w, r, block=block)
+        width = shape[-1] if block is None else block
+        tops = torch.stack([p.abs().amax(-1) for p in yw.split(width, -1)], -1) / 448.0
+        got = scale.unsqueeze(-1) if block is None else scale
+        assert ((got.double() - tops).abs() <= 44 * U * tops).all() and torch.equal(h8, h)
+        spread = got.double().repeat_interleave(width, -1)[:, : shape[-1]]
+        assert ((q.double() * spread - yw).abs() <= (2.0 ** -4 + 90 * U) * yw.abs() + (2.0 ** -10 + 90 * U) * spread).all()
+    g = torch.Generator(device="cuda").manual_seed(4)
+    dy = torch.randn(*shape, generator=g, device="cuda").to(dtype)
+    dh = torch.randn(*shape, generator=g, device="cuda").to(res)
+    leaves = [t.requires_grad_(True) for t in (x, w, r)]
+    dx, dw, dr = torch.autograd.grad(list(rms_norm(x, w, r)), leaves, [dy, dh])
+    with torch.no_grad():
+        stored = half(res)
+        d, mag, want, size = gradients(x, w, r, dy, dh, x.double() + r.double())
+        tol = (2.1 * stored + 160 * U) * mag
+        assert ((dx.double() - d).abs() <= tol + half(dtype) * (d.abs() + tol) + tiny(dtype)).all()
+        assert ((dr.double() - d).abs() <= tol + half(res) * (d.abs() + tol) + tiny(res)).all()
+        # a group adds up its rows one by one (at most 20 here), 32 strands the groups' sums (at most 150 each), then the strands
+        assert ((dw.double() - want).abs() <= (1.1 * stored + (50 + 20 + 150 + 32) * U) * size).all()
+
+
+@pytest.mark.parametrize("block", [None, 128])
+def test_8bit_values_are_the_rounded_quotients(block):
+    """q is e4m3(y / scale), bit for bit, with y as rms_norm returns it in float32 and the quotient rounded to float32: on values at the
+    borders between two e4m3 numbers and up to 3 steps of float32 beside them, where a product with the reciprocal goes astray."""
+    from spear_b200.ops.norm import rms_norm, rms_norm_8bit
+
+    f8 = torch.arange(1, 127, device="cuda", dtype=torch.uint8).view(torch.float8_e4m3fn).double()  # 2^-9 ... 448
+    borders = (f8[1:] + f8[:-1]) / 2
+    dim = 16384
+    width = 128 if block else dim
+    x = torch.ones(1, dim, device="cuda")  # rstd is one number, and the weight sets y
+    for seed in range(20):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        top = torch.exp(4 * torch.randn(dim // width, 1, generator=g, device="cuda", dtype=torch.float64))
+        pick = borders[torch.randint(0, len(borders), (dim // width, width), generator=g, device="cuda")]
+        aside = torch.randint(-3, 4, pick.shape, generator=g, device="cuda").double() * 2.0 ** -23
+        sign = torch.randint(0, 2, pick.shape, generator=g, device="cuda").double() * 2 - 1
+        target = top / 448 * pick * (1 + aside) * sign
+        target[:, 5] = top[:, 0]  # the largest of each scale's columns
+        w = target.view(dim).float()
+        y = rms_norm(x, w)
+        q, scale = rms_norm_8bit(x, w, block=block)
+        want = (y.view(-1, width) / scale.view(-1, 1)).to(torch.float8_e4m3fn).view(1, dim)
+        assert torch.equal(q.view(torch.uint8), want.view(torch.uint8)), seed
+
+
+def test_a_float16_stream_beyond_its_range():
+    """A float16 sum above 65504 is stored as infinity, which the output does not see and the backward pass does: it reads the sum as
+    stored.  Only that row's gradients and that column of the weight's are lost."""
+    from spear_b200.ops.norm import rms_norm
+
+    x, w, r = inputs((4, 64), torch.float16, torch.float16, torch.float32)
+    x[2, 7] = r[2, 7] = 60000.0
+    leaves = [t.requires_grad_(True) for t in (x, w, r)]
+    y, h = rms_norm(x, w, r)
+    assert h[2, 7].isinf() and torch.isfinite(y).all()
+    with torch.no_grad():
+        check_forward(x[:2], w, r[:2], y[:2], h[:2])
+    dx, dw, _ = torch.autograd.grad([y, h], leaves, [torch.ones_like(y), torch.ones_like(h)])
+    keep = torch.arange(64, device="cuda") != 7
+    assert torch.isfinite(dx[[0, 1, 3]]).all() and torch.isfinite(dw[keep]).all() and not torch.isfinite(dw[7])
