@@ -48,7 +48,8 @@ int backward_grid(long long rows, const Shape& s, int sms) {
 
 template <class T, int RES, int OUT, int VPT>
 cudaError_t launch_fwd(const FwdParams& p, const Shape& s, cudaStream_t stream) {
-  if (s.warp_row) return launch_kernel(rms_norm_forward_kernel<T, RES, OUT, VPT, true>, s.grid, 128, 0, stream, p);
+  if constexpr (VPT == 1)  // a row of one warp has one run per thread
+    if (s.warp_row) return launch_kernel(rms_norm_forward_kernel<T, RES, OUT, VPT, true>, s.grid, 128, 0, stream, p);
   return launch_kernel(rms_norm_forward_kernel<T, RES, OUT, VPT, false>, s.grid, s.threads, 0, stream, p);
 }
 template <class T, int RES, int OUT>
@@ -62,7 +63,8 @@ cudaError_t launch_fwd_o(const FwdParams& p, const Shape& s, int out, cudaStream
 }
 template <class T, int RES, int VPT>
 cudaError_t launch_bwd(const BwdParams& p, const Shape& s, int grid, cudaStream_t stream) {
-  if (s.warp_row) return launch_kernel(rms_norm_backward_kernel<T, RES, VPT, true>, grid, 128, 0, stream, p);
+  if constexpr (VPT == 1)
+    if (s.warp_row) return launch_kernel(rms_norm_backward_kernel<T, RES, VPT, true>, grid, 128, 0, stream, p);
   return launch_kernel(rms_norm_backward_kernel<T, RES, VPT, false>, grid, s.threads, 0, stream, p);
 }
 template <class T, int RES>

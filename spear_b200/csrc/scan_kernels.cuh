@@ -70,11 +70,9 @@ struct Tile {
   T x[2][kTile][kChannels];
   T d[2][kTile][kChannels];
   T z[2][kTile][kChannels];
-  T B[2][kTile][kStates];
   T C[2][kTile][kStates];
   float delta[kTile][kChannels];
   float u[kTile][kChannels];
-  float B2[kTile][kStates * 2];
   float C2[kTile][kStates * 2];
 };
 

@@ -229,6 +229,7 @@ int btp_sm100_scan_backward(const void* x, const void* delta, const float* A, co
     rc = launched(fn, dispatch(dtype, N, [&](auto tag, auto groups) {
       using T = decltype(tag);
       constexpr int SG = decltype(groups)::value;
+      static_assert(sizeof(Tile<T, SG>) <= 48 * 1024, "fits without a larger limit");
       return launch_kernel(scan_backward_carry_kernel<T, SG>, static_cast<int>(warps), 32, static_cast<int>(sizeof(Tile<T, SG>)), st, bp);
     }));
     if (rc) return rc;
