@@ -8,11 +8,13 @@ status a RuntimeError carries the library's own message.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libbtp_sm100.so")
+MODULE_PATH = os.path.join(_HERE, "lib", "btp_torch.so")
 
 # dtype tags of include/btp_sm100.h
 DTYPE_BF16 = 0
@@ -62,6 +64,7 @@ SYMBOLS = {
 
 _lock = threading.Lock()
 _lib = None
+_module = None
 
 
 class BtpLibraryError(RuntimeError):
@@ -92,6 +95,24 @@ def load() -> ctypes.CDLL:
             )
         _lib = lib
     return _lib
+
+
+def native():
+    """The module with the token-major operators on torch tensors, linked to the library.  Loaded once, never built here."""
+    global _module
+    if _module is None:
+        load()
+        if not os.path.exists(MODULE_PATH):
+            raise BtpLibraryError(f"{MODULE_PATH} is missing. Build it with `python -m spear_b200.build`.")
+        import torch  # noqa: F401  (the module is linked to its libraries)
+
+        with _lock:
+            if _module is None:
+                spec = importlib.util.spec_from_file_location("btp_torch", MODULE_PATH)
+                module = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(module)
+                _module = module
+    return _module
 
 
 def check(status: int, what: str) -> None:

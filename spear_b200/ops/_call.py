@@ -15,7 +15,8 @@ from .. import _lib
 TAG = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16, torch.float32: _lib.DTYPE_F32}
 
 
-_current_device, _raw_stream = _native._current_device, _native._raw_stream
+# a call has CUDA tensors, so CUDA is initialised and the plain lookup will do
+_current_device, _raw_stream = getattr(torch._C, "_cuda_getDevice", _native._current_device), _native._raw_stream
 _fns: dict = {}  # the library's functions by name, looked up once
 
 
@@ -24,15 +25,12 @@ def _entry(name: str):
     return fn
 
 
-def activation(t: torch.Tensor, what: str) -> None:
+def activation(what: str, name: str, t: torch.Tensor) -> None:
+    """A type that the kernels read, and sizes that fit: the C entries take 32 bits, and ctypes would cut a larger one off without a word."""
     if t.dtype not in TAG:
-        raise RuntimeError(f"{what} must be bfloat16, float16 or float32 (got {t.dtype})")
-
-
-def sizes(what: str, shape) -> None:
-    """The C entries take 32-bit sizes, and ctypes would cut a larger one off without a word."""
-    if max(shape) > 0x7FFFFFFF:
-        raise ValueError(f"{what}: every size must be below 2^31, got {tuple(shape)}")
+        raise RuntimeError(f"{what}: {name} must be bfloat16, float16 or float32 (got {t.dtype})")
+    if t.numel() > 0x7FFFFFFF and max(t.shape) > 0x7FFFFFFF:
+        raise ValueError(f"{what}: every size must be below 2^31, got {tuple(t.shape)}")
 
 
 def on_gpu(what: str, first: torch.Tensor, *others) -> int:
@@ -102,20 +100,36 @@ def pass_on(into: torch.Tensor | None, given: torch.Tensor | None) -> None:
         into.zero_() if given is None else into.copy_(given)
 
 
-_modes, _tracing = torch._C._len_torch_dispatch_stack, torch._C._get_tracing_state
+_modes, _tracing = torch._C._len_torch_dispatch_stack, torch._C._is_tracing
 _DIRECT = frozenset((torch.Tensor, torch.nn.Parameter, type(None), bool, int, float))
 
 
+_compiling = torch.compiler.is_compiling
+
+
+def recorded(*args) -> bool:
+    """Whether somebody records or interprets a call with these arguments: torch.compile, make_fx and other dispatch modes,
+    torch.jit.trace, a tensor subclass."""
+    return _compiling() or _modes() > 0 or _tracing() or not _DIRECT.issuperset(map(type, args))
+
+
+def training(*tensors) -> bool:
+    """Whether the call takes an autograd node (always while torch.compile traces: it may add gradients later)."""
+    return _compiling() or (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors))
+
+
+native = _lib.native
+
+
 def traceable(name: str, direct):
-    """The registered op `spear_btp::name` where somebody records or interprets the call (torch.compile, make_fx and other dispatch
-    modes, torch.jit.trace, a tensor subclass), the function `direct` otherwise (the dispatcher takes longer than a small launch).
+    """The registered op `spear_btp::name` where somebody records the call, the function `direct` otherwise (the dispatcher takes
+    longer than a small launch).
 
     A recorded op is replayed on tensors that no public function has looked at, so the op itself checks its arguments."""
     op = getattr(torch.ops.spear_btp, name)
-    compiling = torch.compiler.is_compiling
 
     def run(*args):
-        if compiling() or _modes() or _tracing() is not None or not _DIRECT.issuperset(map(type, args)):
+        if recorded(*args):
             op(*args)
         else:
             direct(*args)

@@ -27,7 +27,7 @@ _OUT = {None: 1, SCALE_BLOCK: 2}
 def _check(what, x, weight, residual, eps) -> int:
     if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_DIM:
         raise ValueError(f"{what}: x must be [..., D] with 1 <= D <= {MAX_DIM}, got {tuple(x.shape)}")
-    _call.activation(x, f"{what}: x")
+    _call.activation(what, "x", x)
     if weight is not None:
         if weight.shape != x.shape[-1:]:
             raise ValueError(f"{what}: weight must be [{x.shape[-1]}], got {tuple(weight.shape)}")
@@ -117,11 +117,14 @@ def _fake(*args) -> None:
 
 _iface._register(_iface._LIB, "spear_btp", "rms_norm_forward", _op_forward, _fake, ["y", "h", "rstd", "scale"])
 _iface._register(_iface._LIB, "spear_btp", "rms_norm_backward", _op_backward, _fake, ["dx", "dresidual", "dweight"])
+_op = torch.ops.spear_btp.rms_norm_forward
 _forward = _call.traceable("rms_norm_forward", _launch_forward)
 _backward = _call.traceable("rms_norm_backward", _launch_backward)
 
 
 class _RMSNorm(torch.autograd.Function):
+    """The training pass where it is recorded; otherwise the same steps run in C++ (csrc/btp_torch.cpp)."""
+
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
         x2 = _rows(x)
@@ -167,18 +170,20 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, residual: torc
         y [..., D] in x's dtype; with a residual (y, h) where h = x + residual in the residual's dtype.  y is the
         norm of the sum before that rounding.  Both outputs have gradients.
     """
-    index = _check("rms_norm", x, weight, residual, eps)
-    weight = weight if weight is None or weight.is_contiguous() else weight.contiguous()
-    if torch.compiler.is_compiling() or (torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (x, weight, residual))):
+    _check("rms_norm", x, weight, residual, eps)
+    weight = _call.dense(weight)
+    if not _call.recorded(x, weight, residual):
+        y, h = _call.native().rms_norm(x, weight, residual, float(eps))
+        return y if h is None else (y, h)
+    if _call.training(x, weight, residual):
         return _RMSNorm.apply(x, weight, residual, float(eps))
     x2 = _rows(x)
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
     if residual is None:
-        _forward(x2, None, weight, y, None, None, float(eps))
+        _op(x2, None, weight, y, None, None, float(eps))
         return y
     h = torch.empty_like(residual, memory_format=torch.contiguous_format)
-    _forward(x2, _rows(residual), weight, y, h, None, float(eps))
+    _op(x2, _rows(residual), weight, y, h, None, float(eps))
     return y, h
 
 
@@ -202,5 +207,6 @@ def rms_norm_8bit(x: torch.Tensor, weight: torch.Tensor | None = None, residual:
     q = torch.empty_like(x, dtype=torch.float8_e4m3fn, memory_format=torch.contiguous_format)
     scale = x.new_empty(x.shape[:-1] if block is None else (*x.shape[:-1], -(-x.shape[-1] // SCALE_BLOCK)), dtype=torch.float32)
     h = None if residual is None else torch.empty_like(residual, memory_format=torch.contiguous_format)
-    _forward(x2, None if residual is None else _rows(residual), weight, q, h, None, float(eps), scale, _OUT[block])
+    launch = _op if _call.recorded(x, weight, residual) else _launch_forward
+    launch(x2, None if residual is None else _rows(residual), weight, q, h, None, float(eps), scale, _OUT[block])
     return (q, scale) if h is None else (q, scale, h)

@@ -50,8 +50,7 @@ def _check(what, x, weight, bias, activation, initial, lengths) -> tuple[int, in
     if x.dim() != 3 or x.shape[2] < 1:
         raise ValueError(f"{what}: x must be [B, L, D], got {tuple(x.shape)}")
     B, L, D = x.shape
-    _call.activation(x, f"{what}: x")
-    _call.sizes(what, x.shape)
+    _call.activation(what, "x", x)
     W = _check_filter(what, D, x.dtype, weight, bias, activation)
     if initial is not None:
         if tuple(initial.shape) != (B, W - 1, D):
@@ -67,8 +66,7 @@ def _check_step(what, x_t, state, weight, bias, activation) -> int:
     if x_t.dim() != 2 or x_t.shape[1] < 1:
         raise ValueError(f"{what}: x_t must be [B, D], got {tuple(x_t.shape)}")
     B, D = x_t.shape
-    _call.activation(x_t, f"{what}: x_t")
-    _call.sizes(what, x_t.shape)
+    _call.activation(what, "x_t", x_t)
     W = _check_filter(what, D, x_t.dtype, weight, bias, activation)
     if state.shape != (B, W - 1, D) or state.dtype != x_t.dtype or not state.is_contiguous():
         raise ValueError(f"{what}: state must be contiguous {(B, W - 1, D)} of x_t's dtype, got {state.dtype} {tuple(state.shape)}")
@@ -168,10 +166,12 @@ _iface._register(_iface._LIB, "spear_btp", "causal_conv_backward", _op_backward,
 _iface._register(_iface._LIB, "spear_btp", "causal_conv_step", _op_step, _fake, ["y", "state_out"])
 _forward = _call.traceable("causal_conv_forward", _launch_forward)
 _backward = _call.traceable("causal_conv_backward", _launch_backward)
-_step = _call.traceable("causal_conv_step", _launch_step)
+_op, _token_op = torch.ops.spear_btp.causal_conv_forward, torch.ops.spear_btp.causal_conv_step
 
 
 class _CausalConv(torch.autograd.Function):
+    """The training pass where it is recorded; otherwise the same steps run in C++ (csrc/btp_torch.cpp)."""
+
     @staticmethod
     def forward(ctx, x, weight, bias, initial, lengths, silu, want_state):
         B, L, D = x.shape
@@ -226,19 +226,21 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None
     x, weight, bias = dense_last(x), dense(weight), dense(bias)
     initial_state, lengths = dense(initial_state), dense(lengths)
     silu = activation == "silu"
-    if torch.compiler.is_compiling() or (torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (x, weight, bias, initial_state))):
+    if not _call.recorded(x, weight, bias, initial_state, lengths):
+        y, state = _call.native().causal_conv(x, weight, bias, initial_state, lengths, silu, bool(return_state))
+        return (y, state) if return_state else y
+    if _call.training(x, weight, bias, initial_state):
         return _CausalConv.apply(x, weight, bias, initial_state, lengths, silu, bool(return_state))
     y = x.new_empty((B, L, D))
     state = x.new_empty((B, W - 1, D)) if return_state else None
-    _forward(x, weight, bias, initial_state, lengths, y, state, silu)
+    _op(x, weight, bias, initial_state, lengths, y, state, silu)
     return (y, state) if return_state else y
 
 
 def check_state_out(what, state, state_out) -> torch.Tensor:
     """Where the new state goes: fresh memory, or the caller's tensor, which may be the old state itself."""
     if state_out is None:
-        return torch.empty_like(state, memory_format=torch.contiguous_format)
+        return torch.empty_like(state)  # contiguous, as the state is
     if state_out.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{what}: state_out requires grad, and a token has no gradient: detach it, or call under torch.no_grad()")
     if state_out is state:
@@ -251,9 +253,9 @@ def check_state_out(what, state, state_out) -> torch.Tensor:
     return state_out
 
 
-def written(state_out: torch.Tensor | None) -> None:
+def written(state_out: torch.Tensor) -> None:
     """Tells autograd that the caller's tensor has changed, so that a backward pass that needs its old values fails."""
-    if state_out is not None and not torch.compiler.is_compiling() and not state_out.is_inference():
+    if not torch.compiler.is_compiling() and not state_out.is_inference():
         torch.autograd.graph.increment_version(state_out)
 
 
@@ -267,9 +269,15 @@ def causal_conv_step(x_t: torch.Tensor, state: torch.Tensor, weight: torch.Tenso
     """
     what = "causal_conv_step"
     _check_step(what, x_t, state, weight, bias, activation)
-    out = check_state_out(what, state, state_out)
-    y = torch.empty_like(x_t, memory_format=torch.contiguous_format)
-    if x_t.shape[0]:
-        _step(x_t, state, weight, bias, y, out, activation is not None)
-        written(state_out)
-    return y, out
+    if state_out is not None:
+        check_state_out(what, state, state_out)
+    if not _call.recorded(x_t, state, weight, bias, state_out):
+        y, out = _call.native().causal_conv_step(x_t, state, weight, bias, state_out, activation is not None)
+    else:
+        out = check_state_out(what, state, state_out)
+        y = torch.empty_like(x_t, memory_format=torch.contiguous_format)
+        _token_op(x_t, state, weight, bias, y, out, activation is not None)
+    if state_out is None:
+        return y, out
+    written(state_out)
+    return y, state_out

@@ -47,9 +47,12 @@ def _check_params(what, dim, A, D, delta_bias) -> int:
     return shape[1]
 
 
-def _check_tokens(what, x, others) -> None:
-    dtype = x.dtype
-    for t, name, shape in others:
+def _check_tokens(what, x, delta, z, B, C, states, at="") -> None:
+    dtype, shape = x.dtype, x.shape
+    if (delta.shape == shape and B.shape == states and C.shape == states and delta.dtype == dtype and B.dtype == dtype and C.dtype == dtype
+            and (z is None or (z.shape == shape and z.dtype == dtype))):
+        return
+    for t, name, shape in ((delta, "delta" + at, shape), (z, "z" + at, shape), (B, "B" + at, states), (C, "C" + at, states)):
         if t is None:
             continue
         if t.shape != shape:
@@ -63,10 +66,9 @@ def _check(what, x, delta, A, B, C, D, z, delta_bias, initial, lengths) -> tuple
     if x.dim() != 3 or x.shape[2] < 1:
         raise ValueError(f"{what}: x must be [B, L, D], got {tuple(x.shape)}")
     Bsz, L, dim = x.shape
-    _call.activation(x, f"{what}: x")
-    _call.sizes(what, x.shape)
+    _call.activation(what, "x", x)
     N = _check_params(what, dim, A, D, delta_bias)
-    _check_tokens(what, x, ((delta, "delta", (Bsz, L, dim)), (z, "z", (Bsz, L, dim)), (B, "B", (Bsz, L, N)), (C, "C", (Bsz, L, N))))
+    _check_tokens(what, x, delta, z, B, C, (Bsz, L, N))
     if initial is not None and (tuple(initial.shape) != (Bsz, dim, N) or initial.dtype != torch.float32):
         raise ValueError(f"{what}: initial_state must be float32 {(Bsz, dim, N)}, got {initial.dtype} {tuple(initial.shape)}")
     check_lengths(what, lengths, Bsz)
@@ -78,10 +80,9 @@ def _check_step(what, x_t, delta_t, A, B_t, C_t, state, D, z_t, delta_bias) -> i
     if x_t.dim() != 2 or x_t.shape[1] < 1:
         raise ValueError(f"{what}: x_t must be [B, D], got {tuple(x_t.shape)}")
     Bsz, dim = x_t.shape
-    _call.activation(x_t, f"{what}: x_t")
-    _call.sizes(what, x_t.shape)
+    _call.activation(what, "x_t", x_t)
     N = _check_params(what, dim, A, D, delta_bias)
-    _check_tokens(what, x_t, ((delta_t, "delta_t", x_t.shape), (z_t, "z_t", x_t.shape), (B_t, "B_t", (Bsz, N)), (C_t, "C_t", (Bsz, N))))
+    _check_tokens(what, x_t, delta_t, z_t, B_t, C_t, (Bsz, N), "_t")
     if state.shape != (Bsz, dim, N) or state.dtype != torch.float32 or not state.is_contiguous():
         raise ValueError(f"{what}: state must be contiguous float32 {(Bsz, dim, N)}, got {state.dtype} {tuple(state.shape)}")
     return _call.on_gpu(what, x_t, delta_t, A, B_t, C_t, state, D, z_t, delta_bias)
@@ -192,10 +193,12 @@ _iface._register(_iface._LIB, "spear_btp", "scan_backward", _op_backward, _fake,
 _iface._register(_iface._LIB, "spear_btp", "scan_step", _op_step, _fake, ["y", "state_out"])
 _forward = _call.traceable("scan_forward", _launch_forward)
 _backward = _call.traceable("scan_backward", _launch_backward)
-_step = _call.traceable("scan_step", _launch_step)
+_op, _token_op = torch.ops.spear_btp.scan_forward, torch.ops.spear_btp.scan_step
 
 
 class _SelectiveScan(torch.autograd.Function):
+    """The training pass where it is recorded; otherwise the same steps run in C++ (csrc/btp_torch.cpp)."""
+
     @staticmethod
     def forward(ctx, x, delta, A, B, C, D, z, delta_bias, initial, lengths, softplus, want_state):
         Bsz, L, dim = x.shape
@@ -264,12 +267,15 @@ def selective_scan(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: tor
         return y, (x.new_zeros((Bsz, dim, N), dtype=torch.float32) if initial_state is None else initial_state.clone())
     x, delta, B, C, z = dense_last(x), dense_last(delta), dense_last(B), dense_last(C), dense_last(z)
     A, D, delta_bias, initial_state, lengths = dense(A), dense(D), dense(delta_bias), dense(initial_state), dense(lengths)
-    if torch.compiler.is_compiling() or (torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (x, delta, A, B, C, D, z, delta_bias, initial_state))):
-        return _SelectiveScan.apply(x, delta, A, B, C, D, z, delta_bias, initial_state, lengths, bool(delta_softplus), bool(return_state))
+    tensors = (x, delta, A, B, C, D, z, delta_bias, initial_state)
+    if not _call.recorded(*tensors, lengths):
+        y, state = _call.native().selective_scan(*tensors, lengths, bool(delta_softplus), bool(return_state))
+        return (y, state) if return_state else y
+    if _call.training(*tensors):
+        return _SelectiveScan.apply(*tensors, lengths, bool(delta_softplus), bool(return_state))
     y = x.new_empty((Bsz, L, dim))
     state = x.new_empty((Bsz, dim, N), dtype=torch.float32) if return_state else None
-    _forward(x, delta, A, B, C, D, z, delta_bias, initial_state, lengths, y, state, None, bool(delta_softplus))
+    _op(x, delta, A, B, C, D, z, delta_bias, initial_state, lengths, y, state, None, bool(delta_softplus))
     return (y, state) if return_state else y
 
 
@@ -285,9 +291,16 @@ def selective_scan_step(x_t: torch.Tensor, delta_t: torch.Tensor, A: torch.Tenso
     """
     what = "selective_scan_step"
     _check_step(what, x_t, delta_t, A, B_t, C_t, state, D, z_t, delta_bias)
-    out = check_state_out(what, state, state_out)
-    y = torch.empty_like(x_t, memory_format=torch.contiguous_format)
-    if x_t.shape[0]:
-        _step(x_t, delta_t, A, B_t, C_t, state, D, z_t, delta_bias, y, out, bool(delta_softplus))
-        written(state_out)
-    return y, out
+    if state_out is not None:
+        check_state_out(what, state, state_out)
+    tensors = (x_t, delta_t, A, B_t, C_t, state, D, z_t, delta_bias)
+    if not _call.recorded(*tensors, state_out):
+        y, out = _call.native().selective_scan_step(*tensors, state_out, bool(delta_softplus))
+    else:
+        out = check_state_out(what, state, state_out)
+        y = torch.empty_like(x_t, memory_format=torch.contiguous_format)
+        _token_op(*tensors, y, out, bool(delta_softplus))
+    if state_out is None:
+        return y, out
+    written(state_out)
+    return y, state_out

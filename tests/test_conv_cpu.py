@@ -83,10 +83,13 @@ def test_entry_refuses_bad_arguments_before_any_launch():
 @pytest.mark.parametrize("token", ["conv", "scan"])
 def test_autograd_learns_of_a_state_that_is_updated_in_place(monkeypatch, token):
     """A tensor that some graph has saved must not change unseen; a tensor with a gradient of its own is not overwritten."""
+    from types import SimpleNamespace
+
     from spear_b200.ops import _call
     from spear_b200.ops.ssm import selective_scan_step
 
-    monkeypatch.setattr(_call, "call", lambda *args: None)
+    token_call = lambda *args: (torch.empty_like(args[0]), torch.empty_like(state) if args[-2] is None else args[-2])
+    monkeypatch.setattr(_call, "native", lambda: SimpleNamespace(causal_conv_step=token_call, selective_scan_step=token_call))
     monkeypatch.setattr(_call, "on_gpu", lambda what, first, *others: 0)
     if token == "conv":
         state, w = torch.randn(2, 3, 8), torch.nn.Parameter(torch.randn(8, 4))

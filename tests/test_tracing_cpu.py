@@ -61,6 +61,7 @@ def stand_in(monkeypatch):
 
     monkeypatch.setattr(_call, "call", refuse)
     monkeypatch.setattr(_call, "query", refuse)
+    monkeypatch.setattr(_call, "native", lambda: refuse("the module"))
     monkeypatch.setattr(_call, "on_gpu", lambda what, first, *others: first.get_device())
     yield runs
     lib._destroy()
@@ -145,13 +146,8 @@ def test_plain_calls_go_straight_to_the_library(stand_in, case):
     _, fn, make = CALLS[case]
     with pytest.raises(AssertionError, match="past the registered op"):
         fn(*make())
-
-
-def test_functional_transforms_are_refused(stand_in):
-    x = N(4, 8)
-    for call in (lambda: torch.vmap(rms_norm)(x), lambda: torch.func.grad(lambda t: rms_norm(t).sum())(x)):
-        with pytest.raises(RuntimeError):
-            call()
+    with pytest.raises(AssertionError, match="past the registered op"):
+        fn(*(torch.nn.Parameter(t) for t in make()))
 
 
 @pytest.mark.parametrize("case", CALLS, ids=str)

@@ -111,3 +111,16 @@ def test_compiled_token_in_place():
         for _ in range(3):
             assert torch.equal(compiled(*args), step(*other))
             assert all(torch.equal(a, b) for a, b in zip(args, other))
+
+
+def test_functional_transforms_are_refused():
+    """A wrapped tensor has no memory of its own: an error, not a result that the transform does not see."""
+    from spear_b200.ops.norm import rms_norm
+    from spear_b200.ops.ssm import causal_conv, selective_scan_step
+
+    x, w = N(3, 5, 24), N(24, 4)
+    for call in (lambda: torch.vmap(rms_norm)(x), lambda: torch.func.grad(lambda t: rms_norm(t).sum())(x),
+                 lambda: torch.func.grad(lambda t: causal_conv(x, t).sum())(w), lambda: torch.func.jvp(rms_norm, (x,), (x,)),
+                 lambda: torch.vmap(lambda s: selective_scan_step(x[0], x[0], -w, x[0, :, :4], x[0, :, :4], s))(N(2, 5, 24, 4))):
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            call()
