@@ -101,16 +101,18 @@ def pass_on(into: torch.Tensor | None, given: torch.Tensor | None) -> None:
 
 
 _modes, _tracing = torch._C._len_torch_dispatch_stack, torch._C._is_tracing
-_DIRECT = frozenset((torch.Tensor, torch.nn.Parameter, type(None), bool, int, float))
+_PLAIN = frozenset((torch.Tensor, torch.nn.Parameter, type(None)))
 
 
 _compiling = torch.compiler.is_compiling
 
 
-def recorded(*args) -> bool:
-    """Whether somebody records or interprets a call with these arguments: torch.compile, make_fx and other dispatch modes,
-    torch.jit.trace, a tensor subclass."""
-    return _compiling() or _modes() > 0 or _tracing() or not _DIRECT.issuperset(map(type, args))
+def recorded(*tensors) -> bool:
+    """Whether somebody records or interprets a call with these arguments (torch.compile, make_fx and other dispatch modes,
+    torch.jit.trace, a tensor subclass): it then goes through the registered ops `spear_btp::...`.
+
+    A recorded op is replayed on tensors that no public function has looked at, so the ops check their arguments themselves."""
+    return _compiling() or _modes() > 0 or _tracing() or not _PLAIN.issuperset(map(type, tensors))
 
 
 def training(*tensors) -> bool:
@@ -119,19 +121,3 @@ def training(*tensors) -> bool:
 
 
 native = _lib.native
-
-
-def traceable(name: str, direct):
-    """The registered op `spear_btp::name` where somebody records the call, the function `direct` otherwise (the dispatcher takes
-    longer than a small launch).
-
-    A recorded op is replayed on tensors that no public function has looked at, so the op itself checks its arguments."""
-    op = getattr(torch.ops.spear_btp, name)
-
-    def run(*args):
-        if recorded(*args):
-            op(*args)
-        else:
-            direct(*args)
-
-    return run

@@ -117,9 +117,7 @@ def _fake(*args) -> None:
 
 _iface._register(_iface._LIB, "spear_btp", "rms_norm_forward", _op_forward, _fake, ["y", "h", "rstd", "scale"])
 _iface._register(_iface._LIB, "spear_btp", "rms_norm_backward", _op_backward, _fake, ["dx", "dresidual", "dweight"])
-_op = torch.ops.spear_btp.rms_norm_forward
-_forward = _call.traceable("rms_norm_forward", _launch_forward)
-_backward = _call.traceable("rms_norm_backward", _launch_backward)
+_op, _backward_op = torch.ops.spear_btp.rms_norm_forward, torch.ops.spear_btp.rms_norm_backward
 
 
 class _RMSNorm(torch.autograd.Function):
@@ -131,7 +129,7 @@ class _RMSNorm(torch.autograd.Function):
         y = torch.empty_like(x, memory_format=torch.contiguous_format)
         h = None if residual is None else torch.empty_like(residual, memory_format=torch.contiguous_format)
         rstd = x.new_empty(x2.shape[0], dtype=torch.float32)
-        _forward(x2, None if residual is None else _rows(residual), weight, y, h, rstd, eps)
+        _op(x2, None if residual is None else _rows(residual), weight, y, h, rstd, eps)
         ctx.save_for_backward(x2 if h is None else h, weight, rstd)
         ctx.dtype = x.dtype
         ctx.set_materialize_grads(False)
@@ -152,7 +150,7 @@ class _RMSNorm(torch.autograd.Function):
         dres = torch.empty_like(dy, dtype=h.dtype) if need_r and not one else None
         dw = torch.empty_like(weight) if need_w and weight is not None else None
         if dx is not None or dres is not None or dw is not None:
-            _backward(_rows(h), weight, dy, dh, rstd, dx, dres, dw)
+            _backward_op(_rows(h), weight, dy, dh, rstd, dx, dres, dw)
         return dx if need_x else None, dw, (dx if one else dres) if need_r else None, None
 
 

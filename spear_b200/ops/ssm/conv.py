@@ -164,9 +164,8 @@ def _fake(*args) -> None:
 _iface._register(_iface._LIB, "spear_btp", "causal_conv_forward", _op_forward, _fake, ["y", "state"])
 _iface._register(_iface._LIB, "spear_btp", "causal_conv_backward", _op_backward, _fake, ["dx", "dweight", "dbias", "dinitial"])
 _iface._register(_iface._LIB, "spear_btp", "causal_conv_step", _op_step, _fake, ["y", "state_out"])
-_forward = _call.traceable("causal_conv_forward", _launch_forward)
-_backward = _call.traceable("causal_conv_backward", _launch_backward)
-_op, _token_op = torch.ops.spear_btp.causal_conv_forward, torch.ops.spear_btp.causal_conv_step
+_op, _backward_op, _token_op = (torch.ops.spear_btp.causal_conv_forward, torch.ops.spear_btp.causal_conv_backward,
+                                torch.ops.spear_btp.causal_conv_step)
 
 
 class _CausalConv(torch.autograd.Function):
@@ -177,7 +176,7 @@ class _CausalConv(torch.autograd.Function):
         B, L, D = x.shape
         y = x.new_empty((B, L, D))
         state = x.new_empty((B, weight.shape[1] - 1, D)) if want_state else None
-        _forward(x, weight, bias, initial, lengths, y, state, silu)
+        _op(x, weight, bias, initial, lengths, y, state, silu)
         ctx.save_for_backward(x, weight, bias, initial, lengths)
         ctx.silu = silu
         ctx.set_materialize_grads(False)
@@ -196,7 +195,7 @@ class _CausalConv(torch.autograd.Function):
         dw = weight.new_empty(weight.shape) if need_w else None
         db = bias.new_empty(bias.shape) if need_b and bias is not None else None
         di = x.new_empty(initial.shape) if need_i and initial is not None else None
-        _backward(x, weight, bias, initial, lengths, dy, dstate, dx, dw, db, di, ctx.silu)
+        _backward_op(x, weight, bias, initial, lengths, dy, dstate, dx, dw, db, di, ctx.silu)
         return dx if need_x else None, dw, db, di, None, None, None
 
 

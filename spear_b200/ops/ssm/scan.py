@@ -191,9 +191,7 @@ def _fake(*args) -> None:
 _iface._register(_iface._LIB, "spear_btp", "scan_forward", _op_forward, _fake, ["y", "state", "checkpoints"])
 _iface._register(_iface._LIB, "spear_btp", "scan_backward", _op_backward, _fake, ["dx", "ddelta", "dparams", "dB", "dC", "dz", "dinitial"])
 _iface._register(_iface._LIB, "spear_btp", "scan_step", _op_step, _fake, ["y", "state_out"])
-_forward = _call.traceable("scan_forward", _launch_forward)
-_backward = _call.traceable("scan_backward", _launch_backward)
-_op, _token_op = torch.ops.spear_btp.scan_forward, torch.ops.spear_btp.scan_step
+_op, _backward_op, _token_op = torch.ops.spear_btp.scan_forward, torch.ops.spear_btp.scan_backward, torch.ops.spear_btp.scan_step
 
 
 class _SelectiveScan(torch.autograd.Function):
@@ -206,7 +204,7 @@ class _SelectiveScan(torch.autograd.Function):
         y = x.new_empty((Bsz, L, dim))
         state = x.new_empty((Bsz, dim, N), dtype=torch.float32) if want_state else None
         checkpoints = x.new_empty((Bsz, -(-L // _CHECKPOINT), dim, N), dtype=torch.float32)
-        _forward(x, delta, A, B, C, D, z, delta_bias, initial, lengths, y, state, checkpoints, softplus)
+        _op(x, delta, A, B, C, D, z, delta_bias, initial, lengths, y, state, checkpoints, softplus)
         ctx.save_for_backward(x, delta, A, B, C, D, z, delta_bias, lengths, checkpoints)
         ctx.softplus = softplus
         ctx.set_materialize_grads(False)
@@ -228,8 +226,8 @@ class _SelectiveScan(torch.autograd.Function):
         dB, dC = (x.new_empty(B.shape) for _ in range(2))
         dparams = x.new_empty(_parameter_floats(dim, N), dtype=torch.float32)
         dinitial = x.new_empty((Bsz, dim, N), dtype=torch.float32) if need[8] else None
-        _backward(x, delta, A, B, C, D, z, delta_bias, lengths, checkpoints, dy, dstate, dx, ddelta, dparams, dB, dC, dz, dinitial,
-                  ctx.softplus)
+        _backward_op(x, delta, A, B, C, D, z, delta_bias, lengths, checkpoints, dy, dstate, dx, ddelta, dparams, dB, dC, dz, dinitial,
+                     ctx.softplus)
         dA, dD, dbias = dparams[:dim * N].view(dim, N), dparams[dim * N:dim * (N + 1)], dparams[dim * (N + 1):dim * (N + 2)]
         grads = (dx, ddelta, dA, dB, dC, None if D is None else dD, dz, None if delta_bias is None else dbias, dinitial)
         return (*(g if n else None for g, n in zip(grads, need)), None, None, None)
