@@ -2,7 +2,8 @@
 //
 //   h = x + residual          r = 1 / sqrt(mean(h^2) + eps)          y = h r weight
 //
-// forward: one pass; a row stays in registers between the sum of its squares and its output.  y leaves in x's type or as
+// forward: one pass; a row stays in registers between the sum of its squares and its output (up to 8192 columns some instances spill
+// 40 to 220 bytes of it, float or with a float residual; the backward of more than 8192 columns spills 850 to 920).  y leaves in x's type or as
 // e4m3 with scale = max|y| / 448 over the row or over 128 columns (scale 1 where that is 0 or no number).  The norm
 // is taken of the unrounded sum; h is rounded once, to the residual's type, as it is stored.
 // backward: with xhat = h r and g = weight dy,  dh = r (g - xhat mean(g xhat)) + dh_out;  dweight = sum over rows of dy xhat,
@@ -10,8 +11,10 @@
 //
 // Both are bound by memory: forward moves x, residual, y, h once; backward h, dy, dh_out in and the gradients out.  A CTA takes rows in
 // turn and fetches the next one, as it lies in memory, while it works on one.
-// Measured (copy rate of this device type: 6.57 TB/s): 16384 x 2048 bfloat16 with a float residual forward 62 us (6.5 TB/s),
-// backward 93 us (5.8 TB/s); 16384 x 4096 in 8 bits with block scales 90 us (5.2 TB/s; 128 us with a CTA per row and nothing ahead).
+// Measured with a cold L2 (copy rate of this device type: 6.57 TB/s): 16384 x 2048 bfloat16 with a float residual forward 67 us
+// (6.0 TB/s), backward 93 us (5.8 TB/s); 16384 x 4096 in 8 bits with block scales 93 us (5.1 TB/s; 128 us with a CTA per row and nothing
+// ahead).  That form is nearer to the issue rate than to memory (ncu: 68 % of the SM's throughput); it has one barrier per row, for the
+// sum.  4096 rows of 16384 columns: forward 0.6 to 0.9 of the copy rate, backward 210 to 310 us (0.4 to 0.6), for its spills.
 // A group of `TPR` threads owns a row, thread i of it the runs of 8 columns i, i + TPR, ...: 16-byte accesses at 16 bits,
 // and the 128 columns that share a scale always lie in 16 neighbouring lanes.
 #pragma once
@@ -161,9 +164,15 @@ __device__ __forceinline__ void load_weight(f32x2 (&w)[kPairs], const void* base
   }
 }
 
+// CTAs of 512 threads that share an SM.  Two take 64 registers per thread; a row of four runs that is float or comes with a residual, and
+// the one fetched ahead, need up to 128 and spilled up to 984 bytes: 4096 x 16384 bfloat16 with a float residual 237 us against 142,
+// float 158 against 95, float with a residual 327 against 213; bfloat16 alone takes 52 with two and 56 with one.
+template <class T, int RES, int VPT>
+constexpr int kCtas = VPT == 4 && (RES != kNone || sizeof(T) == 4) ? 1 : 2;
+
 // WARP_ROW: a row per warp (4 in a CTA of 128 threads); otherwise a row per CTA.
 template <class T, int RES, int OUT, int VPT, bool WARP_ROW>
-__global__ void __launch_bounds__(WARP_ROW ? 128 : kMaxRowThreads, 2) rms_norm_forward_kernel(const FwdParams p) {
+__global__ void __launch_bounds__(WARP_ROW ? 128 : kMaxRowThreads, kCtas<T, RES, VPT>) rms_norm_forward_kernel(const FwdParams p) {
   using R = typename std::conditional<RES == kResF32, float, T>::type;
   __shared__ float s_sum[2][32];
   __shared__ unsigned s_max[2][32];

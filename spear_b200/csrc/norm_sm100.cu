@@ -18,14 +18,14 @@ struct Shape {
   int threads;
   int grid;
 };
-Shape row_shape(long long rows, int dim, int sms) {
+Shape row_shape(long long rows, int dim, int sms, bool heavy) {
   Shape s{};
   s.vpt = dim > kMaxRowThreads * kRun * 2 ? 4 : dim > (rows < sms ? 4096 : 2048) ? 2 : 1;
   const int threads = (dim + kRun * s.vpt - 1) / (kRun * s.vpt);
   s.warp_row = threads <= 32;
   s.threads = s.warp_row ? 128 : (threads + 31) / 32 * 32;
   // as many CTAs as 1024 threads per SM give; each takes rows in turn and fetches one ahead
-  const long long want = s.warp_row ? (rows + 3) / 4 : rows, cap = static_cast<long long>(sms) * (1024 / s.threads);
+  const long long want = s.warp_row ? (rows + 3) / 4 : rows, cap = static_cast<long long>(sms) * (s.vpt == 4 && heavy ? 1 : 1024 / s.threads);  // see kCtas
   s.grid = static_cast<int>(want < cap ? want : cap);
   return s;
 }
@@ -102,7 +102,7 @@ int btp_sm100_rms_norm_forward(const void* x, const void* residual, const void* 
   int dev;
   DeviceInfo info;
   if ((rc = device_info(&dev, &info))) return rc;
-  const Shape s = row_shape(rows, dim, info.sms);
+  const Shape s = row_shape(rows, dim, info.sms, residual || dtype == BTP_DTYPE_F32);
   const int e = elem_bytes(dtype), er = residual ? elem_bytes(residual_dtype) : e;
   FwdParams p{};
   p.x = x; p.residual = residual; p.weight = weight; p.y = y; p.h = h; p.rstd = rstd; p.scale = scale;
