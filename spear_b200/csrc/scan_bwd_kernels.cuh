@@ -14,8 +14,9 @@
 // and over sequences go through a buffer and a second kernel in a fixed order: the same call gives the same bits.
 //
 // Bound: the two-wide multiply-adds (about 13 per token, channel and state) and two exponentials.  Measured at 8 x 2048 tokens x 2048
-// channels x 16 states, bfloat16: 800 us, and 180 us for the carries of its 16 chunks; 385 instructions per token and warp at 0.44 per
-// cycle with the two warps that registers (255) and shared memory leave a scheduler.
+// channels x 16 states, bfloat16: 816 us, and 169 us for the carries of its 16 chunks; 385 instructions per token and warp at 0.44 per
+// cycle with the two warps that registers and shared memory leave a scheduler.  A thread would want more than the 255 registers that
+// there are: 170 to 260 bytes of it spill.  In float a tile takes 144 KB (120 with 8 or 64 states), so one CTA fits: 1317 and 221 us.
 #pragma once
 
 #include "scan_kernels.cuh"

@@ -10,7 +10,8 @@
 // lanes of its channels by warp exchanges, which also bring the partial sums of y back to it for D x, gate and store.  Nothing but
 // the raw rows goes through shared memory.
 // Measured against lanes of 4 channels x 4 states with step sizes and y staged in shared memory (8 x 2048 tokens x 2048
-// channels x 16 states): 298 us against 520; 2 channels x 8 states 372 (half the warps), 2 x 2 states 343 (more exchanges).
+// channels x 16 states): 298 us against 520; 2 channels x 8 states 372 (half the warps), 2 x 2 states 343 (more exchanges).  Of today's
+// 300 us 4 are for step sizes of full accuracy.
 //
 // Bound: one exponential per (token, channel, state) on the special-function unit, 16 per clock and SM: 119 us for those 5.4e8.  At
 // that shape a scheduler has two warps and issues half of the time; with the tokens split 16 times (many warps) the same kernel
@@ -18,7 +19,7 @@
 // pipe was slower (the instructions it adds count more).
 //
 // Few channels or sequences: the tokens are split over `splits` chunks.  A first kernel runs each chunk from state zero and
-// keeps its last state and its sum of step sizes (the product of its decays is exp(A times that sum), one exponential); the second
+// keeps its last state and its sum of step sizes (the product of its decays is exp(A times that sum), see over_chunk); the second
 // combines the chunks before its own in order and runs its chunk from there.  That doubles the exponentials, so the rule in
 // scan_sm100.cu splits only where warps are missing.
 #pragma once

@@ -41,7 +41,8 @@ Split split_tokens(long long batch, int L, int dim, int N, int sms) {
 
 // The same for the backward, whose CTAs of four warps (two per SM: registers and shared memory) take about 2.6 times as long per token as
 // a pass for the carries, which splitting adds.  Measured at 8 x 2048 tokens x 2048 channels x 16 states, main pass and carries: one
-// chunk 1373 us, 2 chunks 875 + 196, 4 chunks 877 + 167, 16 chunks (the rule's choice) 800 + 180.
+// chunk 1373 us, 2 chunks 875 + 196, 4 chunks 877 + 167, 16 chunks (the rule's choice) 800 + 180, all in bfloat16.  In float one CTA
+// fits an SM, which the rule does not take into account.
 Split split_backward(long long batch, int L, int dim, int N, int sms) {
   const int sg = state_groups(N), wc = 128 / sg, cw = (sg == 2 ? 2 : 4) * wc;
   const long long ctas = batch * ((dim + cw - 1) / cw), warps = batch * ((dim + wc - 1) / wc);

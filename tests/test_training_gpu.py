@@ -211,3 +211,29 @@ def test_on_a_side_stream():
         got = torch.autograd.grad(m(u).square().sum(), params)
     torch.cuda.current_stream().wait_stream(side)
     assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_threads_at_once():
+    """Passes on four threads, each on a stream of its own, among them the first ones of their thread."""
+    import threading
+
+    fn, args = conv()
+    ready = torch.cuda.Event()
+    ready.record()
+    got = [None] * 4
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        stream.wait_event(ready)
+        with torch.cuda.stream(stream):
+            for _ in range(50):
+                got[i] = grads(fn, args, list(args))
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    want = grads(fn, args, list(args))
+    assert all(torch.equal(g[n], want[n]) for g in got for n in args)
