@@ -14,7 +14,8 @@
 // Measured with a cold L2 (copy rate of this device type: 6.57 TB/s): 16384 x 2048 bfloat16 with a float residual forward 67 us
 // (6.0 TB/s), backward 93 us (5.8 TB/s); 16384 x 4096 in 8 bits with block scales 93 us (5.1 TB/s; 128 us with a CTA per row and nothing
 // ahead).  That form is nearer to the issue rate than to memory (ncu: 68 % of the SM's throughput); it has one barrier per row, for the
-// sum.  4096 rows of 16384 columns: forward 0.6 to 0.9 of the copy rate, backward 210 to 310 us (0.4 to 0.6), for its spills.
+// sum.  4096 rows of 16384 columns: forward 0.76 to 0.87 of the copy rate, in 8 bits 0.4 to 0.65; backward 210 to 310 us (0.3 to
+// 0.65), for its spills.
 // A group of `TPR` threads owns a row, thread i of it the runs of 8 columns i, i + TPR, ...: 16-byte accesses at 16 bits,
 // and the 128 columns that share a scale always lie in 16 neighbouring lanes.
 #pragma once

@@ -120,4 +120,9 @@ def training(*tensors) -> bool:
     return _compiling() or (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors))
 
 
+def no_gradient(lib: torch.library.Library, name: str) -> None:
+    """The op is no step of autograd's: it runs as it is under any gradient mode, and what it writes does not require grad."""
+    lib.impl(name, torch.library.fallthrough_kernel, "Autograd")
+
+
 native = _lib.native

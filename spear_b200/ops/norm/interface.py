@@ -21,7 +21,6 @@ __all__ = ["rms_norm", "rms_norm_8bit", "F8_MAX", "SCALE_BLOCK", "MAX_DIM"]
 F8_MAX = 448.0     # largest e4m3 magnitude
 SCALE_BLOCK = 128  # columns that share a scale in the blockwise form
 MAX_DIM = 16384
-_OUT = {None: 1, SCALE_BLOCK: 2}
 
 
 def _check(what, x, weight, residual, eps) -> int:
@@ -69,17 +68,34 @@ def _launch_forward(x, residual, weight, y, h, rstd, eps, scale=None, out_mode=0
 
 
 def _op_forward(x: torch.Tensor, residual: Optional[torch.Tensor], weight: Optional[torch.Tensor], y: torch.Tensor,
-                h: Optional[torch.Tensor], rstd: Optional[torch.Tensor], eps: float, scale: Optional[torch.Tensor] = None,
-                out_mode: int = 0) -> None:
+                h: Optional[torch.Tensor], rstd: Optional[torch.Tensor], eps: float) -> None:
     what = "spear_btp::rms_norm_forward"
     index = _check(what, x, weight, residual, eps)
+    n = x.numel()
+    _check_h(what, residual, h)
+    _call.buffers(what, index, (y, "y", n, x.dtype), (rstd, "rstd", n // x.shape[-1], torch.float32),
+                  (h, "h", n, x.dtype if residual is None else residual.dtype))
+    _launch_forward(_rows(x), None if residual is None else _rows(residual), _call.dense(weight), y, h, rstd, eps)
+
+
+def _op_8bit(x: torch.Tensor, residual: Optional[torch.Tensor], weight: Optional[torch.Tensor], q: torch.Tensor,
+             h: Optional[torch.Tensor], scale: torch.Tensor, eps: float, blocks: bool) -> None:
+    what = "spear_btp::rms_norm_8bit"
+    index = _check(what, x, weight, residual, eps)
     n, dim = x.numel(), x.shape[-1]
-    blocks = {0: 0, 1: 1, 2: -(-dim // SCALE_BLOCK)}.get(out_mode)
-    if blocks is None or (blocks and scale is None) or (residual is not None and h is None):
-        raise ValueError(f"{what}: out_mode must be 0, or 1 or 2 with a scale, and a residual comes with h")
-    _call.buffers(what, index, (y, "y", n, torch.float8_e4m3fn if out_mode else x.dtype), (rstd, "rstd", n // dim, torch.float32),
-                  (h, "h", n, x.dtype if residual is None else residual.dtype), (scale, "scale", n // dim * blocks, torch.float32))
-    _launch_forward(_rows(x), None if residual is None else _rows(residual), _call.dense(weight), y, h, rstd, eps, scale, out_mode)
+    _check_h(what, residual, h)
+    _call.buffers(what, index, (q, "q", n, torch.float8_e4m3fn), (scale, "scale", n // dim * (-(-dim // SCALE_BLOCK) if blocks else 1), torch.float32),
+                  (h, "h", n, x.dtype if residual is None else residual.dtype))
+    _launch_8bit(_rows(x), None if residual is None else _rows(residual), _call.dense(weight), q, h, scale, eps, blocks)
+
+
+def _check_h(what, residual, h) -> None:
+    if residual is not None and h is None:
+        raise ValueError(f"{what}: a residual comes with h")
+
+
+def _launch_8bit(x, residual, weight, q, h, scale, eps, blocks) -> None:
+    _launch_forward(x, residual, weight, q, h, None, eps, scale, 2 if blocks else 1)
 
 
 def _op_backward(h: torch.Tensor, weight: Optional[torch.Tensor], dy: torch.Tensor, dh: Optional[torch.Tensor], rstd: torch.Tensor,
@@ -115,8 +131,10 @@ def _fake(*args) -> None:
     return None
 
 
-_iface._register(_iface._LIB, "spear_btp", "rms_norm_forward", _op_forward, _fake, ["y", "h", "rstd", "scale"])
+_iface._register(_iface._LIB, "spear_btp", "rms_norm_forward", _op_forward, _fake, ["y", "h", "rstd"])
 _iface._register(_iface._LIB, "spear_btp", "rms_norm_backward", _op_backward, _fake, ["dx", "dresidual", "dweight"])
+_iface._register(_iface._LIB, "spear_btp", "rms_norm_8bit", _op_8bit, _fake, ["q", "h", "scale"])
+_call.no_gradient(_iface._LIB, "rms_norm_8bit")
 _op, _backward_op = torch.ops.spear_btp.rms_norm_forward, torch.ops.spear_btp.rms_norm_backward
 
 
@@ -197,7 +215,7 @@ def rms_norm_8bit(x: torch.Tensor, weight: torch.Tensor | None = None, residual:
         [..., ceil(D / 128)] with y = q * scale; scale = max|y| / 448, or 1 where that is NaN or below 1e-37
         (a row of zeros).
     """
-    if block not in _OUT:
+    if block not in (None, SCALE_BLOCK):
         raise ValueError(f"rms_norm_8bit: block must be None or {SCALE_BLOCK} (got {block})")
     _check("rms_norm_8bit", x, weight, residual, eps)
     weight = weight if weight is None or weight.is_contiguous() else weight.contiguous()
@@ -205,6 +223,6 @@ def rms_norm_8bit(x: torch.Tensor, weight: torch.Tensor | None = None, residual:
     q = torch.empty_like(x, dtype=torch.float8_e4m3fn, memory_format=torch.contiguous_format)
     scale = x.new_empty(x.shape[:-1] if block is None else (*x.shape[:-1], -(-x.shape[-1] // SCALE_BLOCK)), dtype=torch.float32)
     h = None if residual is None else torch.empty_like(residual, memory_format=torch.contiguous_format)
-    launch = _op if _call.recorded(x, weight, residual) else _launch_forward
-    launch(x2, None if residual is None else _rows(residual), weight, q, h, None, float(eps), scale, _OUT[block])
+    launch = torch.ops.spear_btp.rms_norm_8bit if _call.recorded(x, weight, residual) else _launch_8bit
+    launch(x2, None if residual is None else _rows(residual), weight, q, h, scale, float(eps), block is not None)
     return (q, scale) if h is None else (q, scale, h)

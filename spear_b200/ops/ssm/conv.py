@@ -164,6 +164,7 @@ def _fake(*args) -> None:
 _iface._register(_iface._LIB, "spear_btp", "causal_conv_forward", _op_forward, _fake, ["y", "state"])
 _iface._register(_iface._LIB, "spear_btp", "causal_conv_backward", _op_backward, _fake, ["dx", "dweight", "dbias", "dinitial"])
 _iface._register(_iface._LIB, "spear_btp", "causal_conv_step", _op_step, _fake, ["y", "state_out"])
+_call.no_gradient(_iface._LIB, "causal_conv_step")
 _op, _backward_op, _token_op = (torch.ops.spear_btp.causal_conv_forward, torch.ops.spear_btp.causal_conv_backward,
                                 torch.ops.spear_btp.causal_conv_step)
 

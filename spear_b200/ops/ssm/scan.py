@@ -191,6 +191,7 @@ def _fake(*args) -> None:
 _iface._register(_iface._LIB, "spear_btp", "scan_forward", _op_forward, _fake, ["y", "state", "checkpoints"])
 _iface._register(_iface._LIB, "spear_btp", "scan_backward", _op_backward, _fake, ["dx", "ddelta", "dparams", "dB", "dC", "dz", "dinitial"])
 _iface._register(_iface._LIB, "spear_btp", "scan_step", _op_step, _fake, ["y", "state_out"])
+_call.no_gradient(_iface._LIB, "scan_step")
 _op, _backward_op, _token_op = torch.ops.spear_btp.scan_forward, torch.ops.spear_btp.scan_backward, torch.ops.spear_btp.scan_step
 
 

@@ -16,7 +16,7 @@ from spear_b200.ops.norm import rms_norm, rms_norm_8bit
 from spear_b200.ops.ssm import causal_conv, causal_conv_step, selective_scan, selective_scan_step
 
 N = torch.randn
-OUTPUTS = {"rms_norm_forward": ("y", "h", "rstd", "scale"), "rms_norm_backward": ("dx", "dresidual", "dweight"),
+OUTPUTS = {"rms_norm_forward": ("y", "h", "rstd"), "rms_norm_8bit": ("q", "h", "scale"), "rms_norm_backward": ("dx", "dresidual", "dweight"),
            "causal_conv_forward": ("y", "state"), "causal_conv_backward": ("dx", "dweight", "dbias", "dinitial"),
            "causal_conv_step": ("y", "state_out"), "scan_forward": ("y", "state", "checkpoints"),
            "scan_backward": ("dx", "ddelta", "dparams", "dB", "dC", "dz", "dinitial"), "scan_step": ("y", "state_out")}
@@ -25,7 +25,7 @@ OUTPUTS = {"rms_norm_forward": ("y", "h", "rstd", "scale"), "rms_norm_backward":
 CALLS = {
     "norm": ("rms_norm_forward", lambda x, w: rms_norm(x, w), lambda: (N(4, 8), N(8))),
     "norm residual": ("rms_norm_forward", lambda x, w, r: rms_norm(x, w, r), lambda: (N(2, 4, 8), N(8), N(2, 4, 8))),
-    "norm 8 bits": ("rms_norm_forward", lambda x, w: tuple(t.float() for t in rms_norm_8bit(x, w, block=128)), lambda: (N(4, 8), N(8))),
+    "norm 8 bits": ("rms_norm_8bit", lambda x, w: tuple(t.float() for t in rms_norm_8bit(x, w, block=128)), lambda: (N(4, 8), N(8))),
     "conv": ("causal_conv_forward", lambda x, w: causal_conv(x, w, return_state=True), lambda: (N(2, 5, 8), N(8, 4))),
     "conv token": ("causal_conv_step", lambda x, s, w: causal_conv_step(x, s, w), lambda: (N(2, 8), N(2, 3, 8), N(8, 4))),
     "scan": ("scan_forward", lambda x, d, A, B, C: selective_scan(x, d, A, B, C, return_state=True),
@@ -44,6 +44,7 @@ def stand_in(monkeypatch):
     def kernel(name):
         schema = getattr(torch.ops.spear_btp, name).default._schema
 
+        @torch.no_grad()
         def run(*args, **kw):
             runs[name] += 1
             given = {a.name: v for a, v in zip(schema.arguments, args)} | kw
@@ -179,8 +180,9 @@ def test_recorded_ops_check_what_they_are_given(monkeypatch):
     monkeypatch.setattr(_call, "query", lambda *a: 4)
     monkeypatch.setattr(_call, "on_gpu", lambda what, first, *others: first.get_device())
     E = torch.empty
-    x, w, y, rstd = N(4, 8), N(8), E(4, 8), E(4)
+    x, w, y, rstd, q = N(4, 8), N(8), E(4, 8), E(4), E(4, 8).to(torch.float8_e4m3fn)
     norm._op_forward(x, None, w, y, None, rstd, 1e-6)
+    norm._op_8bit(x, None, w, q, None, E(4), 1e-6, True)
     norm._op_backward(x, w, y, None, rstd, E(4, 8), None, E(8))
     conv._op_forward(N(2, 5, 8), N(8, 4), None, None, None, E(2, 5, 8), None, False)
     conv._op_backward(N(2, 5, 8), N(8, 4), None, None, None, N(2, 5, 8), None, E(2, 5, 8), E(8, 4), None, None, False)
@@ -191,15 +193,16 @@ def test_recorded_ops_check_what_they_are_given(monkeypatch):
     scan._op_backward(*tokens, None, *back())
     one = (N(2, 8), N(2, 8), N(8, 4), N(2, 4), N(2, 4))
     scan._op_step(*one, E(2, 8, 4), None, None, None, E(2, 8), E(2, 8, 4), False)
-    assert len(called) == 8
+    assert len(called) == 9
     bad = [
         lambda: norm._op_forward(x, None, w, E(3, 8), None, rstd, 1e-6),
         lambda: norm._op_forward(x, None, w, E(8, 4).t(), None, rstd, 1e-6),
         lambda: norm._op_forward(x, None, w, y, None, E(3), 1e-6),
         lambda: norm._op_forward(x, x, w, y, None, rstd, 1e-6),
         lambda: norm._op_forward(x, None, N(7), y, None, rstd, 1e-6),
-        lambda: norm._op_forward(x, None, w, y, None, rstd, 1e-6, None, 1),
-        lambda: norm._op_forward(x, None, w, y, None, rstd, 1e-6, E(4), 1),
+        lambda: norm._op_8bit(x, None, w, y, None, E(4), 1e-6, False),
+        lambda: norm._op_8bit(x, None, w, q, None, E(5), 1e-6, False),
+        lambda: norm._op_8bit(x, x, w, q, None, E(4), 1e-6, True),
         lambda: norm._op_backward(x, w, y, None, E(3), E(4, 8), None, E(8)),
         lambda: norm._op_backward(x, None, y, None, rstd, E(4, 8), None, E(8)),
         lambda: norm._op_backward(x, w, y, E(4, 8).half(), rstd, E(4, 8), None, E(8)),
@@ -220,7 +223,7 @@ def test_recorded_ops_check_what_they_are_given(monkeypatch):
     for call in bad:
         with pytest.raises(ValueError):
             call()
-    assert len(called) == 8
+    assert len(called) == 9
     # strides that the kernels do not read: the op brings them into order itself
     seen = []
     monkeypatch.setattr(_call, "call", lambda name, index, *args: seen.append(args))
@@ -252,3 +255,21 @@ def test_recorded_ops_without_tokens(monkeypatch):
     dw = E(8)
     norm._op_backward(E(0, 8), N(8), E(0, 8), None, E(0), E(0, 8), None, dw)
     assert (dw == 0).all()
+
+
+@pytest.mark.parametrize("case", ["norm 8 bits", "conv token", "scan token"])
+def test_forms_without_gradient_have_none_when_recorded(stand_in, case, recwarn):
+    _, fn, make = CALLS[case]
+    args = [torch.nn.Parameter(t) for t in make()]
+    seen = []
+
+    def run(*args):
+        out = tensors(fn(*args))
+        seen.extend(t.requires_grad for t in out)
+        return out
+
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        fake = tensors(fn(*[torch.nn.Parameter(torch.empty(t.shape)) for t in args]))
+    traced = make_fx(run)(*args)
+    assert not any(seen) and not any(t.requires_grad for t in fake + tensors(traced(*args)))
+    assert not [w for w in recwarn.list if "autograd kernel was not registered" in str(w.message)]
