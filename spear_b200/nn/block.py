@@ -18,7 +18,8 @@ class MixerBlock(nn.Module):
     """``out, h = block(x, residual)`` with ``residual=None`` for the first block.
 
     Args:
-        mixer: a module [B, L, dim] -> [B, L, dim] (Phalanx or SelectiveSSM).
+        mixer: a module [B, L, dim] -> [B, L, dim] (Phalanx or SelectiveSSM).  ``prefill`` and ``step`` need one that has them
+            (SelectiveSSM).
         dim: width of the residual stream.
         eps: of the norm.
         dtype: of the norm's weight.
@@ -43,16 +44,23 @@ class MixerBlock(nn.Module):
         y, h = self._norm(x, residual)
         return self.mixer(y, **kwargs), h
 
+    def _streams(self, name: str):
+        if not hasattr(self.mixer, name):
+            raise TypeError(f"MixerBlock.{name}: {type(self.mixer).__name__} has no {name}")
+        return getattr(self.mixer, name)
+
     @torch.no_grad()
     def prefill(self, x: torch.Tensor, residual: torch.Tensor | None = None, state=None, lengths: torch.Tensor | None = None):
         """A prompt through a mixer that has ``prefill``: returns (out, h, state)."""
+        prefill = self._streams("prefill")
         y, h = self._norm(x, residual)
-        out, state = self.mixer.prefill(y, state, lengths)
+        out, state = prefill(y, state, lengths)
         return out, h, state
 
     @torch.no_grad()
     def step(self, x_t: torch.Tensor, residual: torch.Tensor | None, state, *, in_place: bool = False):
         """One token through a mixer that has ``step``: returns (out_t, h, state)."""
+        step = self._streams("step")
         y, h = self._norm(x_t, residual)
-        out, state = self.mixer.step(y, state, in_place=in_place)
+        out, state = step(y, state, in_place=in_place)
         return out, h, state

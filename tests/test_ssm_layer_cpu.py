@@ -70,3 +70,11 @@ def test_a_cast_layer_works_in_its_new_type(built, cast):
             layer(torch.randn(1, 4, 16, dtype=given))
         with pytest.raises(RuntimeError, match="no CPU path"):
             layer.step(torch.randn(1, 16, dtype=given), layer.empty_state(1))
+
+
+def test_a_mixer_that_cannot_stream_is_named_before_anything_runs():
+    block = MixerBlock(Phalanx(dim=64, length=32, dtype=torch.bfloat16), 64)
+    with pytest.raises(TypeError, match="Phalanx has no prefill"):
+        block.prefill(torch.randn(1, 32, 64))
+    with pytest.raises(TypeError, match="Phalanx has no step"):
+        block.step(torch.randn(1, 64), None, None)
