@@ -109,8 +109,11 @@ def native():
         with _lock:
             if _module is None:
                 spec = importlib.util.spec_from_file_location("btp_torch", MODULE_PATH)
-                module = importlib.util.module_from_spec(spec)
-                spec.loader.exec_module(module)
+                try:
+                    module = importlib.util.module_from_spec(spec)
+                    spec.loader.exec_module(module)
+                except ImportError as e:  # built against another torch or Python
+                    raise BtpLibraryError(f"{MODULE_PATH} does not load ({e}); rebuild it with `python -m spear_b200.build --force`.") from e
                 _module = module
     return _module
 

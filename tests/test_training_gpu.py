@@ -237,3 +237,22 @@ def test_threads_at_once():
         t.join()
     want = grads(fn, args, list(args))
     assert all(torch.equal(g[n], want[n]) for g in got for n in args)
+
+
+def test_one_tensor_for_two_arguments():
+    from spear_b200.ops.norm import rms_norm
+    from spear_b200.ops.ssm import selective_scan
+
+    x, w, up = N(6, 72), N(72), N(6, 72)
+    a, b = x.clone().requires_grad_(True), x.clone().requires_grad_(True)
+    apart = torch.autograd.grad(list(rms_norm(a, w, b)), [a, b], [up, up])
+    both, = torch.autograd.grad(list(rms_norm(a, w, a)), a, [up, up])
+    assert torch.equal(both, apart[0] + apart[1])
+    sum(o.sum() for o in rms_norm(a, w, b)).backward()
+    assert torch.equal(a.grad, b.grad) and a.grad.data_ptr() != b.grad.data_ptr()
+    x, m, A = N(2, 37, 24), N(2, 37, 5), -torch.rand(24, 5, device="cuda")
+    leaf = lambda t: t.clone().requires_grad_(True)
+    x1, x2, m1, m2 = leaf(x), leaf(x), leaf(m), leaf(m)
+    apart = torch.autograd.grad(selective_scan(x1, x2, A, m1, m2, delta_softplus=True).sum(), [x1, x2, m1, m2])
+    both = torch.autograd.grad(selective_scan(x1, x1, A, m1, m1, delta_softplus=True).sum(), [x1, m1])
+    assert torch.equal(both[0], apart[0] + apart[1]) and torch.equal(both[1], apart[2] + apart[3])
