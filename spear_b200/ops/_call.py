@@ -14,7 +14,6 @@ from .. import _lib
 
 TAG = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16, torch.float32: _lib.DTYPE_F32}
 
-
 # a call has CUDA tensors, so CUDA is initialised and the plain lookup will do
 _current_device, _raw_stream = getattr(torch._C, "_cuda_getDevice", _native._current_device), _native._raw_stream
 _fns: dict = {}  # the library's functions by name, looked up once
@@ -101,10 +100,8 @@ def pass_on(into: torch.Tensor | None, given: torch.Tensor | None) -> None:
 
 
 _modes, _tracing = torch._C._len_torch_dispatch_stack, torch._C._is_tracing
-_PLAIN = frozenset((torch.Tensor, torch.nn.Parameter, type(None)))
-
-
 _compiling = torch.compiler.is_compiling
+_PLAIN = frozenset((torch.Tensor, torch.nn.Parameter, type(None)))
 
 
 def recorded(*tensors) -> bool:

@@ -124,3 +124,17 @@ def test_functional_transforms_are_refused():
                  lambda: torch.vmap(lambda s: selective_scan_step(x[0], x[0], -w, x[0, :, :4], x[0, :, :4], s))(N(2, 5, 24, 4))):
         with pytest.raises((RuntimeError, NotImplementedError)):
             call()
+
+
+@pytest.mark.parametrize("case", ["norm", "conv", "conv padded", "scan"])
+@pytest.mark.filterwarnings("ignore")
+def test_jit_trace_of_a_training_pass(case):
+    """Traced with inputs that require grad: the outputs and the gradients of the calls themselves, on other inputs."""
+    fn, make = calls()[case]
+    leaves = lambda: [a.requires_grad_(True) for a in make(70)]
+    traced = torch.jit.trace(fn, leaves(), check_trace=False)
+    args = leaves()
+    got, want = ([o] if torch.is_tensor(o) else list(o) for o in (traced(*args), fn(*args)))
+    ups = [torch.randn_like(o) for o in want]
+    assert same(got, want)
+    assert same(torch.autograd.grad(got, args, ups), torch.autograd.grad(want, args, ups))
